@@ -245,9 +245,10 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 // disjoint from the current tile's ds_reads, so it put s_waitcnt vmcnt(3..0) in front of this tile's
 // QK^T MFMAs -- each tile waited for the NEXT tile's K / V to land and the prefetch hid nothing.  The
 // kernel orders the DMA itself: vmcnt(0) + barrier before a buffer is read.  M0 carries the LDS base
-// and is declared clobbered, so the compiler saves / restores any M0 value of its own around it.
+// and is declared clobbered, so the compiler saves / restores any M0 value of its own around it; the
+// s_nop is gfx9's wait state between the write of M0 and the LDS-DMA that reads it.
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, uint32_t lds_base, uint32_t voff, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(lds_base), "v"(voff), "s"(rs), "s"(soff)
                : "memory", "m0");

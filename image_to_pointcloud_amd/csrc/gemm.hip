@@ -230,15 +230,17 @@ struct ResQ {
   int full;
 };
 
+// (s_nop: gfx9 wants a wait state between a scalar write of M0 and the LDS-DMA that takes its base from it;
+// the compiler does not look into the asm for that hazard)
 __device__ __forceinline__ void dma16_gemm(__amdgpu_buffer_rsrc_t rs, uint32_t lds_base, uint32_t voff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(lds_base), "v"(voff), "s"(rs), "s"(0u)
                : "memory", "m0");
 }
 // the same with sc1 (agent scope: per-call row shifts written by the launch before)
 __device__ __forceinline__ void dma16_gemm_sc1(__amdgpu_buffer_rsrc_t rs, uint32_t lds_base, uint32_t voff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen sc1 lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen sc1 lds"
                :
                : "s"(lds_base), "v"(voff), "s"(rs), "s"(0u)
                : "memory", "m0");

@@ -80,9 +80,10 @@ __device__ __forceinline__ void hlerp(const uint8_t* s_row, int p0, int p1, int 
 // not see these writes, so it inserts no waits for them (it would put a vmcnt(0) -- which also
 // drains the weight loads meant to stay in flight -- in front of every LDS access it cannot prove
 // disjoint); the kernel orders them itself with a counted vmcnt and a barrier.  M0 carries the LDS
-// base and is declared clobbered (the compiler keeps any M0 value of its own around it).
+// base and is declared clobbered (the compiler keeps any M0 value of its own around it); the
+// s_nop is gfx9's wait state between the write of M0 and the LDS-DMA that reads it.
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, uint32_t lds_base, uint32_t voff, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(lds_base), "v"(voff), "s"(rs), "s"(soff)
                : "memory", "m0");

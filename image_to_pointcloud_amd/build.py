@@ -29,6 +29,9 @@ SOURCES = [
     "gemm.hip",
     "misc.hip",
     "attention.hip",
+    "attention_packed.hip",
+    "layernorm_train.hip",
+    "gelu_fp8.hip",
     "preprocess.hip",
     "sor.hip",
     "head.hip",
@@ -40,7 +43,7 @@ SOURCES = [
     "comm.cpp",
     "writers.cpp",
 ]
-HEADERS = ["common.h", "mx.h", "../../include/i2pc.h"]
+HEADERS = ["attn_tile.h", "common.h", "mx.h", "../../include/i2pc.h"]
 
 
 def hipcc() -> str:

@@ -13,6 +13,7 @@
 //   O^T[d][q]  += V^T . P^T    (A = V^T rows from LDS, B = P straight from the
 //                               S accumulators, converted to bf16 in place)
 // so the online-softmax max/sum are lane-local plus one cross-half exchange.
+#include "attn_tile.h"
 #include "common.h"
 #include "mx.h"
 
@@ -23,23 +24,10 @@
 namespace i2pc {
 namespace attn {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef uint16_t bf16_t;
-
 constexpr int kQ = 128;   // query rows per workgroup
-constexpr int kKV = 64;   // keys per tile
-constexpr int kTileBytes = kKV * 64 * 2;   // 8 KiB (K tile and V^T tile each)
 
 __device__ __forceinline__ void glds16(const void* src, void* lds_base) {
   __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)(lds_base), 16, 0, 0);
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-  // one v_cvt_pk_bf16_f32 for the pair (RNE), no shift/or repacking
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
 }
 
 // V^T image: row d (128 B = 64 keys), 8-byte units of 4 keys swizzled by (d >> 1) & 15.
@@ -230,37 +218,6 @@ __global__ __launch_bounds__(256, 2) void k_attention(const bf16_t* __restrict__
 //  * key masking only on the last tile, and a last tile of <= 32 keys computes one
 //    32-key half (T = 577 = 9*64 + 1: the tail was a whole wasted 64-key tile);
 //  * waves whose 32 query rows are all beyond T skip the MFMA/softmax work.
-__device__ __forceinline__ int v_swz(int row) { return ((row >> 1) & 1) << 2; }
-// K image: 16-B chunk c of key row r at c ^ ((r >> 1) & 7).  A ds_read_b128 serves 16 lanes per LDS
-// cycle (lane groups {0-3,12-15,20-27}, {4-11,16-19,28-31} and their +32 twins); a group's 16 keys
-// fall into 8 even and 8 odd rows, the parity picks the 128-B half of the 256-B bank row, and
-// (r >> 1) & 7 is a bijection on each parity class of a group -- conflict-free.  The r & 7 swizzle of
-// r04 mapped keys 20-27 onto the chunks of keys 0-3 / 12-15: every K read was 2-way conflicted.
-__device__ __forceinline__ int k_swz(int row) { return (row >> 1) & 7; }
-
-typedef short v4s __attribute__((ext_vector_type(4)));
-
-// 16 B per lane global -> LDS at lds_base + 16 * lane (buffer_load ... lds), issued by inline asm.
-// Through __builtin_amdgcn_raw_ptr_buffer_load_lds the compiler sees an LDS write it cannot prove
-// disjoint from the current tile's ds_reads, so it put s_waitcnt vmcnt(3..0) in front of this tile's
-// QK^T MFMAs -- each tile waited for the NEXT tile's K / V to land and the prefetch hid nothing.  The
-// kernel orders the DMA itself: vmcnt(0) + barrier before a buffer is read.  M0 carries the LDS base
-// and is declared clobbered, so the compiler saves / restores any M0 value of its own around it; the
-// s_nop is gfx9's wait state between the write of M0 and the LDS-DMA that reads it.
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, uint32_t lds_base, uint32_t voff, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :
-               : "s"(lds_base), "v"(voff), "s"(rs), "s"(soff)
-               : "memory", "m0");
-}
-__device__ __forceinline__ uint32_t lds_addr(const void* p) {
-  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
-}
-
-__device__ __forceinline__ v4s tr_read(const uint8_t* p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(p));
-}
-
 // lazy != 0: skip the alpha exponential and the O / l rescale of a tile when no query row of the
 // wave raised its running max -- alpha would be exp2(0) = 1 exactly, so the skip is bit-exact
 // (the usual case after the first tiles: the max of a row settles early)

@@ -1,0 +1,904 @@
+// Softmax attention over packed sequences of different lengths, with its gradients (gfx950): head dim 64,
+// bf16 in and out, fp32 scores, statistics and sums; grouped heads, an optional causal mask, keys in a pack
+// or in the slabs of a cache.
+//
+//   S = scale Q K^T (masked), P = softmax(S), O = P V, lse = log(sum exp S)
+//   D = rowsum(dO O), dS = P (dO V^T - D), dV = P^T dO, dK = scale dS^T Q, dQ = scale dS K
+//
+// A packed row: the G = heads / kv_heads query heads that share a key head are G rows of one query position,
+// r = i G + g.  A tile of rows then reads its keys once for all of them, a causal tile's diagonal is G times
+// shorter, and one new token of 8 grouped heads is 8 rows, not 8 tiles of one.
+//
+// Lengths are read on the device: the grid is an upper bound that follows from the totals alone, and tile t
+// belongs to the last sequence b with floor(cu[b] G / tile) + b <= t (find_tile) -- a sequence then owns
+// at least ceil(its rows / tile) of these indexes, so no plan, copy or synchronisation precedes the launch.
+// Everything read through cu is held to the totals, so a bad cu gives wrong rows but no access out of range.
+#include "attn_tile.h"
+#include "common.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace i2pc {
+namespace attnp {
+
+using attn::bf16_t;
+using attn::bf16x8;
+using attn::f32x16;
+using attn::kKV;
+using attn::kTileBytes;
+using attn::lds_addr;
+using attn::pack_bf16;
+using attn::tr_read;
+using attn::v4s;
+
+constexpr int kRows = 128;       // packed rows of a workgroup: 4 waves x 32
+constexpr int kKeys = 64;        // keys of a dK / dV workgroup
+
+struct Args {
+  const bf16_t *q, *k, *v;
+  int64_t q_t, q_h, k_t, k_h, v_t, v_h;
+  bf16_t* out;
+  int64_t o_t, o_h;
+  float* lse;
+  const int32_t *cu_q, *cu_k, *k_lens;
+  int B, Tq, Tk, H, Hk, G, zero_tail, nsplit;
+  float c;                       // scale * log2(e)
+  float* part_o;                 // [nsplit][Hk][Tq * G][64], rows normalised
+  float* part_l;                 // [nsplit][Hk][Tq * G], log2(sum exp) or -inf
+  // backward
+  const bf16_t* dout;
+  int64_t d_t, d_h;
+  bf16_t *dq, *dk, *dv;
+  int64_t dq_t, dq_h, dk_t, dk_h, dv_t, dv_h;
+  float scale;
+  float *nlse, *ndelta;          // [H][Tq]: -lse / scale and -D
+};
+
+// The kernel's arguments, read again where they are used: for code that is hardly ever reached, so that its
+// pointers and strides do not occupy scalar registers throughout.
+__device__ __forceinline__ const Args& again() {
+  const Args* p = (const Args*)(const __attribute__((address_space(4))) void*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *p;
+}
+
+// ------------------------------------------------------------------ lookup of a tile
+__device__ __forceinline__ int cu_at(const int32_t* cu, int b, int total) {
+  return b == 0 ? 0 : min(max(cu[b], 0), total);
+}
+// The last sequence b < entries with floor(cu[b] * mult / tile) + b <= t, 64 candidates a step; `local` becomes
+// t's index within it.  (cu[b] * mult < 2^31: the host checks.)
+__device__ __forceinline__ int find_tile(const int32_t* cu, int total, int mult, int tile, int entries, int t, int lane,
+                                         int& local) {
+  int lo = 0, n = entries, first = 0;
+  while (n > 1) {
+    const int step = (n + 63) >> 6;
+    const int at = lane * step;
+    int f = INT_MAX;
+    if (at < n) f = cu_at(cu, lo + at, total) * mult / tile + lo + at;
+    const int cnt = __popcll(__ballot(f <= t));
+    if (cnt == 0) return -1;                     // not reached: f(0) = 0
+    first = __builtin_amdgcn_readlane(f, cnt - 1);
+    lo += (cnt - 1) * step;
+    n = min(step, n - (cnt - 1) * step);
+  }
+  local = t - first;
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+struct Seq {
+  int q0, lq, k0, lk;
+};
+__device__ __forceinline__ Seq sequence(const Args& a, int b) {
+  Seq s;
+  s.q0 = __builtin_amdgcn_readfirstlane(cu_at(a.cu_q, b, a.Tq));
+  s.lq = max(0, __builtin_amdgcn_readfirstlane(cu_at(a.cu_q, b + 1, a.Tq)) - s.q0);
+  s.k0 = __builtin_amdgcn_readfirstlane(cu_at(a.cu_k, b, a.Tk));
+  s.lk = max(0, __builtin_amdgcn_readfirstlane(cu_at(a.cu_k, b + 1, a.Tk)) - s.k0);
+  if (a.k_lens) s.lk = min(s.lk, max(0, __builtin_amdgcn_readfirstlane(a.k_lens[b])));
+  return s;
+}
+
+// ------------------------------------------------------------------ tiles in LDS
+// 16-B chunk c of row r at c ^ swz(r), for tiles that are read both by rows (ds_read_b128, the A operand of
+// S and dP) and transposed (ds_read_b64_tr_b16): a bijection of (r >> 1) & 7 whose lowest bit moves chunk
+// sets {0-3} / {4-7} onto each other, so that neither read has a bank conflict.
+__device__ __forceinline__ int swz(int row) {
+  const int x = (row >> 1) & 7;
+  return ((x & 1) << 2) | (x >> 1);
+}
+
+// 16 B (4 B) per lane global -> LDS.  Inline asm for the reason given at attn::dma16; the s_nop covers the wait
+// states of M0 (1) and of scalars that come from a lane read (5), which the compiler does not see in here.
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, uint32_t lds_base, uint32_t voff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds_base), "v"(voff), "s"(rs)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rs, uint32_t lds_base, uint32_t voff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(lds_base), "v"(voff), "s"(rs)
+               : "memory", "m0");
+}
+
+// A descriptor over `rows` rows of `pitch` elements from p (64 values of the last row): reads behind it give
+// zero.  The base is 64 bits and moves with the tile, so a sequence may span more than 4 GiB.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* p, int64_t pitch, int rows) {
+  const int64_t bytes = rows > 0 ? ((rows - 1) * pitch + 64) * 2 : 0;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)min(bytes, (int64_t)0x7fffffff), 0x00020000);
+}
+
+// one wave's quarter of a 64-row tile: 2 instructions of 8 rows x 128 B
+struct Stage {
+  uint32_t off[2];
+  __device__ __forceinline__ Stage(int wid, int lane, int64_t pitch) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int row = (wid * 2 + j) * 8 + (lane >> 3);
+      off[j] = (uint32_t)((row * pitch + ((lane & 7) ^ swz(row)) * 8) * 2);
+    }
+  }
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, const uint8_t* tile, int wid) const {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) dma16(rs, __builtin_amdgcn_readfirstlane(lds_addr(tile + (wid * 2 + j) * 1024)), off[j]);
+  }
+};
+
+__device__ __forceinline__ bf16x8 row_frag(const uint8_t* tile, int row, int s, int hh) {
+  return *reinterpret_cast<const bf16x8*>(tile + row * 128 + (((2 * s + hh) ^ swz(row)) << 4));
+}
+// columns 32 dt .. + 31 of rows base + {0-3, 8-11} + 4 (lane >> 5) as the A operand of a product over the rows
+__device__ __forceinline__ bf16x8 tr_frag(const uint8_t* tile, int base, int dt, int lane) {
+  const int tg = lane >> 4, tq = (lane >> 2) & 3, tp = lane & 3;
+  const int d0 = 32 * dt + 16 * (tg & 1) + 4 * tp, ch = d0 >> 3, within = (d0 & 7) * 2;
+  const int r0 = base + 4 * (tg >> 1) + tq, r1 = r0 + 8;
+  const v4s lo = tr_read(tile + r0 * 128 + ((ch ^ swz(r0)) << 4) + within);
+  const v4s hi = tr_read(tile + r1 * 128 + ((ch ^ swz(r1)) << 4) + within);
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+__device__ __forceinline__ bf16x8 p_frag(const uint32_t (&pk)[8], int s) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(bf16x8, u32x4{pk[4 * s], pk[4 * s + 1], pk[4 * s + 2], pk[4 * s + 3]});
+}
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ bool nonfinite(bf16x8 f) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 u = __builtin_bit_cast(u32x4, f);
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= (u[i] & 0x7f80u) == 0x7f80u || (u[i] & 0x7f800000u) == 0x7f800000u;
+  return bad;
+}
+
+// A matrix product multiplies a masked row by zero, which is NaN where that row holds an infinity or NaN.  Blocks
+// that are partly masked look for such values (`bad`); a wave that met one does its sums again at the end, a row of
+// K, V, Q or dO at a time and only with the rows that the mask leaves -- slow, and for such inputs only.
+__device__ __forceinline__ float dot_row(const bf16_t* row, const bf16x8 (&f)[4], int hh) {
+  float s = 0.f;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const bf16x8 x = *reinterpret_cast<const bf16x8*>(row + 16 * t + 8 * hh);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fmaf((float)x[j], (float)f[t][j], s);
+  }
+  return s + __shfl_xor(s, 32);
+}
+__device__ __forceinline__ void add_row(f32x16 (&acc)[2], float w, const bf16_t* row, int hh) {
+#pragma unroll
+  for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const uint2 x = *reinterpret_cast<const uint2*>(row + 32 * dt + 8 * g + 4 * hh);
+      const float e[4] = {__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u), __uint_as_float(x.y << 16),
+                          __uint_as_float(x.y & 0xffff0000u)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[dt][4 * g + i] = fmaf(w, e[i], acc[dt][4 * g + i]);
+    }
+}
+
+// 4 consecutive values a lane and register group of an accumulator, times f, as bf16: row[32 dt + 8 g + 4 hh ...]
+__device__ __forceinline__ void store_acc(bf16_t* row, const f32x16 (&o)[2], float f, int hh) {
+#pragma unroll
+  for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      uint2 w;
+      w.x = pack_bf16(o[dt][4 * g + 0] * f, o[dt][4 * g + 1] * f);
+      w.y = pack_bf16(o[dt][4 * g + 2] * f, o[dt][4 * g + 3] * f);
+      *reinterpret_cast<uint2*>(row + 32 * dt + 8 * g + 4 * hh) = w;
+    }
+}
+
+// keys that packed row r's query sees
+__device__ __forceinline__ int seen(bool causal, int i, const Seq& s) {
+  return causal ? min(max(i + 1 + s.lk - s.lq, 0), s.lk) : s.lk;
+}
+
+// rows [from, from + 128) of the rows behind the last sequence, as zero
+__device__ __forceinline__ void zero_rows(bf16_t* out, int64_t o_t, int64_t o_h, int t0, int from, int count, int hk, int G,
+                                          float* lse, int H) {
+  for (int e = threadIdx.x; e < kRows * 8; e += 256) {
+    const int r = from + (e >> 3);
+    if (r >= count) break;
+    const int i = r / G, h = hk * G + r - i * G;
+    *reinterpret_cast<uint4*>(out + (t0 + i) * o_t + h * o_h + (e & 7) * 8) = make_uint4(0, 0, 0, 0);
+    if (lse && (e & 7) == 0) lse[(int64_t)(t0 + i) * H + h] = -INFINITY;
+  }
+}
+
+// ------------------------------------------------------------------ forward
+// One workgroup: 128 packed rows of one key head, over all of their keys or (SPLIT) over one of nsplit shares of
+// them.  Each wave owns 32 rows, a row to a lane: S^T = K Q^T leaves a query's scores in one lane's
+// registers, which then are the B operand of O^T += V^T P^T.  K and V tiles of 64 keys go through LDS by
+// LDS-DMA, double-buffered.  The scores start at minus the row's reference m (the accumulator's start value);
+// m moves only when a probability could pass 2^8, so the usual tile has no maximum and no rescale.
+template <bool CAUSAL, bool SPLIT>
+__global__ __launch_bounds__(256, 3) void k_attnp_fwd(const Args a) {
+  __shared__ __attribute__((aligned(16))) uint8_t smem[4 * kTileBytes];
+  const int lane = threadIdx.x & 63, hh = lane >> 5, lr = lane & 31;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // key heads fastest: workgroups b and b + 8 share an XCD, so with 8 heads (4, 2) each XCD (pair, four) keeps to
+  // one head's keys; later tiles, which a causal mask leaves the most keys, come first
+  const int hk = blockIdx.x % a.Hk;
+  int rest = blockIdx.x / a.Hk;
+  const int split = SPLIT ? rest % a.nsplit : 0;
+  if (SPLIT) rest /= a.nsplit;
+  const int tiles = gridDim.x / (a.Hk * (SPLIT ? a.nsplit : 1));
+  int tile;
+  const int b = find_tile(a.cu_q, a.Tq, a.G, kRows, a.B + a.zero_tail, tiles - 1 - rest, lane, tile);
+  if (b == a.B) {                                    // the rows behind the last sequence
+    const int t0 = cu_at(a.cu_q, a.B, a.Tq);
+    if (!SPLIT) zero_rows(a.out, a.o_t, a.o_h, t0, tile * kRows, (a.Tq - t0) * a.G, hk, a.G, a.lse, a.H);
+    return;
+  }
+  const Seq s = sequence(a, b);
+  const int R = s.lq * a.G, r0 = tile * kRows;
+  if (r0 >= R) return;
+  const int r = r0 + wid * 32 + lr, rc = min(r, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
+  const int nk = seen(CAUSAL, qi, s);
+  // first and last row of the wave, last row of the tile (uniform)
+  const int w0 = min(r0 + wid * 32, R - 1);
+  const bool wave_on = r0 + wid * 32 < R;
+  const int nk_first = seen(CAUSAL, w0 / a.G, s), nk_last = seen(CAUSAL, min(w0 + 31, R - 1) / a.G, s);
+  int ks = 0, ke = seen(CAUSAL, (min(r0 + kRows, R) - 1) / a.G, s);
+  if (SPLIT) {
+    const int chunk = ((s.lk + a.nsplit - 1) / a.nsplit + kKV - 1) / kKV * kKV;
+    ks = min((int64_t)split * chunk, (int64_t)ke);
+    ke = min(ke, ks + chunk);
+  }
+
+  const bf16_t* Kg = a.k + (s.k0 * a.k_t + hk * a.k_h);
+  const bf16_t* Vg = a.v + (s.k0 * a.v_t + hk * a.v_h);
+  const Stage stk(wid, lane, a.k_t), stv(wid, lane, a.v_t);
+  auto stage = [&](int buf, int key) {
+    stk.load(rows_rsrc(Kg + key * a.k_t, a.k_t, s.lk - key), smem + buf * 2 * kTileBytes, wid);
+    stv.load(rows_rsrc(Vg + key * a.v_t, a.v_t, s.lk - key), smem + (buf * 2 + 1) * kTileBytes, wid);
+  };
+  if (ks < ke) stage(0, ks);
+  bf16x8 qf[4];
+  {
+    const bf16_t* qr = a.q + (s.q0 + qi) * a.q_t + h * a.q_h;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) qf[t] = *reinterpret_cast<const bf16x8*>(qr + 16 * t + 8 * hh);
+  }
+  __builtin_amdgcn_s_waitcnt(0xF70);                 // vmcnt(0), known to the compiler: Q and the first tile
+  __syncthreads();
+
+  const float c = a.c;
+  f32x16 o[2], nm;
+  for (int i = 0; i < 16; ++i) o[0][i] = o[1][i] = nm[i] = 0.f;
+  float l = 0.f;
+  int bad = 0;
+  constexpr float kThresh = 256.f;
+
+  for (int key0 = ks, cur = 0; key0 < ke; key0 += kKV, cur ^= 1) {
+    if (key0 + kKV < ke) stage(cur ^ 1, key0 + kKV);
+    const uint8_t* sK = smem + cur * 2 * kTileBytes;
+    const uint8_t* sV = sK + kTileBytes;
+    if (wave_on) {
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2) {
+        if (key0 + 32 * k2 >= nk_last) break;        // no row of the wave sees these keys
+        bf16x8 kf[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) kf[t] = row_frag(sK, 32 * k2 + lr, t, hh);
+        f32x16 st;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) st = mfma(kf[t], qf[t], t == 0 ? nm : st);
+        const bool partial = key0 + 32 * k2 + 32 > nk_first;    // uniform
+        const int left = nk - key0 - 32 * k2;
+        if (partial) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if ((i & 3) + 8 * (i >> 2) + 4 * hh >= left) st[i] = -INFINITY;
+        }
+        float ls = 0.f;
+        uint32_t pk[8];
+        auto probs = [&](float sub) {                // sub: in units of the raw scores
+          ls = 0.f;
+          const float nsub = -sub * c;
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(st[i], c, nsub));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(st[i + 1], c, nsub));
+            ls += p0 + p1;
+            pk[i >> 1] = pack_bf16(p0, p1);
+          }
+        };
+        const bool first = key0 == ks && k2 == 0;
+        bool full = first;
+        if (!full) {
+          probs(0.f);
+          full = __ballot(ls >= kThresh) != 0;
+        }
+        if (full) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[i]);
+          const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+          mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+          // a row that sees nothing here keeps its reference
+          const float delta = first ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, 0.f);
+          probs(delta);
+          if (!first) {
+            const float alpha = __builtin_amdgcn_exp2f(-delta * c);
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              o[0][i] *= alpha;
+              o[1][i] *= alpha;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) nm[i] -= delta;
+        }
+        l += ls;
+        bf16x8 vf[2][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int dt = 0; dt < 2; ++dt) vf[t][dt] = tr_frag(sV, 32 * k2 + 16 * t, dt, lane);
+        if (CAUSAL && partial) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) bad |= (int)nonfinite(vf[t][0]) + (int)nonfinite(vf[t][1]);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int dt = 0; dt < 2; ++dt) o[dt] = mfma(vf[t][dt], p_frag(pk, t), o[dt]);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the next tile landed (this wave's part)
+    __syncthreads();                                     // ... and every wave's
+  }
+  if (CAUSAL && __ballot(bad) != 0) {
+    float m = -INFINITY;
+    l = 0.f;
+    for (int i = 0; i < 16; ++i) o[0][i] = o[1][i] = 0.f;
+#pragma clang loop unroll(disable)
+    for (int j = ks; j < min(ke, nk_last); ++j) {
+      const float x = dot_row(Kg + j * a.k_t, qf, hh);
+      if (j < nk) {
+        const float m_new = fmaxf(m, x), alpha = m == m_new ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
+        const float p = __builtin_amdgcn_exp2f((x - m_new) * c);
+        m = m_new;
+        l = fmaf(l, alpha, p);
+        for (int i = 0; i < 16; ++i) {
+          o[0][i] *= alpha;
+          o[1][i] *= alpha;
+        }
+        add_row(o, p, Vg + j * a.v_t, hh);
+      }
+    }
+    nm[0] = -m;
+    if (hh) l = 0.f;                                   // both halves hold the whole sum
+  }
+  l += __shfl_xor(l, 32);
+  if (r >= R) return;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const float l2 = l == 0.f ? -INFINITY : fmaf(-nm[0], c, log2f(l));
+  if (SPLIT) {
+    const int64_t row = ((int64_t)split * a.Hk + hk) * a.Tq * a.G + (int64_t)s.q0 * a.G + r;
+    if (hh == 0) a.part_l[row] = l2;
+    if (l2 != -INFINITY) {
+#pragma unroll
+      for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4*>(a.part_o + row * 64 + 32 * dt + 8 * g + 4 * hh) =
+              make_float4(o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv, o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv);
+    }
+  } else {
+    store_acc(a.out + (s.q0 + qi) * a.o_t + h * a.o_h, o, inv, hh);
+    if (hh == 0) a.lse[(int64_t)(s.q0 + qi) * a.H + h] = l2 * 0.69314718055994531f;
+  }
+}
+
+// The shares of a split call joined, a wave to a row: out = sum_s 2^(l_s - m) O_s / sum_s 2^(l_s - m).
+__global__ __launch_bounds__(256) void k_attnp_join(const Args a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t rows = (int64_t)a.Tq * a.G, n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (n >= rows * a.Hk) return;
+  const int hk = (int)(n / rows), row = (int)(n - hk * rows), t = row / a.G, h = hk * a.G + row - t * a.G;
+  const bool tail = t >= cu_at(a.cu_q, a.B, a.Tq);
+  if (tail && !a.zero_tail) return;
+  bf16_t* out = a.out + t * a.o_t + h * a.o_h + lane;
+  float acc = 0.f, m = -INFINITY, total = 0.f;
+  if (!tail) {
+    for (int s = lane; s < a.nsplit; s += 64) m = fmaxf(m, a.part_l[((int64_t)s * a.Hk + hk) * rows + row]);
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+    for (int s0 = 0; s0 < a.nsplit; s0 += 64) {
+      const int s = s0 + lane;
+      const float ls = s < a.nsplit ? a.part_l[((int64_t)s * a.Hk + hk) * rows + row] : -INFINITY;
+      // NaN shares (a NaN or infinite score) stay NaN
+      const float w = ls == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ls - m);
+      total += w;
+      const int last = min(64, a.nsplit - s0);
+      for (int j = 0; j < last; ++j) {
+        const float wj = __shfl(w, j);
+        if (wj != 0.f) acc = fmaf(wj, a.part_o[(((int64_t)(s0 + j) * a.Hk + hk) * rows + row) * 64 + lane], acc);
+      }
+    }
+    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off);
+  }
+  const float v = total == 0.f ? 0.f : acc / total;
+  const __bf16 o = (__bf16)v;
+  *out = __builtin_bit_cast(bf16_t, o);
+  if (lane == 0) a.lse[(int64_t)t * a.H + h] = total == 0.f ? -INFINITY : (m + log2f(total)) * 0.69314718055994531f;
+}
+
+// ------------------------------------------------------------------ backward
+// nlse = -lse / scale (a row that saw nothing: -inf, so that its probabilities are 0) and ndelta = -D, both [H][Tq]:
+// 8 lanes a row.
+__global__ __launch_bounds__(256) void k_attnp_delta(const Args a) {
+  const int64_t n = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
+  if (n >= (int64_t)a.Tq * a.H) return;
+  const int t = (int)(n / a.H), h = (int)(n - (int64_t)t * a.H), ch = threadIdx.x & 7;
+  const uint4 x = *reinterpret_cast<const uint4*>(a.dout + t * a.d_t + h * a.d_h + ch * 8);
+  const uint4 y = *reinterpret_cast<const uint4*>(a.out + t * a.o_t + h * a.o_h + ch * 8);
+  const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+  float d = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    d = fmaf(__uint_as_float(xs[i] << 16), __uint_as_float(ys[i] << 16), d);
+    d = fmaf(__uint_as_float(xs[i] & 0xffff0000u), __uint_as_float(ys[i] & 0xffff0000u), d);
+  }
+  d += __shfl_xor(d, 1);
+  d += __shfl_xor(d, 2);
+  d += __shfl_xor(d, 4);
+  if (ch == 0) {
+    const float lse = a.lse[n];
+    a.nlse[(int64_t)h * a.Tq + t] = lse == -INFINITY ? -INFINITY : -lse / a.scale;
+    a.ndelta[(int64_t)h * a.Tq + t] = lse == -INFINITY ? 0.f : -d;
+  }
+}
+
+// dQ: the forward's rows and tiles; per 32 keys S^T = K Q^T and dP^T = V dO^T, then dQ^T += K^T dS^T.
+template <bool CAUSAL>
+__global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
+  __shared__ __attribute__((aligned(16))) uint8_t smem[4 * kTileBytes];
+  const int lane = threadIdx.x & 63, hh = lane >> 5, lr = lane & 31;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hk = blockIdx.x % a.Hk, tiles = gridDim.x / a.Hk;
+  int tile;
+  const int b = find_tile(a.cu_q, a.Tq, a.G, kRows, a.B + a.zero_tail, tiles - 1 - (int)(blockIdx.x / a.Hk), lane, tile);
+  if (b == a.B) {
+    const int t0 = cu_at(a.cu_q, a.B, a.Tq);
+    zero_rows(a.dq, a.dq_t, a.dq_h, t0, tile * kRows, (a.Tq - t0) * a.G, hk, a.G, nullptr, 0);
+    return;
+  }
+  const Seq s = sequence(a, b);
+  const int R = s.lq * a.G, r0 = tile * kRows;
+  if (r0 >= R) return;
+  const int r = r0 + wid * 32 + lr, rc = min(r, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
+  const int nk = seen(CAUSAL, qi, s);
+  const int w0 = min(r0 + wid * 32, R - 1);
+  const bool wave_on = r0 + wid * 32 < R;
+  const int nk_first = seen(CAUSAL, w0 / a.G, s), nk_last = seen(CAUSAL, min(w0 + 31, R - 1) / a.G, s);
+  const int ke = seen(CAUSAL, (min(r0 + kRows, R) - 1) / a.G, s);
+
+  const bf16_t* Kg = a.k + (s.k0 * a.k_t + hk * a.k_h);
+  const bf16_t* Vg = a.v + (s.k0 * a.v_t + hk * a.v_h);
+  const Stage stk(wid, lane, a.k_t), stv(wid, lane, a.v_t);
+  auto stage = [&](int buf, int key) {
+    stk.load(rows_rsrc(Kg + key * a.k_t, a.k_t, s.lk - key), smem + buf * 2 * kTileBytes, wid);
+    stv.load(rows_rsrc(Vg + key * a.v_t, a.v_t, s.lk - key), smem + (buf * 2 + 1) * kTileBytes, wid);
+  };
+  if (ke > 0) stage(0, 0);
+  bf16x8 qf[4], df[4];
+  const bf16_t* qr = a.q + (s.q0 + qi) * a.q_t + h * a.q_h;
+  const bf16_t* dr = a.dout + (s.q0 + qi) * a.d_t + h * a.d_h;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    qf[t] = *reinterpret_cast<const bf16x8*>(qr + 16 * t + 8 * hh);
+    df[t] = *reinterpret_cast<const bf16x8*>(dr + 16 * t + 8 * hh);
+  }
+  const float c = a.c, nl = a.nlse[(int64_t)h * a.Tq + s.q0 + qi] * c;
+  f32x16 nd, dq[2];
+  {
+    const float d = a.ndelta[(int64_t)h * a.Tq + s.q0 + qi];
+    for (int i = 0; i < 16; ++i) {
+      nd[i] = d;
+      dq[0][i] = dq[1][i] = 0.f;
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0xF70);
+  __syncthreads();
+
+  int bad = 0;
+  for (int key0 = 0, cur = 0; key0 < ke; key0 += kKV, cur ^= 1) {
+    if (key0 + kKV < ke) stage(cur ^ 1, key0 + kKV);
+    const uint8_t* sK = smem + cur * 2 * kTileBytes;
+    const uint8_t* sV = sK + kTileBytes;
+    if (wave_on) {
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2) {
+        if (key0 + 32 * k2 >= nk_last) break;
+        f32x16 st, dp;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          st = mfma(row_frag(sK, 32 * k2 + lr, t, hh), qf[t], t == 0 ? f32x16{} : st);
+          dp = mfma(row_frag(sV, 32 * k2 + lr, t, hh), df[t], t == 0 ? nd : dp);
+        }
+        const bool partial = key0 + 32 * k2 + 32 > nk_first;
+        const int left = nk - key0 - 32 * k2;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(fmaf(st[i], c, nl));
+        if (partial) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if ((i & 3) + 8 * (i >> 2) + 4 * hh >= left) dp[i] = 0.f;
+        }
+        uint32_t pk[8];
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) pk[i >> 1] = pack_bf16(dp[i], dp[i + 1]);
+        bf16x8 kt[2][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int dt = 0; dt < 2; ++dt) kt[t][dt] = tr_frag(sK, 32 * k2 + 16 * t, dt, lane);
+        if (CAUSAL && partial) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) bad |= (int)nonfinite(kt[t][0]) + (int)nonfinite(kt[t][1]);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int dt = 0; dt < 2; ++dt) dq[dt] = mfma(kt[t][dt], p_frag(pk, t), dq[dt]);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+  if (CAUSAL && __ballot(bad) != 0) {
+    for (int i = 0; i < 16; ++i) dq[0][i] = dq[1][i] = 0.f;
+#pragma clang loop unroll(disable)
+    for (int j = 0; j < nk_last; ++j) {
+      const float x = dot_row(Kg + j * a.k_t, qf, hh), y = dot_row(Vg + j * a.v_t, df, hh);
+      if (j < nk) add_row(dq, __builtin_amdgcn_exp2f(fmaf(x, c, nl)) * (y + nd[0]), Kg + j * a.k_t, hh);
+    }
+  }
+  if (r < R) store_acc(a.dq + (s.q0 + qi) * a.dq_t + h * a.dq_h, dq, a.scale, hh);
+}
+
+// dK, dV: 64 keys of one key head a workgroup, over the rows of its G query heads one after the other.  A key to a
+// lane: S = Q K^T and dP = dO V^T leave a key's column in one lane's registers, which then are the B operand of
+// dV^T += dO^T P and dK^T += Q^T dS.  Waves 0, 1 take rows 0-31 of each 64-row tile, waves 2, 3 rows 32-63; their sums
+// are added at the end.
+template <bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
+  // two buffers of Q tile, dO tile, 64 nlse, 64 ndelta
+  constexpr int kBuf = 2 * kTileBytes + 512;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[2 * kBuf];
+  const int lane = threadIdx.x & 63, hh = lane >> 5, lr = lane & 31;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kh = wid & 1, qh = wid >> 1;
+  const int hk = blockIdx.x % a.Hk;
+  int tile;
+  const int b = find_tile(a.cu_k, a.Tk, 1, kKeys, a.B + a.zero_tail, blockIdx.x / a.Hk, lane, tile);
+  if (b == a.B) {
+    const int t0 = cu_at(a.cu_k, a.B, a.Tk);
+    for (int e = threadIdx.x; e < kKeys * 8; e += 256) {
+      const int64_t t = t0 + tile * kKeys + (e >> 3);
+      if (t >= a.Tk) break;
+      *reinterpret_cast<uint4*>(a.dk + t * a.dk_t + hk * a.dk_h + (e & 7) * 8) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(a.dv + t * a.dv_t + hk * a.dv_h + (e & 7) * 8) = make_uint4(0, 0, 0, 0);
+    }
+    return;
+  }
+  const Seq s = sequence(a, b);
+  const int key0 = tile * kKeys;
+  if (key0 >= s.lk) return;
+  const int kw = key0 + 32 * kh;                       // the wave's first key
+  const int key = kw + lr, kc = min(key, s.lk - 1);
+  // causal: key j is seen by the queries from j - (lk - lq) on
+  const int off = s.lk - s.lq;
+  const int i_first = CAUSAL ? max(0, key0 - off) : 0;
+  const int tiles = s.lq > i_first ? (s.lq - i_first + 63) / 64 : 0, total = tiles * a.G;
+
+  const Stage stq(wid, lane, a.q_t), std_(wid, lane, a.d_t);
+  auto stage = [&](int buf, int n) {
+    const int g = n / tiles, h = hk * a.G + g, i = i_first + (n - g * tiles) * 64;
+    uint8_t* base = smem + buf * kBuf;
+    stq.load(rows_rsrc(a.q + ((s.q0 + i) * a.q_t + h * a.q_h), a.q_t, s.lq - i), base, wid);
+    std_.load(rows_rsrc(a.dout + ((s.q0 + i) * a.d_t + h * a.d_h), a.d_t, s.lq - i), base + kTileBytes, wid);
+    if (wid < 2) {
+      const float* st = (wid ? a.ndelta : a.nlse) + (int64_t)h * a.Tq + s.q0 + i;
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(st), 0, min(s.lq - i, 64) * 4, 0x00020000);
+      dma4(rs, __builtin_amdgcn_readfirstlane(lds_addr(base + 2 * kTileBytes + wid * 256)), lane * 4);
+    }
+  };
+  if (total > 0) stage(0, 0);
+  bf16x8 kf[4], vf[4];
+  {
+    const bf16_t* kr = a.k + (s.k0 + kc) * a.k_t + hk * a.k_h;
+    const bf16_t* vr = a.v + (s.k0 + kc) * a.v_t + hk * a.v_h;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      kf[t] = *reinterpret_cast<const bf16x8*>(kr + 16 * t + 8 * hh);
+      vf[t] = *reinterpret_cast<const bf16x8*>(vr + 16 * t + 8 * hh);
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0xF70);
+  __syncthreads();
+
+  const float c = a.c;
+  f32x16 dk[2], dv[2];
+  for (int i = 0; i < 16; ++i) dk[0][i] = dk[1][i] = dv[0][i] = dv[1][i] = 0.f;
+
+  int bad = 0;
+  for (int n = 0, cur = 0; n < total; ++n, cur ^= 1) {
+    if (n + 1 < total) stage(cur ^ 1, n + 1);
+    const uint8_t* sQ = smem + cur * kBuf;
+    const uint8_t* sD = sQ + kTileBytes;
+    const float* stat = reinterpret_cast<const float*>(sQ + 2 * kTileBytes);
+    const int i0 = i_first + n % tiles * 64 + 32 * qh;      // the wave's first query
+    // some query of the block exists and sees some key of the wave
+    const bool on = i0 < s.lq && (!CAUSAL || i0 + 31 >= kw - off);
+    if (on) {
+      f32x16 st, dp;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 x = *reinterpret_cast<const float4*>(stat + 32 * qh + 8 * g + 4 * hh);
+        const float4 y = *reinterpret_cast<const float4*>(stat + 64 + 32 * qh + 8 * g + 4 * hh);
+        st[4 * g] = x.x, st[4 * g + 1] = x.y, st[4 * g + 2] = x.z, st[4 * g + 3] = x.w;
+        dp[4 * g] = y.x, dp[4 * g + 1] = y.y, dp[4 * g + 2] = y.z, dp[4 * g + 3] = y.w;
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        st = mfma(row_frag(sQ, 32 * qh + lr, t, hh), kf[t], st);
+        dp = mfma(row_frag(sD, 32 * qh + lr, t, hh), vf[t], dp);
+      }
+      const bool partial = CAUSAL && i0 < kw + 31 - off;     // uniform
+      const int first = key - off - i0;                      // the block's rows below this do not see the lane's key
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        st[i] = __builtin_amdgcn_exp2f(st[i] * c);
+        dp[i] *= st[i];
+      }
+      if (partial) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if ((i & 3) + 8 * (i >> 2) + 4 * hh < first) st[i] = dp[i] = 0.f;
+      }
+      uint32_t pk[8], dsk[8];
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        pk[i >> 1] = pack_bf16(st[i], st[i + 1]);
+        dsk[i >> 1] = pack_bf16(dp[i], dp[i + 1]);
+      }
+      if (partial) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int dt = 0; dt < 2; ++dt)
+            bad |= (int)nonfinite(tr_frag(sD, 32 * qh + 16 * t, dt, lane)) + (int)nonfinite(tr_frag(sQ, 32 * qh + 16 * t, dt, lane));
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt) {
+          dv[dt] = mfma(tr_frag(sD, 32 * qh + 16 * t, dt, lane), p_frag(pk, t), dv[dt]);
+          dk[dt] = mfma(tr_frag(sQ, 32 * qh + 16 * t, dt, lane), p_frag(dsk, t), dk[dt]);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+  if (CAUSAL && __ballot(bad) != 0) {
+    for (int i = 0; i < 16; ++i) dk[0][i] = dk[1][i] = dv[0][i] = dv[1][i] = 0.f;
+    const Args& w = again();
+    for (int g = 0; g < w.G; ++g) {
+      const int h = hk * w.G + g;
+#pragma clang loop unroll(disable)
+      for (int i = i_first; i < s.lq; ++i) {
+        if (((i - i_first) >> 5 & 1) != qh) continue;         // the other waves' rows
+        const bf16_t* qr = w.q + (s.q0 + i) * w.q_t + h * w.q_h;
+        const bf16_t* dr = w.dout + (s.q0 + i) * w.d_t + h * w.d_h;
+        const float x = dot_row(qr, kf, hh), y = dot_row(dr, vf, hh);
+        if (i >= key - off) {
+          const int64_t st = (int64_t)h * w.Tq + s.q0 + i;
+          const float p = __builtin_amdgcn_exp2f((x + w.nlse[st]) * c);
+          add_row(dv, p, dr, hh);
+          add_row(dk, p * (y + w.ndelta[st]), qr, hh);
+        }
+      }
+    }
+  }
+  // the two row halves' sums: 64 floats x 64 lanes of waves 2, 3 through LDS (32 KiB, the buffers' own)
+  float* x = reinterpret_cast<float*>(smem) + kh * 64 * 64;
+  if (qh == 1) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[i * 64 + lane] = dk[0][i];
+      x[(16 + i) * 64 + lane] = dk[1][i];
+      x[(32 + i) * 64 + lane] = dv[0][i];
+      x[(48 + i) * 64 + lane] = dv[1][i];
+    }
+  }
+  __syncthreads();
+  if (qh == 1 || key >= s.lk) return;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    dk[0][i] += x[i * 64 + lane];
+    dk[1][i] += x[(16 + i) * 64 + lane];
+    dv[0][i] += x[(32 + i) * 64 + lane];
+    dv[1][i] += x[(48 + i) * 64 + lane];
+  }
+  store_acc(a.dk + (s.k0 + key) * a.dk_t + hk * a.dk_h, dk, a.scale, hh);
+  store_acc(a.dv + (s.k0 + key) * a.dv_t + hk * a.dv_h, dv, 1.0f, hh);
+}
+
+// ------------------------------------------------------------------ host side
+inline int64_t row_tiles(const i2pc_attn_packed_desc& d) {
+  return (int64_t)d.total_q * (d.heads / d.kv_heads) / kRows + d.batch + (d.zero_tail ? 1 : 0);
+}
+
+// Shares of the keys: one where the row tiles fill the chip, else so many that they do, of 256 keys at least (an
+// upper bound: a share may be empty).
+inline int splits(const i2pc_attn_packed_desc& d) {
+  const int64_t tiles = row_tiles(d) * d.kv_heads;
+  if (tiles >= 512 || d.total_k == 0) return 1;
+  const int64_t want = (1024 + tiles - 1) / tiles, most = (d.total_k + 255) / 256;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 512}));
+}
+
+// Rows apart (the range checks of the tiles' loads go by the row stride), heads apart too where they are written.
+inline bool rows_ok(const void* p, int64_t t, int64_t h, int rows, int heads, bool written) {
+  return rows == 0 || (p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && t % 8 == 0 && h % 8 == 0 && (rows == 1 || t >= 64) &&
+                       t >= 0 && t < ((int64_t)1 << 23) && (written && heads > 1 ? h >= 64 : h >= 0) && h < ((int64_t)1 << 40));
+}
+
+int check(const char* what, const i2pc_attn_packed_desc* d) {
+  I2PC_REQUIRE(d, "NULL descriptor");
+  I2PC_REQUIRE(d->batch >= 0 && d->total_q >= 0 && d->total_k >= 0 && d->heads > 0 && d->kv_heads > 0 &&
+                   d->heads % d->kv_heads == 0,
+               "%s: batch=%d total_q=%d total_k=%d heads=%d kv_heads=%d (heads a multiple of kv_heads)", what, d->batch,
+               d->total_q, d->total_k, d->heads, d->kv_heads);
+  if (d->head_dim != 64) return set_error(I2PC_EUNSUPPORTED, "%s: head_dim=%d, the kernels are of 64", what, d->head_dim);
+  // grids of 256-thread workgroups hold 2^24 of them
+  const int64_t most = (int64_t)1 << 24;
+  if ((int64_t)d->total_q * d->heads >= most * 32 || ((int64_t)d->total_q / kRows + d->batch + 1) * d->heads >= most ||
+      ((int64_t)d->total_k / kKeys + d->batch + 1) * d->kv_heads >= most)
+    return set_error(I2PC_EUNSUPPORTED, "%s: total_q * heads must stay below 2^29, (total_k / 64 + batch) * kv_heads below 2^24", what);
+  I2PC_REQUIRE(std::isfinite(d->scale) && d->scale > 0.f, "%s: scale=%g must be finite and above zero", what, (double)d->scale);
+  I2PC_REQUIRE(d->batch == 0 || (d->cu_q && d->cu_k), "%s: NULL cu_q or cu_k", what);
+  I2PC_REQUIRE(rows_ok(d->q, d->q_t, d->q_h, d->total_q, d->heads, false) &&
+                   rows_ok(d->out, d->o_t, d->o_h, d->total_q, d->heads, true) &&
+                   rows_ok(d->k, d->k_t, d->k_h, d->total_k, d->kv_heads, false) &&
+                   rows_ok(d->v, d->v_t, d->v_h, d->total_k, d->kv_heads, false) &&
+                   (d->total_q == 0 || d->lse),
+               "%s: q, k, v, out must be 16-byte aligned with strides that are multiples of 8 "
+               "(row strides from 64 to 2^23)", what);
+  return I2PC_OK;
+}
+
+Args args_of(const i2pc_attn_packed_desc& d) {
+  Args a = {};
+  a.q = static_cast<const bf16_t*>(d.q), a.k = static_cast<const bf16_t*>(d.k), a.v = static_cast<const bf16_t*>(d.v);
+  a.q_t = d.q_t, a.q_h = d.q_h, a.k_t = d.k_t, a.k_h = d.k_h, a.v_t = d.v_t, a.v_h = d.v_h;
+  a.out = static_cast<bf16_t*>(d.out), a.o_t = d.o_t, a.o_h = d.o_h, a.lse = d.lse;
+  a.cu_q = d.cu_q, a.cu_k = d.cu_k, a.k_lens = d.k_lens;
+  a.B = d.batch, a.Tq = d.total_q, a.Tk = d.total_k, a.H = d.heads, a.Hk = d.kv_heads, a.G = d.heads / d.kv_heads;
+  a.zero_tail = d.zero_tail != 0;
+  a.scale = d.scale;
+  a.c = d.scale * 1.4426950408889634f;
+  a.nsplit = 1;
+  return a;
+}
+
+}  // namespace attnp
+}  // namespace i2pc
+
+using namespace i2pc;
+
+extern "C" size_t i2pc_attention_packed_workspace_bytes(const i2pc_attn_packed_desc* d) {
+  if (attnp::check("attention_packed", d) != I2PC_OK) return 0;
+  const int n = attnp::splits(*d);
+  return n == 1 ? 0 : (size_t)n * d->heads * d->total_q * 65 * sizeof(float);
+}
+
+extern "C" int i2pc_attention_packed(const i2pc_attn_packed_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (const int rc = attnp::check("attention_packed", d)) return rc;
+  if (d->total_q == 0 || (d->batch == 0 && !d->zero_tail)) return I2PC_OK;
+  I2PC_REQUIRE(d->batch > 0, "attention_packed: zero_tail without a sequence");
+  const size_t need = i2pc_attention_packed_workspace_bytes(d);
+  if (need > workspace_bytes || (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16)))
+    return set_error(I2PC_EWORKSPACE, "attention_packed: workspace of %zu bytes, needs %zu (16-byte aligned)", workspace_bytes, need);
+  attnp::Args a = attnp::args_of(*d);
+  hipStream_t s = as_stream(stream);
+  a.nsplit = attnp::splits(*d);
+  const dim3 block(256), grid((uint32_t)(attnp::row_tiles(*d) * a.Hk * a.nsplit));
+  if (a.nsplit == 1) {
+    if (d->causal) hipLaunchKernelGGL((attnp::k_attnp_fwd<true, false>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((attnp::k_attnp_fwd<false, false>), grid, block, 0, s, a);
+    return check_launch("attention_packed");
+  }
+  a.part_o = static_cast<float*>(workspace);
+  a.part_l = a.part_o + (size_t)a.nsplit * a.H * a.Tq * 64;
+  if (d->causal) hipLaunchKernelGGL((attnp::k_attnp_fwd<true, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((attnp::k_attnp_fwd<false, true>), grid, block, 0, s, a);
+  hipLaunchKernelGGL(attnp::k_attnp_join, dim3((uint32_t)(((int64_t)a.Tq * a.H + 3) / 4)), block, 0, s, a);
+  return check_launch("attention_packed");
+}
+
+static int check_grad(const i2pc_attn_packed_grad_desc* g) {
+  using attnp::rows_ok;
+  I2PC_REQUIRE(g, "NULL descriptor");
+  const i2pc_attn_packed_desc& d = g->f;
+  if (const int rc = attnp::check("attention_packed_backward", &d)) return rc;
+  I2PC_REQUIRE(!d.k_lens, "attention_packed_backward: k_lens is of the forward call only");
+  I2PC_REQUIRE(rows_ok(g->dout, g->d_t, g->d_h, d.total_q, d.heads, false) &&
+                   rows_ok(g->dq, g->dq_t, g->dq_h, d.total_q, d.heads, true) &&
+                   rows_ok(g->dk, g->dk_t, g->dk_h, d.total_k, d.kv_heads, true) &&
+                   rows_ok(g->dv, g->dv_t, g->dv_h, d.total_k, d.kv_heads, true),
+               "attention_packed_backward: dout, dq, dk, dv must be 16-byte aligned with strides that are multiples of 8 "
+               "(row strides from 64 to 2^23)");
+  return I2PC_OK;
+}
+
+extern "C" size_t i2pc_attention_packed_backward_workspace_bytes(const i2pc_attn_packed_grad_desc* g) {
+  if (check_grad(g) != I2PC_OK) return 0;
+  return (size_t)2 * g->f.total_q * g->f.heads * sizeof(float);
+}
+
+extern "C" int i2pc_attention_packed_backward(const i2pc_attn_packed_grad_desc* g, void* workspace, size_t workspace_bytes,
+                                              void* stream) {
+  clear_error();
+  if (const int rc = check_grad(g)) return rc;
+  const i2pc_attn_packed_desc& d = g->f;
+  if (d.batch == 0) {
+    I2PC_REQUIRE(!d.zero_tail, "attention_packed_backward: zero_tail without a sequence");
+    return I2PC_OK;
+  }
+  const size_t need = i2pc_attention_packed_backward_workspace_bytes(g);
+  if (need > workspace_bytes || (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16)))
+    return set_error(I2PC_EWORKSPACE, "attention_packed_backward: workspace of %zu bytes, needs %zu (16-byte aligned)",
+                     workspace_bytes, need);
+  attnp::Args a = attnp::args_of(d);
+  a.dout = static_cast<const attn::bf16_t*>(g->dout), a.d_t = g->d_t, a.d_h = g->d_h;
+  a.dq = static_cast<attn::bf16_t*>(g->dq), a.dk = static_cast<attn::bf16_t*>(g->dk), a.dv = static_cast<attn::bf16_t*>(g->dv);
+  a.dq_t = g->dq_t, a.dq_h = g->dq_h, a.dk_t = g->dk_t, a.dk_h = g->dk_h, a.dv_t = g->dv_t, a.dv_h = g->dv_h;
+  a.nlse = static_cast<float*>(workspace);
+  a.ndelta = a.nlse + (size_t)a.Tq * a.H;
+  hipStream_t s = as_stream(stream);
+  const dim3 block(256);
+  if (a.Tq > 0) {
+    hipLaunchKernelGGL(attnp::k_attnp_delta, dim3((uint32_t)(((int64_t)a.Tq * a.H + 31) / 32)), block, 0, s, a);
+    const dim3 grid((uint32_t)(attnp::row_tiles(d) * a.Hk));
+    if (d.causal) hipLaunchKernelGGL(attnp::k_attnp_dq<true>, grid, block, 0, s, a);
+    else hipLaunchKernelGGL(attnp::k_attnp_dq<false>, grid, block, 0, s, a);
+  }
+  if (a.Tk > 0) {
+    const dim3 grid((uint32_t)(((int64_t)a.Tk / attnp::kKeys + a.B + a.zero_tail) * a.Hk));
+    if (d.causal) hipLaunchKernelGGL(attnp::k_attnp_dkdv<true>, grid, block, 0, s, a);
+    else hipLaunchKernelGGL(attnp::k_attnp_dkdv<false>, grid, block, 0, s, a);
+  }
+  return check_launch("attention_packed_backward");
+}

@@ -1,0 +1,358 @@
+// LayerNorm's training step (gfx950): forward with its row statistics, backward with the gradients of
+// the input, the scale and the offset.
+//
+//   mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), h = (x - mu) r
+//   y  = h gamma + beta
+//   dx = r (dy gamma - mean(dy gamma) - h mean(dy gamma h)) [+ add]
+//   dgamma = sum over rows of dy h,   dbeta = sum over rows of dy
+//
+// Both directions are bound by HBM: x, dy, add read once, y / dx written once, the row in registers
+// between its reductions (two-pass variance in fp32).  The column sums of the backward pass ride on the
+// same read: a wave keeps the partial sums of its columns in registers over all the rows it takes, a
+// workgroup adds its waves' through LDS and writes one partial row, and k_lnt_cols adds the partial rows
+// -- fixed assignment and order, so the result does not change from run to run (no atomics).
+#include "common.h"
+
+#include <algorithm>
+
+namespace i2pc {
+namespace lnt {
+
+typedef uint16_t bf16_t;
+
+constexpr int kThreads = 512;                 // 8 waves
+constexpr int kMaxDim = 8192;
+constexpr int kMaxGroups = 512;               // two workgroups of 8 waves on each of 256 CUs
+
+__device__ __forceinline__ float wave_sum(float x) {
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+
+// E consecutive elements as floats, from / to an address with the element's own alignment only (rows of
+// an odd pitch): global memory takes such vector accesses, and one 16-byte request stays one request.
+template <typename T, int E>
+struct Vec;
+template <int E>
+struct Vec<float, E> {
+  static __device__ __forceinline__ void load(const float* p, float (&v)[E]) { __builtin_memcpy(v, p, E * 4); }
+  static __device__ __forceinline__ void store(float* p, const float (&v)[E]) { __builtin_memcpy(p, v, E * 4); }
+};
+template <int E>
+struct Vec<bf16_t, E> {
+  static __device__ __forceinline__ void load(const bf16_t* p, float (&v)[E]) {
+    bf16_t u[E];
+    __builtin_memcpy(u, p, E * 2);
+#pragma unroll
+    for (int j = 0; j < E; ++j) v[j] = __uint_as_float((uint32_t)u[j] << 16);
+  }
+  static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[E]) {
+    if constexpr (E == 1) {
+      const __bf16 b = (__bf16)v[0];
+      __builtin_memcpy(p, &b, 2);
+    } else {
+      uint32_t u[E / 2];
+#pragma unroll
+      for (int j = 0; j < E / 2; ++j) u[j] = pk2bf(v[2 * j], v[2 * j + 1]);
+      __builtin_memcpy(p, u, E * 2);
+    }
+  }
+};
+
+// A row's columns over WPR waves: chunk i of a lane starts at column (i * 64 * WPR + wave * 64 + lane) * E.
+// The last chunk of a row whose width is no multiple of E starts at dim - E instead and repeats columns of
+// the chunk before it: every load is a whole vector, `live` keeps the repeated columns out of the row
+// sums, and what is stored for them is stored twice with the same value.
+template <int E, int V, int WPR>
+struct Cols {
+  int col[V];
+  uint32_t first[V];      // elements below this index repeat another chunk's (E: the whole chunk is off the row)
+  __device__ __forceinline__ Cols(int lane, int sub, int dim) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int at = ((i * WPR + sub) * 64 + lane) * E;
+      col[i] = min(at, dim - E);
+      first[i] = (uint32_t)min(at - col[i], E);
+    }
+  }
+  __device__ __forceinline__ bool live(int i, int j) const { return (uint32_t)j >= first[i]; }
+};
+
+// sum of a over the row's WPR waves (every lane gets it)
+template <int WPR>
+__device__ __forceinline__ float row_sum(float a, float* red, int wave) {
+  a = wave_sum(a);
+  if constexpr (WPR > 1) {
+    __syncthreads();                               // the slots' last readers are done
+    if ((threadIdx.x & 63) == 0) red[wave] = a;
+    __syncthreads();
+    const int w0 = wave / WPR * WPR;
+    a = 0.f;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) a += red[w0 + w];
+  }
+  return a;
+}
+
+// One row per WPR waves of a workgroup of four waves (eight for the widest rows).
+template <typename T, int E, int V, int WPR>
+__global__ __launch_bounds__(WPR == 8 ? 512 : 256) void k_lnt_fwd(const T* __restrict__ x, int64_t ldx, const float* __restrict__ gamma,
+                                                 const float* __restrict__ beta, float eps, int rows, int dim,
+                                                 bf16_t* __restrict__ y, int64_t ldy, float2* __restrict__ stats) {
+  __shared__ float red[8];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Cols<E, V, WPR> c(lane, wave % WPR, dim);
+  constexpr int R = WPR == 1 ? 4 : 1;              // WPR > 1: one row a workgroup, all its waves or none
+  for (int64_t row = (int64_t)blockIdx.x * R + (WPR == 1 ? wave : 0); row < rows; row += (int64_t)gridDim.x * R) {
+    const T* xr = x + row * ldx;
+    float v[V][E];
+#pragma unroll
+    for (int i = 0; i < V; ++i) Vec<T, E>::load(xr + c.col[i], v[i]);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < E; ++j) s += c.live(i, j) ? v[i][j] : 0.f;
+    const float mean = row_sum<WPR>(s, red, wave) / (float)dim;
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        v[i][j] -= mean;
+        q += c.live(i, j) ? v[i][j] * v[i][j] : 0.f;
+      }
+    const float rstd = 1.0f / sqrtf(row_sum<WPR>(q, red, wave) / (float)dim + eps);
+    if (lane == 0 && wave % WPR == 0) stats[row] = make_float2(mean, rstd);
+    bf16_t* yr = y + row * ldy;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float g[E], b[E];
+      Vec<float, E>::load(gamma + c.col[i], g);
+      Vec<float, E>::load(beta + c.col[i], b);
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[i][j] = v[i][j] * rstd * g[j] + b[j];
+      if (c.first[i] < (uint32_t)E) Vec<bf16_t, E>::store(yr + c.col[i], v[i]);
+    }
+  }
+}
+
+// Rows blockIdx.x * R + k * gridDim.x * R for the R = 8 / WPR rows a workgroup takes at a time.  A partial row
+// of `part` is dim column sums of dgamma, then dim of dbeta.
+template <typename T, int E, int V, int WPR>
+__global__ __launch_bounds__(kThreads) void k_lnt_bwd(const bf16_t* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
+                                                      int64_t ldx, const float2* __restrict__ stats,
+                                                      const float* __restrict__ gamma, const T* add, int64_t lda, int rows,
+                                                      int dim, T* dx, int64_t lddx, float* __restrict__ part) {
+  __shared__ float red[8];
+  extern __shared__ float sums[];                  // [2][dim], rows of one wave only
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int R = 8 / WPR;
+  const Cols<E, V, WPR> c(lane, wave % WPR, dim);
+  float g[V][E], dg[V][E], db[V][E];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    Vec<float, E>::load(gamma + c.col[i], g[i]);
+#pragma unroll
+    for (int j = 0; j < E; ++j) dg[i][j] = db[i][j] = 0.f;
+  }
+  const float inv = 1.0f / (float)dim;
+  // WPR > 1 meets barriers inside: every wave runs the same number of rounds
+  for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < rows; row0 += (int64_t)gridDim.x * R) {
+    const int64_t row = row0 + wave / WPR;
+    const bool on = row < rows;
+    if (WPR == 1 && !on) break;
+    const int64_t rc = on ? row : rows - 1;
+    float xv[V][E], gy[V][E], av[V][E];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      Vec<T, E>::load(x + rc * ldx + c.col[i], xv[i]);
+      Vec<bf16_t, E>::load(dy + rc * lddy + c.col[i], gy[i]);
+    }
+    if (add) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) Vec<T, E>::load(add + rc * lda + c.col[i], av[i]);
+    }
+    const float2 st = stats[rc];
+    float a = 0.f, b = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float h = (xv[i][j] - st.x) * st.y, d = gy[i][j], gd = d * g[i][j];
+        xv[i][j] = h;
+        gy[i][j] = gd;
+        a += c.live(i, j) ? gd : 0.f;
+        b += c.live(i, j) ? gd * h : 0.f;
+        if (WPR == 1 || on) {
+          dg[i][j] += d * h;
+          db[i][j] += d;
+        }
+      }
+    a = row_sum<WPR>(a, red, wave) * inv;
+    b = row_sum<WPR>(b, red, wave) * inv;
+    if (WPR == 1 || on) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float o[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          o[j] = st.y * (gy[i][j] - a - xv[i][j] * b);
+          if (add) o[j] += av[i][j];
+        }
+        if (c.first[i] < (uint32_t)E) Vec<T, E>::store(dx + row * lddx + c.col[i], o);
+      }
+    }
+  }
+  if constexpr (WPR > 1) {                         // wide rows: a partial row for each row group
+    float* out = part + (int64_t)(blockIdx.x * R + wave / WPR) * 2 * dim;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (c.first[i] < (uint32_t)E) {
+        Vec<float, E>::store(out + c.col[i], dg[i]);
+        Vec<float, E>::store(out + dim + c.col[i], db[i]);
+      }
+  } else {                                         // the row groups' column sums, one after the other
+    for (int w = 0; w < R; ++w) {
+      __syncthreads();
+      if (wave == w) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (c.live(i, j)) {
+              const int at = c.col[i] + j;
+              sums[at] = w == 0 ? dg[i][j] : sums[at] + dg[i][j];
+              sums[dim + at] = w == 0 ? db[i][j] : sums[dim + at] + db[i][j];
+            }
+      }
+    }
+    __syncthreads();
+    float* out = part + (int64_t)blockIdx.x * 2 * dim;
+    for (int i = threadIdx.x; i < 2 * dim; i += kThreads) out[i] = sums[i];
+  }
+}
+
+// dgamma | dbeta [2 * dim] = the sum of `parts` partial rows: 64 columns a workgroup, 16 waves over the
+// rows, eight loads in flight each.
+__global__ __launch_bounds__(1024) void k_lnt_cols(const float* __restrict__ part, int parts, int dim,
+                                                   float* __restrict__ dgamma, float* __restrict__ dbeta) {
+  __shared__ float s[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = blockIdx.x * 64 + lane, n = 2 * dim, cc = min(col, n - 1);
+  float a = 0.f;
+  for (int p0 = wave; p0 < parts; p0 += 128) {
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = part[(int64_t)min(p0 + 16 * u, parts - 1) * n + cc];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) a += p0 + 16 * u < parts ? v[u] : 0.f;
+  }
+  s[wave][lane] = a;
+  __syncthreads();
+  if (wave == 0 && col < n) {
+    a = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) a += s[w][lane];
+    if (col < dim) dgamma[col] = a;
+    else dbeta[col - dim] = a;
+  }
+}
+
+// Rows a backward workgroup takes at a time (LNT_DISPATCH's 8 / WPR), its workgroups (one round each while
+// there are few rows) and their partial rows.
+inline int rows_at_once(int dim) { return dim <= 1024 ? 8 : dim <= 4096 ? 2 : 1; }
+inline int groups_for(int rows, int dim) {
+  const int r = rows_at_once(dim);
+  return std::max(1, std::min(kMaxGroups, (rows - 1) / r + 1));
+}
+inline int parts_for(int rows, int dim) { return groups_for(rows, dim) * (dim <= 1024 ? 1 : rows_at_once(dim)); }
+
+template <typename T, int E, int V, int WPR>
+void launch_fwd(const T* x, int64_t ldx, const float* gamma, const float* beta, float eps, int rows, int dim, bf16_t* y,
+                int64_t ldy, float2* stats, hipStream_t s) {
+  constexpr int R = WPR == 1 ? 4 : 1;
+  hipLaunchKernelGGL((k_lnt_fwd<T, E, V, WPR>), dim3(std::min((rows - 1) / R + 1, 1 << 22)), dim3(WPR == 8 ? 512 : 256), 0, s, x, ldx, gamma, beta, eps, rows,
+                     dim, y, ldy, stats);
+}
+template <typename T, int E, int V, int WPR>
+void launch_bwd(const bf16_t* dy, int64_t lddy, const T* x, int64_t ldx, const float2* stats, const float* gamma,
+                const T* add, int64_t lda, int rows, int dim, T* dx, int64_t lddx, float* part, hipStream_t s) {
+  hipLaunchKernelGGL((k_lnt_bwd<T, E, V, WPR>), dim3(groups_for(rows, dim)), dim3(kThreads),
+                     WPR == 1 ? 2 * dim * sizeof(float) : 0, s, dy,
+                     lddy, x, ldx, stats, gamma, add, lda, rows, dim, dx, lddx, part);
+}
+
+// The narrowest instance that holds the row: E elements a load, V loads a lane, WPR waves a row.  Rows above
+// 1024 take four waves or eight: the backward pass holds four values and two sums a column, and one wave's
+// registers would leave two waves a SIMD (200 to 256 VGPRs at 1536 and 2048).
+#define LNT_DISPATCH(FN, T, ...)                       \
+  do {                                                 \
+    if (dim <= 64) FN<T, 1, 1, 1>(__VA_ARGS__);        \
+    else if (dim <= 128) FN<T, 2, 1, 1>(__VA_ARGS__);  \
+    else if (dim <= 256) FN<T, 4, 1, 1>(__VA_ARGS__);  \
+    else if (dim <= 384) FN<T, 2, 3, 1>(__VA_ARGS__);  \
+    else if (dim <= 512) FN<T, 4, 2, 1>(__VA_ARGS__);  \
+    else if (dim <= 768) FN<T, 4, 3, 1>(__VA_ARGS__);  \
+    else if (dim <= 1024) FN<T, 4, 4, 1>(__VA_ARGS__); \
+    else if (dim <= 2048) FN<T, 4, 2, 4>(__VA_ARGS__); \
+    else if (dim <= 4096) FN<T, 8, 2, 4>(__VA_ARGS__); \
+    else FN<T, 8, 2, 8>(__VA_ARGS__);                  \
+  } while (0)
+
+}  // namespace lnt
+}  // namespace i2pc
+
+using namespace i2pc;
+
+extern "C" int i2pc_layernorm_train(const void* x, int x_f32, int64_t ldx, const float* gamma, const float* beta, float eps,
+                                    int rows, int dim, void* y, int64_t ldy, float* stats, void* stream) {
+  clear_error();
+  I2PC_REQUIRE(rows >= 0 && dim > 0, "layernorm_train: empty shape");
+  I2PC_REQUIRE(dim <= lnt::kMaxDim, "layernorm_train: dim=%d is above %d", dim, lnt::kMaxDim);
+  if (rows == 0) return I2PC_OK;
+  I2PC_REQUIRE(x && gamma && beta && y && stats, "NULL pointer");
+  I2PC_REQUIRE(ldx >= dim && ldy >= dim, "layernorm_train: row strides must be at least dim");
+  hipStream_t s = as_stream(stream);
+  auto* yy = static_cast<lnt::bf16_t*>(y);
+  auto* st = reinterpret_cast<float2*>(stats);
+  using namespace lnt;
+  if (x_f32)
+    LNT_DISPATCH(launch_fwd, float, static_cast<const float*>(x), ldx, gamma, beta, eps, rows, dim, yy, ldy, st, s);
+  else
+    LNT_DISPATCH(launch_fwd, bf16_t, static_cast<const bf16_t*>(x), ldx, gamma, beta, eps, rows, dim, yy, ldy, st, s);
+  return check_launch("layernorm_train");
+}
+
+extern "C" size_t i2pc_layernorm_backward_workspace_bytes(int rows, int dim) {
+  if (rows < 0 || dim <= 0 || dim > lnt::kMaxDim) return 0;
+  return (size_t)lnt::parts_for(rows, dim) * 2 * dim * sizeof(float);
+}
+
+extern "C" int i2pc_layernorm_backward(const void* dy, int64_t lddy, const void* x, int x_f32, int64_t ldx,
+                                       const float* stats, const float* gamma, const void* add, int64_t lda, int rows,
+                                       int dim, void* dx, int64_t lddx, float* dgamma, float* dbeta, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+  clear_error();
+  I2PC_REQUIRE(rows >= 0 && dim > 0, "layernorm_backward: empty shape");
+  I2PC_REQUIRE(dim <= lnt::kMaxDim, "layernorm_backward: dim=%d is above %d", dim, lnt::kMaxDim);
+  I2PC_REQUIRE(gamma && dgamma && dbeta && workspace && (rows == 0 || (dy && x && stats && dx)), "NULL pointer");
+  I2PC_REQUIRE(rows == 0 || (ldx >= dim && lddy >= dim && lddx >= dim && (!add || lda >= dim)),
+               "layernorm_backward: row strides must be at least dim");
+  if (workspace_bytes < i2pc_layernorm_backward_workspace_bytes(rows, dim))
+    return set_error(I2PC_EWORKSPACE, "layernorm_backward: workspace of %zu bytes, needs %zu", workspace_bytes,
+                     i2pc_layernorm_backward_workspace_bytes(rows, dim));
+  hipStream_t s = as_stream(stream);
+  float* part = static_cast<float*>(workspace);
+  using namespace lnt;
+  auto* g = static_cast<const bf16_t*>(dy);
+  auto* st = reinterpret_cast<const float2*>(stats);
+  if (x_f32)
+    LNT_DISPATCH(launch_bwd, float, g, lddy, static_cast<const float*>(x), ldx, st, gamma, static_cast<const float*>(add),
+                 lda, rows, dim, static_cast<float*>(dx), lddx, part, s);
+  else
+    LNT_DISPATCH(launch_bwd, bf16_t, g, lddy, static_cast<const bf16_t*>(x), ldx, st, gamma, static_cast<const bf16_t*>(add),
+                 lda, rows, dim, static_cast<bf16_t*>(dx), lddx, part, s);
+  hipLaunchKernelGGL(k_lnt_cols, dim3((2 * dim + 63) / 64), dim3(1024), 0, s, part, parts_for(rows, dim), dim, dgamma, dbeta);
+  return check_launch("layernorm_backward");
+}

@@ -847,3 +847,308 @@ def maxpool3s2(x, out=None):
     with _Timed("k_maxpool", 0.0, x.numel() * 2.0 + out.numel() * 2.0):
         _lib.call("i2pc_maxpool3s2", _p(x), B, H, W, C, OH, OW, pt, pl, _p(out), _stream())
     return out
+
+
+# ------------------------------------------------------------------ training steps of the encoder's operators
+_lib.register("i2pc_layernorm_train", ctypes.c_int, [c_void_p, ctypes.c_int, c_int64, c_void_p, c_void_p, ctypes.c_float,
+                                                     ctypes.c_int, ctypes.c_int, c_void_p, c_int64, c_void_p, c_void_p])
+_lib.register("i2pc_layernorm_backward_workspace_bytes", ctypes.c_size_t, [ctypes.c_int, ctypes.c_int])
+_lib.register("i2pc_layernorm_backward", ctypes.c_int, [c_void_p, c_int64, c_void_p, ctypes.c_int, c_int64, c_void_p, c_void_p,
+                                                        c_void_p, c_int64, ctypes.c_int, ctypes.c_int, c_void_p, c_int64,
+                                                        c_void_p, c_void_p, c_void_p, ctypes.c_size_t, c_void_p])
+_lib.register("i2pc_gelu_fp8", ctypes.c_int, [c_void_p, c_int64, c_int64, ctypes.c_int, c_void_p, c_int64, c_void_p, c_void_p,
+                                              c_void_p])
+_lib.register("i2pc_gelu_fp8_backward", ctypes.c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, ctypes.c_int, c_void_p,
+                                                       c_int64, c_void_p, c_int64, c_void_p])
+
+
+def _operand(t, name, shape, dtypes, like=None):
+    """Refuses a tensor that is not on the device, not of `shape` / one of `dtypes`, or whose last axis is not
+    dense; `like`: the tensor whose device it has to share."""
+    if not t.is_cuda:
+        raise _lib.I2PCError(f"{name} must be a device tensor")
+    if like is not None and t.device != like.device:
+        raise _lib.I2PCError(f"{name} is on {t.device}, not on {like.device}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: expected {' or '.join(map(str, dtypes))}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected the shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.shape and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last axis must be dense, its stride is {t.stride(-1)}")
+
+
+def _pitch(t):
+    """Row pitch of a 2-D tensor (one row has none of its own: its width)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _on_device_of(t):
+    """The device of `t` made current for a launch, where it is not already."""
+    import contextlib
+    torch = _torch()
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def layernorm_train(x, gamma, beta, eps, out=None, stats=None):
+    """LayerNorm of the rows of x [rows, dim] (fp32 or bf16, any row pitch and alignment; dim <= 8192) for a
+    training step: (y, stats) with y bf16 [rows, dim] and stats fp32 [rows, 2] = each row's (mean, 1 / std),
+    which layernorm_backward reads.  gamma, beta: fp32 [dim].  Rows and statistics are held in fp32."""
+    torch = _torch()
+    if x.dim() != 2:
+        raise ValueError(f"x: expected [rows, dim], got the shape {tuple(x.shape)}")
+    rows, dim = x.shape
+    f32 = (torch.float32,)
+    _operand(x, "x", (rows, dim), (torch.float32, torch.bfloat16))
+    _operand(gamma, "gamma", (dim,), f32, x)
+    _operand(beta, "beta", (dim,), f32, x)
+    with _on_device_of(x):
+        if out is None:
+            out = torch.empty((rows, dim), dtype=torch.bfloat16, device=x.device)
+        else:
+            _operand(out, "out", (rows, dim), (torch.bfloat16,), x)
+        if stats is None:
+            stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
+        else:
+            _operand(stats, "stats", (rows, 2), f32, x)
+            if not stats.is_contiguous():
+                raise ValueError("stats must be contiguous")
+        with _Timed("k_lnt_fwd", 0.0, rows * dim * (x.element_size() + 2.0) + 8.0 * rows):
+            _lib.call("i2pc_layernorm_train", _p(x), int(x.dtype == torch.float32), _pitch(x), _p(gamma), _p(beta),
+                      float(eps), rows, dim, _p(out), _pitch(out), _p(stats), _stream())
+    return out, stats
+
+
+def layernorm_backward(dy, x, stats, gamma, add=None, dx=None, dgamma=None, dbeta=None):
+    """Gradients of layernorm_train: (dx, dgamma, dbeta) from dy bf16 [rows, dim], the x and stats of the forward
+    pass and gamma.  dx has x's type; add (x's type): a gradient added to it before its rounding (the residual
+    stream's), dx may be add itself.  dgamma, dbeta: fp32 [dim], summed in fp32 in a fixed order."""
+    torch = _torch()
+    if x.dim() != 2:
+        raise ValueError(f"x: expected [rows, dim], got the shape {tuple(x.shape)}")
+    rows, dim = x.shape
+    f32 = (torch.float32,)
+    _operand(x, "x", (rows, dim), (torch.float32, torch.bfloat16))
+    _operand(dy, "dy", (rows, dim), (torch.bfloat16,), x)
+    _operand(stats, "stats", (rows, 2), f32, x)
+    if not stats.is_contiguous():
+        raise ValueError("stats must be contiguous")
+    _operand(gamma, "gamma", (dim,), f32, x)
+    if add is not None:
+        _operand(add, "add", (rows, dim), (x.dtype,), x)
+    with _on_device_of(x):
+        if dx is None:
+            dx = torch.empty((rows, dim), dtype=x.dtype, device=x.device)
+        else:
+            _operand(dx, "dx", (rows, dim), (x.dtype,), x)
+        dgamma = _column_sums(dgamma, "dgamma", dim, x)
+        dbeta = _column_sums(dbeta, "dbeta", dim, x)
+        nb = _lib.load().i2pc_layernorm_backward_workspace_bytes(rows, dim)
+        ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
+        e = x.element_size()
+        with _Timed("k_lnt_bwd", 0.0, rows * dim * (2.0 + 2.0 * e + (e if add is not None else 0)) + 12.0 * dim):
+            _lib.call("i2pc_layernorm_backward", _p(dy), _pitch(dy), _p(x), int(x.dtype == torch.float32), _pitch(x),
+                      _p(stats), _p(gamma), _p(add), 0 if add is None else _pitch(add), rows, dim, _p(dx), _pitch(dx),
+                      _p(dgamma), _p(dbeta), _p(ws), nb, _stream())
+    return dx, dgamma, dbeta
+
+
+def _column_sums(t, name, dim, like):
+    torch = _torch()
+    if t is None:
+        return torch.empty(dim, dtype=torch.float32, device=like.device)
+    _operand(t, name, (dim,), (torch.float32,), like)
+    return t
+
+
+def gelu_fp8(x, out=None, kept=None):
+    """GELU (the erf form) of bf16 rows x [rows, dim], dim % 32 == 0: (y, kept) with y bf16 and kept the Fp8 rows
+    of x (quant_fp8's block rule) that gelu_fp8_backward works from: 1.03 bytes a value instead of two."""
+    torch = _torch()
+    if x.dim() != 2:
+        raise ValueError(f"x: expected [rows, dim], got the shape {tuple(x.shape)}")
+    rows, dim = x.shape
+    _operand(x, "x", (rows, dim), (torch.bfloat16,))
+    with _on_device_of(x):
+        if out is None:
+            out = torch.empty((rows, dim), dtype=torch.bfloat16, device=x.device)
+        else:
+            _operand(out, "out", (rows, dim), (torch.bfloat16,), x)
+        if kept is None:
+            kept = empty_fp8((rows, dim), x.device)
+        else:
+            _kept_operand(kept, rows, dim, x)
+        with _Timed("k_gelu_keep", 0.0, rows * dim * (5.0 + 1.0 / 32)):
+            _lib.call("i2pc_gelu_fp8", _p(x), _pitch(x), rows, dim, _p(out), _pitch(out), _p(kept.data), _p(kept.scale),
+                      _stream())
+    return out, kept
+
+
+def gelu_fp8_backward(dy, kept, dx=None, again=None, recompute=False):
+    """dx = dy * GELU'(x~) (bf16) from dy bf16 [rows, dim] and the Fp8 rows x~ that gelu_fp8 kept; with recompute
+    (or an `again` to write to): (dx, again), again = GELU(x~) in bf16, for the next linear layer's weight
+    gradient."""
+    torch = _torch()
+    if dy.dim() != 2:
+        raise ValueError(f"dy: expected [rows, dim], got the shape {tuple(dy.shape)}")
+    rows, dim = dy.shape
+    _operand(dy, "dy", (rows, dim), (torch.bfloat16,))
+    _kept_operand(kept, rows, dim, dy)
+    with _on_device_of(dy):
+        if dx is None:
+            dx = torch.empty((rows, dim), dtype=torch.bfloat16, device=dy.device)
+        else:
+            _operand(dx, "dx", (rows, dim), (torch.bfloat16,), dy)
+        if again is not None:
+            _operand(again, "again", (rows, dim), (torch.bfloat16,), dy)
+        elif recompute:
+            again = torch.empty((rows, dim), dtype=torch.bfloat16, device=dy.device)
+        nbytes = rows * dim * (5.0 + 1.0 / 32 + (2.0 if again is not None else 0.0))
+        with _Timed("k_gelu_back", 0.0, nbytes):
+            _lib.call("i2pc_gelu_fp8_backward", _p(dy), _pitch(dy), _p(kept.data), _p(kept.scale), rows, dim, _p(dx),
+                      _pitch(dx), _p(again), 0 if again is None else _pitch(again), _stream())
+    return dx if again is None else (dx, again)
+
+
+def _kept_operand(kept, rows, dim, like):
+    torch = _torch()
+    if not isinstance(kept, Fp8):
+        raise TypeError(f"kept: expected Fp8 rows, got {type(kept).__name__}")
+    if dim % 32:
+        raise ValueError(f"dim={dim} must be a multiple of 32")
+    _operand(kept.data, "kept.data", (rows, dim), (torch.uint8,), like)
+    _operand(kept.scale, "kept.scale", (rows, dim // 32), (torch.uint8,), like)
+    if not (kept.data.is_contiguous() and kept.scale.is_contiguous()):
+        raise ValueError("kept must be contiguous")
+
+
+# ------------------------------------------------------------------ attention over packed sequences
+class AttnPackedDesc(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p),
+                ("q_t", c_int64), ("q_h", c_int64), ("k_t", c_int64), ("k_h", c_int64), ("v_t", c_int64), ("v_h", c_int64),
+                ("out", c_void_p), ("o_t", c_int64), ("o_h", c_int64), ("lse", c_void_p),
+                ("cu_q", c_void_p), ("cu_k", c_void_p), ("k_lens", c_void_p),
+                ("batch", c_int32), ("total_q", c_int32), ("total_k", c_int32), ("heads", c_int32), ("kv_heads", c_int32),
+                ("head_dim", c_int32), ("causal", c_int32), ("zero_tail", c_int32), ("scale", ctypes.c_float)]
+
+
+class AttnPackedGradDesc(ctypes.Structure):
+    _fields_ = [("f", AttnPackedDesc), ("dout", c_void_p), ("d_t", c_int64), ("d_h", c_int64),
+                ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p),
+                ("dq_t", c_int64), ("dq_h", c_int64), ("dk_t", c_int64), ("dk_h", c_int64), ("dv_t", c_int64),
+                ("dv_h", c_int64)]
+
+
+_lib.register("i2pc_attention_packed_workspace_bytes", ctypes.c_size_t, [ctypes.POINTER(AttnPackedDesc)])
+_lib.register("i2pc_attention_packed", ctypes.c_int, [ctypes.POINTER(AttnPackedDesc), c_void_p, ctypes.c_size_t, c_void_p])
+_lib.register("i2pc_attention_packed_backward_workspace_bytes", ctypes.c_size_t, [ctypes.POINTER(AttnPackedGradDesc)])
+_lib.register("i2pc_attention_packed_backward", ctypes.c_int, [ctypes.POINTER(AttnPackedGradDesc), c_void_p, ctypes.c_size_t,
+                                                               c_void_p])
+
+
+def _attn_packed_desc(d, q, k, v, cu_q, cu_k, k_lens, scale, causal):
+    """Checks the operands of a packed attention call and fills the descriptor's input side."""
+    torch = _torch()
+    bf = (torch.bfloat16,)
+    i32 = (torch.int32,)
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"q, k: expected [tokens, heads, head_dim], got the shapes {tuple(q.shape)}, {tuple(k.shape)}")
+    tq, heads, hd = q.shape
+    tk, kv = k.shape[0], k.shape[1]
+    _operand(q, "q", q.shape, bf)
+    _operand(k, "k", (tk, kv, hd), bf, q)
+    _operand(v, "v", (tk, kv, hd), bf, q)
+    if cu_q.dim() != 1 or cu_q.shape[0] < 2:
+        raise ValueError(f"cu_q: expected int32 [sequences + 1] of one sequence at least, got the shape {tuple(cu_q.shape)}")
+    batch = cu_q.shape[0] - 1
+    _operand(cu_q, "cu_q", (batch + 1,), i32, q)
+    if cu_k is None:
+        if tk != tq:
+            raise ValueError(f"k has {tk} rows and q {tq}: give cu_k")
+        cu_k = cu_q
+    _operand(cu_k, "cu_k", (batch + 1,), i32, q)
+    if k_lens is not None:
+        _operand(k_lens, "k_lens", (batch,), i32, q)
+    d.q, d.q_t, d.q_h = _p(q), q.stride(0), q.stride(1)
+    d.k, d.k_t, d.k_h = _p(k), k.stride(0), k.stride(1)
+    d.v, d.v_t, d.v_h = _p(v), v.stride(0), v.stride(1)
+    d.cu_q, d.cu_k, d.k_lens = _p(cu_q), _p(cu_k), _p(k_lens)
+    d.batch, d.total_q, d.total_k, d.heads, d.kv_heads, d.head_dim = batch, tq, tk, heads, kv, hd
+    d.causal = int(bool(causal))
+    d.scale = hd ** -0.5 if scale is None else float(scale)
+
+
+def attention_packed(q, k, v, cu_q, cu_k=None, k_lens=None, scale=None, causal=False, out=None, lse=None):
+    """Softmax attention over packed sequences (i2pc_attention_packed): (out, lse).
+
+    q bf16 [total_q, heads, 64], k / v bf16 [total_k, kv_heads, 64]: any strides that are multiples of 8 values (the
+    slices of a [tokens, 3, heads, 64] QKV buffer, a cache), heads a multiple of kv_heads.  cu_q / cu_k: int32
+    [sequences + 1] on the device, rising from 0; sequence b's queries are the rows cu_q[b] .. cu_q[b + 1], its keys the
+    rows from cu_k[b] on, up to cu_k[b + 1] or k_lens[b] of them (int32 [sequences]: the filled part of a cache's
+    slab).  cu_k None: the keys are packed as the queries are.  The lengths are read on the device when the kernel
+    runs.  causal: query i of lq sees the keys j <= i + lk - lq of lk.  scale defaults to 1 / 8.
+    out bf16 [total_q, heads, 64]; lse fp32 [total_q, heads] = log(sum(exp(scores))).  A query that sees no key has
+    out 0, lse -inf.  Rows behind the last sequence keep what a given `out` / `lse` holds, and are 0 / -inf in new ones.
+    """
+    torch = _torch()
+    d = AttnPackedDesc()
+    _attn_packed_desc(d, q, k, v, cu_q, cu_k, k_lens, scale, causal)
+    with _on_device_of(q):
+        d.zero_tail = int(out is None)
+        if (out is None) != (lse is None):
+            raise ValueError("give both out and lse, or neither")
+        if out is None:
+            out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        else:
+            _operand(out, "out", q.shape, (torch.bfloat16,), q)
+            _operand(lse, "lse", q.shape[:2], (torch.float32,), q)
+            if not lse.is_contiguous():
+                raise ValueError("lse must be contiguous")
+        d.out, d.o_t, d.o_h, d.lse = _p(out), out.stride(0), out.stride(1), _p(lse)
+        nb = _lib.load().i2pc_attention_packed_workspace_bytes(ctypes.byref(d))
+        ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
+        # flops of the dense bound are not known here (the lengths are on the device)
+        with _Timed("k_attnp_fwd", 0.0, 2.0 * (2 * q.numel() + k.numel() + v.numel()) + 4.0 * lse.numel()):
+            _lib.call("i2pc_attention_packed", ctypes.byref(d), _p(ws), nb, _stream())
+    return out, lse
+
+
+def attention_packed_backward(dout, q, k, v, out, lse, cu_q, cu_k=None, scale=None, causal=False, dq=None, dk=None, dv=None):
+    """Gradients of attention_packed (i2pc_attention_packed_backward): (dq, dk, dv), bf16, from dout bf16 [total_q,
+    heads, 64], the forward call's operands and its (out, lse).  dk, dv are summed over the query heads that share a key
+    head; all sums are fp32 in a fixed order.  Rows behind the last sequence keep what a given dq / dk / dv holds (give all
+    three, or none), and are 0 in new ones."""
+    torch = _torch()
+    g = AttnPackedGradDesc()
+    d = g.f
+    bf = (torch.bfloat16,)
+    _attn_packed_desc(d, q, k, v, cu_q, cu_k, None, scale, causal)
+    _operand(dout, "dout", q.shape, bf, q)
+    _operand(out, "out", q.shape, bf, q)
+    _operand(lse, "lse", q.shape[:2], (torch.float32,), q)
+    if not lse.is_contiguous():
+        raise ValueError("lse must be contiguous")
+    given = [t is not None for t in (dq, dk, dv)]
+    if any(given) and not all(given):
+        raise ValueError("give all of dq, dk, dv, or none")
+    with _on_device_of(q):
+        d.zero_tail = int(not any(given))
+        if any(given):
+            _operand(dq, "dq", q.shape, bf, q)
+            _operand(dk, "dk", k.shape, bf, q)
+            _operand(dv, "dv", v.shape, bf, q)
+        else:
+            dq = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+            dk = torch.empty(k.shape, dtype=torch.bfloat16, device=q.device)
+            dv = torch.empty(v.shape, dtype=torch.bfloat16, device=q.device)
+        d.out, d.o_t, d.o_h, d.lse = _p(out), out.stride(0), out.stride(1), _p(lse)
+        g.dout, g.d_t, g.d_h = _p(dout), dout.stride(0), dout.stride(1)
+        g.dq, g.dq_t, g.dq_h = _p(dq), dq.stride(0), dq.stride(1)
+        g.dk, g.dk_t, g.dk_h = _p(dk), dk.stride(0), dk.stride(1)
+        g.dv, g.dv_t, g.dv_h = _p(dv), dv.stride(0), dv.stride(1)
+        nb = _lib.load().i2pc_attention_packed_backward_workspace_bytes(ctypes.byref(g))
+        ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
+        nbytes = 2.0 * (4 * q.numel() + 2 * k.numel() + 2 * v.numel()) + 4.0 * lse.numel()
+        with _Timed("k_attnp_bwd", 0.0, nbytes):
+            _lib.call("i2pc_attention_packed_backward", ctypes.byref(g), _p(ws), nb, _stream())
+    return dq, dk, dv

@@ -567,6 +567,66 @@ int i2pc_depth_forward(i2pc_model* model, const uint8_t* bgr, float* depth, void
 int i2pc_model_file_info(const char* path, int32_t* ints32, float* floats16, int* ntensors);
 
 /* ------------------------------------------------------------------------
+ * Training steps of the encoder's operators: LayerNorm and GELU with their gradients, and attention over
+ * packed sequences with its gradients.
+ * ------------------------------------------------------------------------ */
+/* y = (x - mean) / std * gamma + beta per row, std = sqrt(var + eps); x [rows][ldx] fp32 (x_f32) or bf16,
+ * any alignment; y bf16 [rows][ldy]; stats fp32 [rows][2] = (mean, 1 / std).  0 < dim <= 8192; rows may be 0. */
+int i2pc_layernorm_train(const void* x, int x_f32, int64_t ldx, const float* gamma, const float* beta, float eps,
+                         int rows, int dim, void* y, int64_t ldy, float* stats, void* stream);
+/* Its gradients from dy bf16 [rows][lddy]: dx (x's type) [rows][lddx] (+ add, x's type [rows][lda], or NULL; dx may
+ * be add, no other output may overlap an input), dgamma and dbeta fp32 [dim] (written, not added to; zero for
+ * rows 0).  The workspace holds partial column sums; its contents do not matter before or after. */
+size_t i2pc_layernorm_backward_workspace_bytes(int rows, int dim);
+int i2pc_layernorm_backward(const void* dy, int64_t lddy, const void* x, int x_f32, int64_t ldx, const float* stats,
+                            const float* gamma, const void* add, int64_t lda, int rows, int dim, void* dx, int64_t lddx,
+                            float* dgamma, float* dbeta, void* workspace, size_t workspace_bytes, void* stream);
+/* y = GELU(x) (erf form) of bf16 rows, and x kept as MX fp8 (i2pc_quant_fp8's block rule): kept e4m3 [rows][dim],
+ * kept_scale E8M0 [rows][dim / 32], both dense.  dim % 32 == 0; row pitches multiples of 8, 16-byte aligned. */
+int i2pc_gelu_fp8(const void* x, int64_t ldx, int64_t rows, int dim, void* y, int64_t ldy, void* kept, void* kept_scale,
+                  void* stream);
+/* dx = dy GELU'(x~) of the kept x~, and with `again` not NULL also again = GELU(x~); bf16 rows. */
+int i2pc_gelu_fp8_backward(const void* dy, int64_t lddy, const void* kept, const void* kept_scale, int64_t rows, int dim,
+                           void* dx, int64_t lddx, void* again, int64_t ld_again, void* stream);
+
+/* Attention over packed sequences.  Sequence b's queries are the rows [cu_q[b], cu_q[b + 1]) of q, out, lse, its
+ * keys the rows from cu_k[b] of k, v: cu_k[b + 1] - cu_k[b] of them, or k_lens[b] (at most that many) where k_lens
+ * is given -- a cache with a slab of slots for each sequence.  cu_q, cu_k: int32 [batch + 1] on the device, rising,
+ * cu_q[0] = 0; the kernels read them when they run, so a captured graph follows their contents, and hold what they
+ * say to total_q / total_k rows.  Element (row t, head h) of q starts at q + t * q_t + h * q_h elements (out, k, v
+ * alike) and its head_dim = 64 bf16 values are dense; query head h reads key head h / (heads / kv_heads).
+ *   S = scale Q K^T; causal: query i of a sequence of lq queries and lk keys sees keys j <= i + lk - lq;
+ *   out = softmax(S) V, lse [total_q][heads] = log(sum exp(S)) (fp32); a query that sees no key has out = 0,
+ *   lse = -inf.
+ * Rows behind the last sequence are left as they were, or zero (lse -inf) with zero_tail. */
+typedef struct i2pc_attn_packed_desc {
+  const void *q, *k, *v;
+  int64_t q_t, q_h, k_t, k_h, v_t, v_h;
+  void* out;
+  int64_t o_t, o_h;
+  float* lse;
+  const int32_t *cu_q, *cu_k, *k_lens;
+  int32_t batch, total_q, total_k, heads, kv_heads, head_dim, causal, zero_tail;
+  float scale;                   /* > 0 */
+} i2pc_attn_packed_desc;
+/* Scratch memory of the call (0 where its keys are not split); contents do not matter before or after. */
+size_t i2pc_attention_packed_workspace_bytes(const i2pc_attn_packed_desc* desc);
+int i2pc_attention_packed(const i2pc_attn_packed_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients from dout and the forward's out and lse (desc as in the forward call, k_lens NULL): dq, dk, dv with the
+ * shapes of q, k, v and their own strides.  Sums over the queries, and over the query heads that share a key head,
+ * are fp32 in a fixed order.  Rows behind the last sequence are left as they were, or zero with zero_tail. */
+typedef struct i2pc_attn_packed_grad_desc {
+  i2pc_attn_packed_desc f;
+  const void* dout;
+  int64_t d_t, d_h;
+  void *dq, *dk, *dv;
+  int64_t dq_t, dq_h, dk_t, dk_h, dv_t, dv_h;
+} i2pc_attn_packed_grad_desc;
+size_t i2pc_attention_packed_backward_workspace_bytes(const i2pc_attn_packed_grad_desc* desc);
+int i2pc_attention_packed_backward(const i2pc_attn_packed_grad_desc* desc, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/* ------------------------------------------------------------------------
  * Artefact writers (save_point_cloud, backend/app.py:310-389) from HOST buffers
  * (xyz float32 [n][3], rgb uint8 [n][3] or NULL for grey 128). Not stream-ordered.
  * ------------------------------------------------------------------------ */

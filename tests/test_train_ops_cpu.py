@@ -1,0 +1,172 @@
+"""Refusals of the training operators and of packed attention: no device work (CPU tensors, or descriptors that the C side
+turns down before it launches anything)."""
+import ctypes
+import os
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from image_to_pointcloud_amd import _lib, ops  # noqa: E402
+
+
+def _built():
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("libi2pc.so not built")
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(4, 64)
+    b = x.to(torch.bfloat16)
+    g = torch.ones(64)
+    with pytest.raises(_lib.I2PCError):
+        ops.layernorm_train(x, g, g, 1e-6)
+    with pytest.raises(_lib.I2PCError):
+        ops.layernorm_backward(b, x, torch.zeros(4, 2), g)
+    with pytest.raises(_lib.I2PCError):
+        ops.gelu_fp8(b)
+    with pytest.raises(_lib.I2PCError):
+        ops.gelu_fp8_backward(b, ops.Fp8(torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)))
+    q = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(_lib.I2PCError):
+        ops.attention_packed(q, q, q, cu)
+    with pytest.raises(_lib.I2PCError):
+        ops.attention_packed_backward(q, q, q, q, q, torch.zeros(4, 2), cu)
+
+
+class _Device:
+    """A CPU tensor that says it is on the device: what Python checks before any call into the library."""
+
+    def __init__(self, t):
+        self._t = t
+        self.is_cuda = True
+
+    def __getattr__(self, n):
+        return getattr(self._t, n)
+
+
+def test_shapes_types_and_strides():
+    bf = torch.bfloat16
+    op = ops._operand
+    op(_Device(torch.zeros(3, 4)), "t", (3, 4), (torch.float32,))
+    with pytest.raises(TypeError):
+        op(_Device(torch.zeros(3, 4)), "t", (3, 4), (bf,))
+    with pytest.raises(ValueError):
+        op(_Device(torch.zeros(3, 5)), "t", (3, 4), (torch.float32,))
+    with pytest.raises(ValueError):
+        op(_Device(torch.zeros(4, 3).t()), "t", (3, 4), (torch.float32,))
+    with pytest.raises(ValueError):
+        ops.layernorm_train(torch.zeros(2, 3, 4), None, None, 1e-6)
+    with pytest.raises(ValueError):
+        ops.gelu_fp8(torch.zeros(2, 3, 4))
+    with pytest.raises(TypeError):
+        ops._kept_operand(torch.zeros(2, 32), 2, 32, None)
+    with pytest.raises(ValueError):
+        ops._kept_operand(ops.Fp8(None, None), 2, 33, None)
+    q = _Device(torch.zeros(4, 2, 64, dtype=bf))
+    for bad_cu in (torch.zeros(1, dtype=torch.int32), torch.zeros(2, 2, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            ops.attention_packed(q, q, q, bad_cu)
+    with pytest.raises(ValueError):                                      # other rows than q's need a cu_k
+        ops.attention_packed(q, *[_Device(torch.zeros(5, 2, 64, dtype=bf))] * 2, _Device(torch.zeros(2, dtype=torch.int32)))
+
+
+def _rc(name, *args):
+    lib = _lib.load()
+    rc = getattr(lib, name)(*args)
+    return rc, lib.i2pc_last_error().decode()
+
+
+def test_layernorm_refusals():
+    _built()
+    train = lambda rows, dim, x=16, ldx=None: _rc("i2pc_layernorm_train", x, 1, ldx or dim, 16, 16, 1e-6, rows, dim, 16, dim,  # noqa: E731
+                                                  16, None)
+    assert train(0, 64) == (0, "")
+    for rows, dim, kw in ((-1, 64, {}), (4, 0, {}), (4, 8193, {}), (4, 64, {"x": None}), (4, 64, {"ldx": 63})):
+        rc, msg = train(rows, dim, **kw)
+        assert rc == -1 and msg, (rows, dim, kw)
+    lib = _lib.load()
+    need = lib.i2pc_layernorm_backward_workspace_bytes(100, 384)
+    assert need > 0 and lib.i2pc_layernorm_backward_workspace_bytes(100, 9000) == 0
+
+    def backward(rows=100, dim=384, lda=384, ws=16, nb=need, dx=16):
+        return _rc("i2pc_layernorm_backward", 16, dim, 16, 1, dim, 16, 16, 16, lda, rows, dim, dx, dim, 16, 16, ws, nb, None)
+    assert backward(nb=need - 1)[0] == -2
+    for kw in ({"rows": -1}, {"dim": 9000}, {"lda": 100}, {"ws": None}, {"dx": None}):
+        assert backward(**kw)[0] == -1, kw
+
+
+def test_gelu_refusals():
+    _built()
+    for rows, dim, ld, p in ((4, 33, 64, 16), (4, 0, 64, 16), (-1, 64, 64, 16), (4, 64, 60, 16), (4, 64, 68, 16), (4, 64, 64, 18),
+                             (4, 64, 64, None)):
+        assert _rc("i2pc_gelu_fp8", p, ld, rows, dim, 16, 64, 16, 16, None)[0] == -1, (rows, dim, ld, p)
+        assert _rc("i2pc_gelu_fp8_backward", p, ld, 16, 16, rows, dim, 16, 64, None, 0, None)[0] == -1, (rows, dim, ld, p)
+    assert _rc("i2pc_gelu_fp8", 16, 64, 1 << 40, 64, 16, 64, 16, 16, None)[0] == -4
+    assert _rc("i2pc_gelu_fp8", None, 64, 0, 64, None, 64, None, None, None) == (0, "")
+
+
+def _desc(**kw):
+    d = ops.AttnPackedDesc()
+    for n in ("q", "k", "v", "out", "lse", "cu_q", "cu_k"):
+        setattr(d, n, 16)
+    for n in ("q", "k", "v", "o"):
+        setattr(d, n + "_t", 256)
+        setattr(d, n + "_h", 64)
+    d.batch, d.total_q, d.total_k, d.heads, d.kv_heads, d.head_dim, d.scale = 2, 100, 100, 4, 4, 64, 0.125
+    for n, x in kw.items():
+        setattr(d, n, x)
+    return d
+
+
+BAD = [({"head_dim": 128}, -4), ({"kv_heads": 3}, -1), ({"heads": 0}, -1), ({"total_q": -1}, -1), ({"batch": -1}, -1),
+       ({"scale": 0.0}, -1), ({"scale": -1.0}, -1), ({"scale": float("nan")}, -1), ({"scale": float("inf")}, -1),
+       ({"q": 24}, -1), ({"k_t": 252}, -1), ({"v_h": 60}, -1), ({"k_t": 0}, -1), ({"o_h": 0}, -1), ({"q_t": 1 << 23}, -1),
+       ({"cu_q": None}, -1), ({"cu_k": None}, -1), ({"lse": None}, -1), ({"q": None}, -1), ({"total_q": 1 << 30}, -4),
+       ({"total_k": (1 << 31) - 1, "kv_heads": 4}, -4)]
+
+
+@pytest.mark.parametrize("kw,code", BAD, ids=[",".join(k) for k, _ in BAD])
+def test_attention_refusals(kw, code):
+    _built()
+    d = _desc(**kw)
+    rc, msg = _rc("i2pc_attention_packed", ctypes.byref(d), 16, 1 << 40, None)
+    assert rc == code and msg
+    g = ops.AttnPackedGradDesc()
+    g.f = d
+    for n in ("dout", "dq", "dk", "dv"):
+        setattr(g, n, 16)
+    for n in ("d", "dq", "dk", "dv"):
+        setattr(g, n + "_t", 256)
+        setattr(g, n + "_h", 64)
+    assert _rc("i2pc_attention_packed_backward", ctypes.byref(g), 16, 1 << 40, None)[0] == code
+    assert _lib.load().i2pc_attention_packed_workspace_bytes(ctypes.byref(d)) == 0
+
+
+def test_attention_workspaces_and_the_backward_pass_own_refusals():
+    _built()
+    lib = _lib.load()
+    d = _desc(batch=1, total_q=1, total_k=100000, q_t=256)
+    need = lib.i2pc_attention_packed_workspace_bytes(ctypes.byref(d))
+    assert need > 0                                                      # one token over many keys: they are split
+    assert _rc("i2pc_attention_packed", ctypes.byref(d), 16, need - 1, None)[0] == -2
+    assert _rc("i2pc_attention_packed", ctypes.byref(d), None, need, None)[0] == -2
+    # the split takes the workspace from the totals alone, and no more shares than 256 keys each allow
+    assert lib.i2pc_attention_packed_workspace_bytes(ctypes.byref(_desc(batch=1, total_q=1, total_k=256))) == 0
+    assert lib.i2pc_attention_packed_workspace_bytes(ctypes.byref(_desc(batch=8, total_q=70000, total_k=70000))) == 0
+    g = ops.AttnPackedGradDesc()
+    g.f = _desc()
+    for n in ("dout", "dq", "dk", "dv"):
+        setattr(g, n, 16)
+    for n in ("d", "dq", "dk", "dv"):
+        setattr(g, n + "_t", 256)
+        setattr(g, n + "_h", 64)
+    need = lib.i2pc_attention_packed_backward_workspace_bytes(ctypes.byref(g))
+    assert need > 0 and _rc("i2pc_attention_packed_backward", ctypes.byref(g), 16, need - 1, None)[0] == -2
+    g.f.k_lens = 16
+    assert _rc("i2pc_attention_packed_backward", ctypes.byref(g), 16, need, None)[0] == -1
+    g.f.k_lens = None
+    g.dk_h = 0
+    assert _rc("i2pc_attention_packed_backward", ctypes.byref(g), 16, need, None)[0] == -1
+    assert _rc("i2pc_attention_packed", ctypes.byref(_desc(total_q=0)), None, 0, None) == (0, "")

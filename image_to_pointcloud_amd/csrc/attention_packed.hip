@@ -232,11 +232,122 @@ __device__ __forceinline__ void zero_rows(bf16_t* out, int64_t o_t, int64_t o_h,
 }
 
 // ------------------------------------------------------------------ forward
+// A row's running state, a row to a lane (its two lane halves hold different keys' probabilities and different d of O).
+struct Rows {
+  f32x16 o[2];                   // O^T, not normalised
+  f32x16 nm;                     // minus the reference m, in units of the raw scores, all 16 alike
+  float l;                       // this half's sum of 2^(c (s - m))
+  int bad;                       // met an infinity or NaN in a partly masked block
+  __device__ __forceinline__ void clear() {
+    for (int i = 0; i < 16; ++i) o[0][i] = o[1][i] = nm[i] = 0.f;
+    l = 0.f;
+    bad = 0;
+  }
+};
+
+// 32 keys (rows base .. base + 31 of the K and V tiles) for 32 rows.  S^T = K Q^T starts at -m (the accumulator's start
+// value), so p = 2^(c s); m moves only when a probability could pass 2^8 (harmless for the bf16 operand and the fp32
+// sums), so the usual block has no maximum and no rescale.  `first`: the rows' first block, which sets m.  left: how many
+// of the block's keys the lane's row sees; partial (uniform): not all of them for some row of the wave.
+template <bool CAUSAL>
+__device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const uint8_t* sK, const uint8_t* sV, int base, bool first,
+                                       bool partial, int left, float c, int lane) {
+  constexpr float kThresh = 256.f;
+  const int hh = lane >> 5, lr = lane & 31;
+  bf16x8 kf[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) kf[t] = row_frag(sK, base + lr, t, hh);
+  f32x16 st;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) st = mfma(kf[t], qf[t], t == 0 ? w.nm : st);
+  if (partial) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if ((i & 3) + 8 * (i >> 2) + 4 * hh >= left) st[i] = -INFINITY;
+  }
+  float ls = 0.f;
+  uint32_t pk[8];
+  auto probs = [&](float sub) {                      // sub: in units of the raw scores
+    ls = 0.f;
+    const float nsub = -sub * c;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(st[i], c, nsub));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(st[i + 1], c, nsub));
+      ls += p0 + p1;
+      pk[i >> 1] = pack_bf16(p0, p1);
+    }
+  };
+  bool full = first;
+  if (!full) {
+    probs(0.f);
+    full = __ballot(ls >= kThresh) != 0;
+  }
+  if (full) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[i]);
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+    mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+    // a row that sees nothing here keeps its reference
+    const float delta = first ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, 0.f);
+    probs(delta);
+    if (!first) {
+      const float alpha = __builtin_amdgcn_exp2f(-delta * c);
+      w.l *= alpha;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        w.o[0][i] *= alpha;
+        w.o[1][i] *= alpha;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w.nm[i] -= delta;
+  }
+  w.l += ls;
+  bf16x8 vf[2][2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) vf[t][dt] = tr_frag(sV, base + 16 * t, dt, lane);
+  if (CAUSAL && partial) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) w.bad |= (int)nonfinite(vf[t][0]) | (int)nonfinite(vf[t][1]);
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) w.o[dt] = mfma(vf[t][dt], p_frag(pk, t), w.o[dt]);
+}
+
+// The state of the keys [from, to) again, key by key: rows that `bad` says need it.
+__device__ __forceinline__ void attend_again(Rows& w, const bf16x8 (&qf)[4], const bf16_t* K, int64_t k_t, const bf16_t* V,
+                                             int64_t v_t, int from, int to, int step, int nk, float c, int hh) {
+  float m = -INFINITY, l = 0.f;
+  w.clear();
+#pragma clang loop unroll(disable)
+  for (int j = from; j < to; j += (j & 31) == 31 ? step : 1) {
+    const float x = dot_row(K + j * k_t, qf, hh);
+    if (j < nk) {
+      const float m_new = fmaxf(m, x), alpha = m == m_new ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
+      const float p = __builtin_amdgcn_exp2f((x - m_new) * c);
+      m = m_new;
+      l = fmaf(l, alpha, p);
+      for (int i = 0; i < 16; ++i) {
+        w.o[0][i] *= alpha;
+        w.o[1][i] *= alpha;
+      }
+      add_row(w.o, p, V + j * v_t, hh);
+    }
+  }
+  for (int i = 0; i < 16; ++i) w.nm[i] = m == -INFINITY ? 0.f : -m;
+  w.l = hh ? 0.f : l;                                // the whole sum; the halves' are added
+}
+
 // One workgroup: 128 packed rows of one key head, over all of their keys or (SPLIT) over one of nsplit shares of
 // them.  Each wave owns 32 rows, a row to a lane: S^T = K Q^T leaves a query's scores in one lane's
 // registers, which then are the B operand of O^T += V^T P^T.  K and V tiles of 64 keys go through LDS by
-// LDS-DMA, double-buffered.  The scores start at minus the row's reference m (the accumulator's start value);
-// m moves only when a probability could pass 2^8, so the usual tile has no maximum and no rescale.
+// LDS-DMA, double-buffered.
 template <bool CAUSAL, bool SPLIT>
 __global__ __launch_bounds__(256, 3) void k_attnp_fwd(const Args a) {
   __shared__ __attribute__((aligned(16))) uint8_t smem[4 * kTileBytes];
@@ -290,118 +401,27 @@ __global__ __launch_bounds__(256, 3) void k_attnp_fwd(const Args a) {
   __syncthreads();
 
   const float c = a.c;
-  f32x16 o[2], nm;
-  for (int i = 0; i < 16; ++i) o[0][i] = o[1][i] = nm[i] = 0.f;
-  float l = 0.f;
-  int bad = 0;
-  constexpr float kThresh = 256.f;
-
+  Rows w;
+  w.clear();
   for (int key0 = ks, cur = 0; key0 < ke; key0 += kKV, cur ^= 1) {
     if (key0 + kKV < ke) stage(cur ^ 1, key0 + kKV);
     const uint8_t* sK = smem + cur * 2 * kTileBytes;
-    const uint8_t* sV = sK + kTileBytes;
     if (wave_on) {
 #pragma unroll
       for (int k2 = 0; k2 < 2; ++k2) {
-        if (key0 + 32 * k2 >= nk_last) break;        // no row of the wave sees these keys
-        bf16x8 kf[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) kf[t] = row_frag(sK, 32 * k2 + lr, t, hh);
-        f32x16 st;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) st = mfma(kf[t], qf[t], t == 0 ? nm : st);
-        const bool partial = key0 + 32 * k2 + 32 > nk_first;    // uniform
-        const int left = nk - key0 - 32 * k2;
-        if (partial) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if ((i & 3) + 8 * (i >> 2) + 4 * hh >= left) st[i] = -INFINITY;
-        }
-        float ls = 0.f;
-        uint32_t pk[8];
-        auto probs = [&](float sub) {                // sub: in units of the raw scores
-          ls = 0.f;
-          const float nsub = -sub * c;
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(st[i], c, nsub));
-            const float p1 = __builtin_amdgcn_exp2f(fmaf(st[i + 1], c, nsub));
-            ls += p0 + p1;
-            pk[i >> 1] = pack_bf16(p0, p1);
-          }
-        };
-        const bool first = key0 == ks && k2 == 0;
-        bool full = first;
-        if (!full) {
-          probs(0.f);
-          full = __ballot(ls >= kThresh) != 0;
-        }
-        if (full) {
-          float mx = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[i]);
-          const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-          mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-          // a row that sees nothing here keeps its reference
-          const float delta = first ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, 0.f);
-          probs(delta);
-          if (!first) {
-            const float alpha = __builtin_amdgcn_exp2f(-delta * c);
-            l *= alpha;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              o[0][i] *= alpha;
-              o[1][i] *= alpha;
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) nm[i] -= delta;
-        }
-        l += ls;
-        bf16x8 vf[2][2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int dt = 0; dt < 2; ++dt) vf[t][dt] = tr_frag(sV, 32 * k2 + 16 * t, dt, lane);
-        if (CAUSAL && partial) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t) bad |= (int)nonfinite(vf[t][0]) + (int)nonfinite(vf[t][1]);
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int dt = 0; dt < 2; ++dt) o[dt] = mfma(vf[t][dt], p_frag(pk, t), o[dt]);
+        const int key = key0 + 32 * k2;
+        if (key >= nk_last) break;                   // no row of the wave sees these keys
+        attend<CAUSAL>(w, qf, sK, sK + kTileBytes, 32 * k2, key == ks, key + 32 > nk_first, nk - key, c, lane);
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the next tile landed (this wave's part)
     __syncthreads();                                     // ... and every wave's
   }
-  if (CAUSAL && __ballot(bad) != 0) {
-    float m = -INFINITY;
-    l = 0.f;
-    for (int i = 0; i < 16; ++i) o[0][i] = o[1][i] = 0.f;
-#pragma clang loop unroll(disable)
-    for (int j = ks; j < min(ke, nk_last); ++j) {
-      const float x = dot_row(Kg + j * a.k_t, qf, hh);
-      if (j < nk) {
-        const float m_new = fmaxf(m, x), alpha = m == m_new ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
-        const float p = __builtin_amdgcn_exp2f((x - m_new) * c);
-        m = m_new;
-        l = fmaf(l, alpha, p);
-        for (int i = 0; i < 16; ++i) {
-          o[0][i] *= alpha;
-          o[1][i] *= alpha;
-        }
-        add_row(o, p, Vg + j * a.v_t, hh);
-      }
-    }
-    nm[0] = -m;
-    if (hh) l = 0.f;                                   // both halves hold the whole sum
-  }
-  l += __shfl_xor(l, 32);
+  if (CAUSAL && __ballot(w.bad) != 0) attend_again(w, qf, Kg, a.k_t, Vg, a.v_t, ks, min(ke, nk_last), 1, nk, c, hh);
+  const float l = w.l + __shfl_xor(w.l, 32);
   if (r >= R) return;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  const float l2 = l == 0.f ? -INFINITY : fmaf(-nm[0], c, log2f(l));
+  const float l2 = l == 0.f ? -INFINITY : fmaf(-w.nm[0], c, log2f(l));
   if (SPLIT) {
     const int64_t row = ((int64_t)split * a.Hk + hk) * a.Tq * a.G + (int64_t)s.q0 * a.G + r;
     if (hh == 0) a.part_l[row] = l2;
@@ -411,44 +431,187 @@ __global__ __launch_bounds__(256, 3) void k_attnp_fwd(const Args a) {
 #pragma unroll
         for (int g = 0; g < 4; ++g)
           *reinterpret_cast<float4*>(a.part_o + row * 64 + 32 * dt + 8 * g + 4 * hh) =
-              make_float4(o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv, o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv);
+              make_float4(w.o[dt][4 * g] * inv, w.o[dt][4 * g + 1] * inv, w.o[dt][4 * g + 2] * inv, w.o[dt][4 * g + 3] * inv);
     }
   } else {
-    store_acc(a.out + (s.q0 + qi) * a.o_t + h * a.o_h, o, inv, hh);
+    store_acc(a.out + (s.q0 + qi) * a.o_t + h * a.o_h, w.o, inv, hh);
     if (hh == 0) a.lse[(int64_t)(s.q0 + qi) * a.H + h] = l2 * 0.69314718055994531f;
   }
 }
 
-// The shares of a split call joined, a wave to a row: out = sum_s 2^(l_s - m) O_s / sum_s 2^(l_s - m).
-__global__ __launch_bounds__(256) void k_attnp_join(const Args a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t rows = (int64_t)a.Tq * a.G, n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+// Few rows (new tokens over a cache): 32 packed rows of one key head a workgroup, whose four waves take every fourth
+// block of 32 keys of a share, each with its own two LDS buffers and no barrier until the end -- what counts is how many
+// bytes of K and V are on their way, 8 KiB a wave.  A share is lk / nsplit keys, 256 at least.
+constexpr int kFew = 32;
+constexpr int kFewBlock = 32 * 128;                  // bytes of 32 keys' K (or V)
+template <bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void k_attnp_few(const Args a) {
+  // per wave two buffers of K block, V block; at the end the waves' sums, rows of 68 floats
+  __shared__ __attribute__((aligned(16))) uint8_t smem[4 * 4 * kFewBlock];
+  __shared__ float ml[2][4][32];
+  const int lane = threadIdx.x & 63, hh = lane >> 5, lr = lane & 31;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hk = blockIdx.x % a.Hk;
+  int rest = blockIdx.x / a.Hk;
+  const int split = rest % a.nsplit;
+  int tile;
+  const int b = find_tile(a.cu_q, a.Tq, a.G, kFew, a.B + a.zero_tail, rest / a.nsplit, lane, tile);
+  if (b == a.B) {
+    const int t0 = cu_at(a.cu_q, a.B, a.Tq);
+    if (split == 0 && a.nsplit == 1) zero_rows(a.out, a.o_t, a.o_h, t0, tile * kFew, min((tile + 1) * kFew, (a.Tq - t0) * a.G), hk, a.G, a.lse, a.H);
+    return;
+  }
+  const Seq s = sequence(a, b);
+  const int R = s.lq * a.G, r0 = tile * kFew;
+  if (r0 >= R) return;
+  const int rc = min(r0 + lr, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
+  const int nk = seen(CAUSAL, qi, s), nk_first = seen(CAUSAL, r0 / a.G, s);
+  int ke = seen(CAUSAL, (min(r0 + kFew, R) - 1) / a.G, s);
+  const int chunk = max(256, ((s.lk + a.nsplit - 1) / a.nsplit + 127) / 128 * 128);
+  const int ks = (int)min((int64_t)split * chunk, (int64_t)ke);
+  ke = min(ke, ks + chunk);
+
+  const bf16_t* Kg = a.k + (s.k0 * a.k_t + hk * a.k_h);
+  const bf16_t* Vg = a.v + (s.k0 * a.v_t + hk * a.v_h);
+  uint32_t offk[4], offv[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int row = j * 8 + (lane >> 3), ch = ((lane & 7) ^ swz(row)) * 8;
+    offk[j] = (uint32_t)((row * a.k_t + ch) * 2);
+    offv[j] = (uint32_t)((row * a.v_t + ch) * 2);
+  }
+  uint8_t* mine = smem + wid * 4 * kFewBlock;
+  auto stage = [&](int buf, int key) {
+    const auto rk = rows_rsrc(Kg + key * a.k_t, a.k_t, s.lk - key), rv = rows_rsrc(Vg + key * a.v_t, a.v_t, s.lk - key);
+    const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(mine + buf * 2 * kFewBlock));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dma16(rk, base + j * 1024, offk[j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dma16(rv, base + kFewBlock + j * 1024, offv[j]);
+  };
+  bf16x8 qf[4];
+  {
+    const bf16_t* qr = a.q + (s.q0 + qi) * a.q_t + h * a.q_h;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) qf[t] = *reinterpret_cast<const bf16x8*>(qr + 16 * t + 8 * hh);
+  }
+  const int first = ks + 32 * wid;
+  if (first < ke) stage(0, first);
+  const float c = a.c;
+  Rows w;
+  w.clear();
+  for (int key = first, cur = 0; key < ke; key += 128, cur ^= 1) {
+    if (key + 128 < ke) {
+      // the other buffer's reads have returned before it is written again
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      stage(cur ^ 1, key + 128);
+      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // this block landed, the next one's 8 loads may be on their way
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    const uint8_t* sK = mine + cur * 2 * kFewBlock;
+    attend<CAUSAL>(w, qf, sK, sK + kFewBlock, 0, key == first, key + 32 > nk_first, nk - key, c, lane);
+  }
+  if (CAUSAL && __ballot(w.bad) != 0) attend_again(w, qf, Kg, a.k_t, Vg, a.v_t, first, ke, 97, nk, c, hh);
+  const float l = w.l + __shfl_xor(w.l, 32);
+
+  // the four waves' sums: sum_w f_w O_w, f_w = 2^(c (m_w - m))
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  float* ow = reinterpret_cast<float*>(mine);
+#pragma unroll
+  for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<float4*>(ow + lr * 68 + 32 * dt + 8 * g + 4 * hh) =
+          make_float4(w.o[dt][4 * g], w.o[dt][4 * g + 1], w.o[dt][4 * g + 2], w.o[dt][4 * g + 3]);
+  if (hh == 0) {
+    ml[0][wid][lr] = l == 0.f ? -INFINITY : -w.nm[0];
+    ml[1][wid][lr] = l;
+  }
+  __syncthreads();
+  const int row = threadIdx.x >> 3, d = (threadIdx.x & 7) * 8, r = r0 + row;
+  if (r >= R) return;
+  float m = -INFINITY, total = 0.f, acc[8] = {};
+#pragma unroll
+  for (int v = 0; v < 4; ++v) m = fmaxf(m, ml[0][v][row]);
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    const float lv = ml[1][v][row];
+    if (lv == 0.f) continue;                         // saw nothing (a NaN sum is not skipped)
+    const float mv = ml[0][v][row], f = mv == m ? 1.f : __builtin_amdgcn_exp2f((mv - m) * c);
+    total = fmaf(f, lv, total);
+    const float* x = reinterpret_cast<const float*>(smem + v * 4 * kFewBlock) + row * 68 + d;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = fmaf(f, x[i], acc[i]);
+  }
+  const float inv = total == 0.f ? 0.f : 1.0f / total;
+  const float l2 = total == 0.f ? -INFINITY : fmaf(m, c, log2f(total));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] *= inv;
+  const int i = r / a.G, hq = hk * a.G + r - i * a.G;
+  if (a.nsplit == 1) {
+    *reinterpret_cast<uint4*>(a.out + (s.q0 + i) * a.o_t + hq * a.o_h + d) =
+        make_uint4(pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3]), pack_bf16(acc[4], acc[5]), pack_bf16(acc[6], acc[7]));
+    if (d == 0) a.lse[(int64_t)(s.q0 + i) * a.H + hq] = l2 * 0.69314718055994531f;
+  } else {
+    const int64_t at = ((int64_t)split * a.Hk + hk) * a.Tq * a.G + (int64_t)s.q0 * a.G + r;
+    if (d == 0) a.part_l[at] = l2;
+    if (l2 != -INFINITY) {
+      *reinterpret_cast<float4*>(a.part_o + at * 64 + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      *reinterpret_cast<float4*>(a.part_o + at * 64 + d + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    }
+  }
+}
+
+// The shares of a split call joined, W waves to a row: out = sum_s 2^(l_s - m) O_s / sum_s 2^(l_s - m).  Wave v takes the
+// shares 8 v .. 8 v + 7, then 8 W further, eight loads in flight; a lane is a d.
+template <int W>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_attnp_join(const Args a) {
+  __shared__ float red[W == 1 ? 1 : W][W == 1 ? 1 : 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, v = W == 1 ? 0 : wave;
+  const int64_t rows = (int64_t)a.Tq * a.G, n = W == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
   if (n >= rows * a.Hk) return;
   const int hk = (int)(n / rows), row = (int)(n - hk * rows), t = row / a.G, h = hk * a.G + row - t * a.G;
   const bool tail = t >= cu_at(a.cu_q, a.B, a.Tq);
   if (tail && !a.zero_tail) return;
-  bf16_t* out = a.out + t * a.o_t + h * a.o_h + lane;
+  const int64_t step = rows * a.Hk;                  // from share to share
+  const float* pl = a.part_l + hk * rows + row;
+  const float* po = a.part_o + (hk * rows + row) * 64 + lane;
   float acc = 0.f, m = -INFINITY, total = 0.f;
   if (!tail) {
-    for (int s = lane; s < a.nsplit; s += 64) m = fmaxf(m, a.part_l[((int64_t)s * a.Hk + hk) * rows + row]);
+    for (int s = lane; s < a.nsplit; s += 64) m = fmaxf(m, pl[s * step]);
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-    for (int s0 = 0; s0 < a.nsplit; s0 += 64) {
-      const int s = s0 + lane;
-      const float ls = s < a.nsplit ? a.part_l[((int64_t)s * a.Hk + hk) * rows + row] : -INFINITY;
-      // NaN shares (a NaN or infinite score) stay NaN
-      const float w = ls == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ls - m);
-      total += w;
-      const int last = min(64, a.nsplit - s0);
-      for (int j = 0; j < last; ++j) {
-        const float wj = __shfl(w, j);
-        if (wj != 0.f) acc = fmaf(wj, a.part_o[(((int64_t)(s0 + j) * a.Hk + hk) * rows + row) * 64 + lane], acc);
+    for (int s0 = 8 * v; s0 < a.nsplit; s0 += 8 * W) {
+      float l[8], o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) l[j] = pl[min(s0 + j, a.nsplit - 1) * step];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = po[min(s0 + j, a.nsplit - 1) * step * 64];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        // an empty share wrote no O; NaN shares (a NaN or infinite score) stay NaN
+        const bool on = s0 + j < a.nsplit && l[j] != -INFINITY;
+        const float w = on ? __builtin_amdgcn_exp2f(l[j] - m) : 0.f;
+        total += w;
+        acc = on ? fmaf(w, o[j], acc) : acc;
       }
     }
-    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off);
   }
-  const float v = total == 0.f ? 0.f : acc / total;
-  const __bf16 o = (__bf16)v;
-  *out = __builtin_bit_cast(bf16_t, o);
+  if constexpr (W > 1) {
+    red[v][lane] = acc;
+    __shared__ float tot[W];
+    if (lane == 0) tot[v] = total;
+    __syncthreads();
+    if (v) return;
+    acc = total = 0.f;
+#pragma unroll
+    for (int u = 0; u < W; ++u) {
+      acc += red[u][lane];
+      total += tot[u];
+    }
+  }
+  const __bf16 o = (__bf16)(total == 0.f ? 0.f : acc / total);
+  a.out[t * a.o_t + h * a.o_h + lane] = __builtin_bit_cast(bf16_t, o);
   if (lane == 0) a.lse[(int64_t)t * a.H + h] = total == 0.f ? -INFINITY : (m + log2f(total)) * 0.69314718055994531f;
 }
 
@@ -759,12 +922,23 @@ inline int64_t row_tiles(const i2pc_attn_packed_desc& d) {
   return (int64_t)d.total_q * (d.heads / d.kv_heads) / kRows + d.batch + (d.zero_tail ? 1 : 0);
 }
 
+// Sequences of 32 packed rows or fewer on average take the kernel for few rows.  (Right for any lengths: the rule only
+// decides the speed.)
+inline bool few_rows(const i2pc_attn_packed_desc& d) {
+  return (int64_t)d.total_q * (d.heads / d.kv_heads) <= (int64_t)d.batch * kFew;
+}
+inline int64_t few_tiles(const i2pc_attn_packed_desc& d) {
+  return (int64_t)d.total_q * (d.heads / d.kv_heads) / kFew + d.batch + (d.zero_tail ? 1 : 0);
+}
+
 // Shares of the keys: one where the row tiles fill the chip, else so many that they do, of 256 keys at least (an
 // upper bound: a share may be empty).
 inline int splits(const i2pc_attn_packed_desc& d) {
-  const int64_t tiles = row_tiles(d) * d.kv_heads;
-  if (tiles >= 512 || d.total_k == 0) return 1;
-  const int64_t want = (1024 + tiles - 1) / tiles, most = (d.total_k + 255) / 256;
+  if (d.total_k == 0) return 1;
+  const int64_t tiles = (few_rows(d) ? few_tiles(d) : row_tiles(d)) * d.kv_heads;
+  const int64_t most = (d.total_k + 255) / 256;
+  static const int target = [] { const char* e = getenv("I2PC_FEW"); return e ? atoi(e) : 1024; }();
+  const int64_t want = few_rows(d) ? target / tiles : tiles >= 512 ? 1 : (1024 + tiles - 1) / tiles;
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 512}));
 }
 
@@ -783,8 +957,8 @@ int check(const char* what, const i2pc_attn_packed_desc* d) {
   if (d->head_dim != 64) return set_error(I2PC_EUNSUPPORTED, "%s: head_dim=%d, the kernels are of 64", what, d->head_dim);
   // grids of 256-thread workgroups hold 2^24 of them
   const int64_t most = (int64_t)1 << 24;
-  if ((int64_t)d->total_q * d->heads >= most * 32 || ((int64_t)d->total_q / kRows + d->batch + 1) * d->heads >= most ||
-      ((int64_t)d->total_k / kKeys + d->batch + 1) * d->kv_heads >= most)
+  if ((int64_t)d->total_q * d->heads >= most * 32 || ((int64_t)d->total_q / kRows + 2 * (int64_t)d->batch + 2) * d->heads >= most ||
+      ((int64_t)d->total_k / kKeys + (int64_t)d->batch + 1) * d->kv_heads >= most)
     return set_error(I2PC_EUNSUPPORTED, "%s: total_q * heads must stay below 2^29, (total_k / 64 + batch) * kv_heads below 2^24", what);
   I2PC_REQUIRE(std::isfinite(d->scale) && d->scale > 0.f, "%s: scale=%g must be finite and above zero", what, (double)d->scale);
   I2PC_REQUIRE(d->batch == 0 || (d->cu_q && d->cu_k), "%s: NULL cu_q or cu_k", what);
@@ -834,17 +1008,23 @@ extern "C" int i2pc_attention_packed(const i2pc_attn_packed_desc* d, void* works
   attnp::Args a = attnp::args_of(*d);
   hipStream_t s = as_stream(stream);
   a.nsplit = attnp::splits(*d);
-  const dim3 block(256), grid((uint32_t)(attnp::row_tiles(*d) * a.Hk * a.nsplit));
-  if (a.nsplit == 1) {
-    if (d->causal) hipLaunchKernelGGL((attnp::k_attnp_fwd<true, false>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((attnp::k_attnp_fwd<false, false>), grid, block, 0, s, a);
-    return check_launch("attention_packed");
+  const bool few = attnp::few_rows(*d);
+  const dim3 block(256), grid((uint32_t)((few ? attnp::few_tiles(*d) : attnp::row_tiles(*d)) * a.Hk * a.nsplit));
+  if (a.nsplit > 1) {
+    a.part_o = static_cast<float*>(workspace);
+    a.part_l = a.part_o + (size_t)a.nsplit * a.H * a.Tq * 64;
   }
-  a.part_o = static_cast<float*>(workspace);
-  a.part_l = a.part_o + (size_t)a.nsplit * a.H * a.Tq * 64;
-  if (d->causal) hipLaunchKernelGGL((attnp::k_attnp_fwd<true, true>), grid, block, 0, s, a);
+  if (few && d->causal) hipLaunchKernelGGL(attnp::k_attnp_few<true>, grid, block, 0, s, a);
+  else if (few) hipLaunchKernelGGL(attnp::k_attnp_few<false>, grid, block, 0, s, a);
+  else if (a.nsplit == 1 && d->causal) hipLaunchKernelGGL((attnp::k_attnp_fwd<true, false>), grid, block, 0, s, a);
+  else if (a.nsplit == 1) hipLaunchKernelGGL((attnp::k_attnp_fwd<false, false>), grid, block, 0, s, a);
+  else if (d->causal) hipLaunchKernelGGL((attnp::k_attnp_fwd<true, true>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((attnp::k_attnp_fwd<false, true>), grid, block, 0, s, a);
-  hipLaunchKernelGGL(attnp::k_attnp_join, dim3((uint32_t)(((int64_t)a.Tq * a.H + 3) / 4)), block, 0, s, a);
+  const int64_t rows = (int64_t)a.Tq * a.H;
+  if (a.nsplit > 32)
+    hipLaunchKernelGGL(attnp::k_attnp_join<16>, dim3((uint32_t)rows), dim3(1024), 0, s, a);
+  else if (a.nsplit > 1)
+    hipLaunchKernelGGL(attnp::k_attnp_join<1>, dim3((uint32_t)((rows + 3) / 4)), block, 0, s, a);
   return check_launch("attention_packed");
 }
 

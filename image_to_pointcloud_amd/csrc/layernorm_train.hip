@@ -137,13 +137,14 @@ __global__ __launch_bounds__(WPR == 8 ? 512 : 256) void k_lnt_fwd(const T* __res
   }
 }
 
-// Rows blockIdx.x * R + k * gridDim.x * R for the R = 8 / WPR rows a workgroup takes at a time.  A partial row
-// of `part` is dim column sums of dgamma, then dim of dbeta.
+// Rows blockIdx.x * R + k * gridDim.x * R for the R = 8 / WPR rows a workgroup takes at a time.  Partial row p of the
+// column sums goes to dgamma + p * 2 * dim and dbeta + p * 2 * dim: with one partial row, the outputs themselves.
 template <typename T, int E, int V, int WPR>
 __global__ __launch_bounds__(kThreads) void k_lnt_bwd(const bf16_t* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
                                                       int64_t ldx, const float2* __restrict__ stats,
                                                       const float* __restrict__ gamma, const T* add, int64_t lda, int rows,
-                                                      int dim, T* dx, int64_t lddx, float* __restrict__ part) {
+                                                      int dim, T* dx, int64_t lddx, float* __restrict__ dgamma,
+                                                      float* __restrict__ dbeta) {
   __shared__ float red[8];
   extern __shared__ float sums[];                  // [2][dim], rows of one wave only
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -205,12 +206,12 @@ __global__ __launch_bounds__(kThreads) void k_lnt_bwd(const bf16_t* __restrict__
     }
   }
   if constexpr (WPR > 1) {                         // wide rows: a partial row for each row group
-    float* out = part + (int64_t)(blockIdx.x * R + wave / WPR) * 2 * dim;
+    const int64_t p = (int64_t)(blockIdx.x * R + wave / WPR) * 2 * dim;
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (c.first[i] < (uint32_t)E) {
-        Vec<float, E>::store(out + c.col[i], dg[i]);
-        Vec<float, E>::store(out + dim + c.col[i], db[i]);
+        Vec<float, E>::store(dgamma + p + c.col[i], dg[i]);
+        Vec<float, E>::store(dbeta + p + c.col[i], db[i]);
       }
   } else {                                         // the row groups' column sums, one after the other
     for (int w = 0; w < R; ++w) {
@@ -228,8 +229,11 @@ __global__ __launch_bounds__(kThreads) void k_lnt_bwd(const bf16_t* __restrict__
       }
     }
     __syncthreads();
-    float* out = part + (int64_t)blockIdx.x * 2 * dim;
-    for (int i = threadIdx.x; i < 2 * dim; i += kThreads) out[i] = sums[i];
+    const int64_t p = (int64_t)blockIdx.x * 2 * dim;
+    for (int i = threadIdx.x; i < dim; i += kThreads) {
+      dgamma[p + i] = sums[i];
+      dbeta[p + i] = sums[dim + i];
+    }
   }
 }
 
@@ -277,10 +281,10 @@ void launch_fwd(const T* x, int64_t ldx, const float* gamma, const float* beta, 
 }
 template <typename T, int E, int V, int WPR>
 void launch_bwd(const bf16_t* dy, int64_t lddy, const T* x, int64_t ldx, const float2* stats, const float* gamma,
-                const T* add, int64_t lda, int rows, int dim, T* dx, int64_t lddx, float* part, hipStream_t s) {
+                const T* add, int64_t lda, int rows, int dim, T* dx, int64_t lddx, float* dgamma, float* dbeta, hipStream_t s) {
   hipLaunchKernelGGL((k_lnt_bwd<T, E, V, WPR>), dim3(groups_for(rows, dim)), dim3(kThreads),
                      WPR == 1 ? 2 * dim * sizeof(float) : 0, s, dy,
-                     lddy, x, ldx, stats, gamma, add, lda, rows, dim, dx, lddx, part);
+                     lddy, x, ldx, stats, gamma, add, lda, rows, dim, dx, lddx, dgamma, dbeta);
 }
 
 // The narrowest instance that holds the row: E elements a load, V loads a lane, WPR waves a row.  Rows above
@@ -326,7 +330,8 @@ extern "C" int i2pc_layernorm_train(const void* x, int x_f32, int64_t ldx, const
 
 extern "C" size_t i2pc_layernorm_backward_workspace_bytes(int rows, int dim) {
   if (rows < 0 || dim <= 0 || dim > lnt::kMaxDim) return 0;
-  return (size_t)lnt::parts_for(rows, dim) * 2 * dim * sizeof(float);
+  const int parts = lnt::parts_for(rows, dim);
+  return parts == 1 ? 0 : (size_t)parts * 2 * dim * sizeof(float);
 }
 
 extern "C" int i2pc_layernorm_backward(const void* dy, int64_t lddy, const void* x, int x_f32, int64_t ldx,
@@ -336,23 +341,25 @@ extern "C" int i2pc_layernorm_backward(const void* dy, int64_t lddy, const void*
   clear_error();
   I2PC_REQUIRE(rows >= 0 && dim > 0, "layernorm_backward: empty shape");
   I2PC_REQUIRE(dim <= lnt::kMaxDim, "layernorm_backward: dim=%d is above %d", dim, lnt::kMaxDim);
-  I2PC_REQUIRE(gamma && dgamma && dbeta && workspace && (rows == 0 || (dy && x && stats && dx)), "NULL pointer");
+  I2PC_REQUIRE(gamma && dgamma && dbeta && (rows == 0 || (dy && x && stats && dx)), "NULL pointer");
   I2PC_REQUIRE(rows == 0 || (ldx >= dim && lddy >= dim && lddx >= dim && (!add || lda >= dim)),
                "layernorm_backward: row strides must be at least dim");
-  if (workspace_bytes < i2pc_layernorm_backward_workspace_bytes(rows, dim))
-    return set_error(I2PC_EWORKSPACE, "layernorm_backward: workspace of %zu bytes, needs %zu", workspace_bytes,
-                     i2pc_layernorm_backward_workspace_bytes(rows, dim));
+  const size_t need = i2pc_layernorm_backward_workspace_bytes(rows, dim);
+  if (workspace_bytes < need || (need && !workspace))
+    return set_error(I2PC_EWORKSPACE, "layernorm_backward: workspace of %zu bytes, needs %zu", workspace_bytes, need);
   hipStream_t s = as_stream(stream);
   float* part = static_cast<float*>(workspace);
+  float *pg = need ? part : dgamma, *pb = need ? part + dim : dbeta;
   using namespace lnt;
   auto* g = static_cast<const bf16_t*>(dy);
   auto* st = reinterpret_cast<const float2*>(stats);
   if (x_f32)
     LNT_DISPATCH(launch_bwd, float, g, lddy, static_cast<const float*>(x), ldx, st, gamma, static_cast<const float*>(add),
-                 lda, rows, dim, static_cast<float*>(dx), lddx, part, s);
+                 lda, rows, dim, static_cast<float*>(dx), lddx, pg, pb, s);
   else
     LNT_DISPATCH(launch_bwd, bf16_t, g, lddy, static_cast<const bf16_t*>(x), ldx, st, gamma, static_cast<const bf16_t*>(add),
-                 lda, rows, dim, static_cast<bf16_t*>(dx), lddx, part, s);
-  hipLaunchKernelGGL(k_lnt_cols, dim3((2 * dim + 63) / 64), dim3(1024), 0, s, part, parts_for(rows, dim), dim, dgamma, dbeta);
+                 lda, rows, dim, static_cast<bf16_t*>(dx), lddx, pg, pb, s);
+  if (need)
+    hipLaunchKernelGGL(k_lnt_cols, dim3((2 * dim + 63) / 64), dim3(1024), 0, s, part, parts_for(rows, dim), dim, dgamma, dbeta);
   return check_launch("layernorm_backward");
 }

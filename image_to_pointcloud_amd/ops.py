@@ -7,6 +7,7 @@ Layouts: activations bf16 NHWC / [rows][features]; residual stream fp32.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Optional
 
@@ -865,16 +866,23 @@ _lib.register("i2pc_gelu_fp8_backward", ctypes.c_int, [c_void_p, c_int64, c_void
 def _operand(t, name, shape, dtypes, like=None):
     """Refuses a tensor that is not on the device, not of `shape` / one of `dtypes`, or whose last axis is not
     dense; `like`: the tensor whose device it has to share."""
-    if not t.is_cuda:
+    at = t.get_device()
+    if at < 0:
         raise _lib.I2PCError(f"{name} must be a device tensor")
-    if like is not None and t.device != like.device:
-        raise _lib.I2PCError(f"{name} is on {t.device}, not on {like.device}")
+    if like is not None and at != like.get_device():
+        raise _lib.I2PCError(f"{name} is on device {at}, not on {like.get_device()}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: expected {' or '.join(map(str, dtypes))}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name}: expected the shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.shape and t.shape[-1] > 1 and t.stride(-1) != 1:
+    if shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name}: the last axis must be dense, its stride is {t.stride(-1)}")
+
+
+def _rows_dim(t, name):
+    if t.dim() != 2:
+        raise ValueError(f"{name}: expected [rows, dim], got the shape {tuple(t.shape)}")
+    return t.shape
 
 
 def _pitch(t):
@@ -884,9 +892,20 @@ def _pitch(t):
 
 def _on_device_of(t):
     """The device of `t` made current for a launch, where it is not already."""
-    import contextlib
     torch = _torch()
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    at = t.get_device()
+    return contextlib.nullcontext() if at < 0 or at == torch._C._cuda_getDevice() else torch.cuda.device(at)
+
+
+def _launch(label, nbytes, name, t, *args):
+    """Calls the entry point on the current stream of the device of `t`, timed where a profile is taken.  (The raw
+    stream handle: building a Stream object for it costs more than the launch leaves to the host.)"""
+    stream = _torch()._C._cuda_getCurrentRawStream(t.get_device())
+    if profile is None:
+        _lib.call(name, *args, stream)
+        return
+    with _Timed(label, 0.0, nbytes):
+        _lib.call(name, *args, stream)
 
 
 def layernorm_train(x, gamma, beta, eps, out=None, stats=None):
@@ -894,27 +913,23 @@ def layernorm_train(x, gamma, beta, eps, out=None, stats=None):
     training step: (y, stats) with y bf16 [rows, dim] and stats fp32 [rows, 2] = each row's (mean, 1 / std),
     which layernorm_backward reads.  gamma, beta: fp32 [dim].  Rows and statistics are held in fp32."""
     torch = _torch()
-    if x.dim() != 2:
-        raise ValueError(f"x: expected [rows, dim], got the shape {tuple(x.shape)}")
-    rows, dim = x.shape
+    rows, dim = _rows_dim(x, "x")
     f32 = (torch.float32,)
     _operand(x, "x", (rows, dim), (torch.float32, torch.bfloat16))
     _operand(gamma, "gamma", (dim,), f32, x)
     _operand(beta, "beta", (dim,), f32, x)
     with _on_device_of(x):
         if out is None:
-            out = torch.empty((rows, dim), dtype=torch.bfloat16, device=x.device)
+            out = x.new_empty((rows, dim), dtype=torch.bfloat16)
         else:
             _operand(out, "out", (rows, dim), (torch.bfloat16,), x)
         if stats is None:
-            stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
+            stats = x.new_empty((rows, 2), dtype=torch.float32)
         else:
-            _operand(stats, "stats", (rows, 2), f32, x)
-            if not stats.is_contiguous():
-                raise ValueError("stats must be contiguous")
-        with _Timed("k_lnt_fwd", 0.0, rows * dim * (x.element_size() + 2.0) + 8.0 * rows):
-            _lib.call("i2pc_layernorm_train", _p(x), int(x.dtype == torch.float32), _pitch(x), _p(gamma), _p(beta),
-                      float(eps), rows, dim, _p(out), _pitch(out), _p(stats), _stream())
+            _dense(stats, "stats", (rows, 2), x)
+        e = x.element_size()
+        _launch("k_lnt_fwd", rows * dim * (e + 2.0) + 8.0 * rows, "i2pc_layernorm_train", x, _p(x), int(e == 4), _pitch(x),
+                _p(gamma), _p(beta), eps, rows, dim, _p(out), _pitch(out), _p(stats))
     return out, stats
 
 
@@ -923,63 +938,60 @@ def layernorm_backward(dy, x, stats, gamma, add=None, dx=None, dgamma=None, dbet
     pass and gamma.  dx has x's type; add (x's type): a gradient added to it before its rounding (the residual
     stream's), dx may be add itself.  dgamma, dbeta: fp32 [dim], summed in fp32 in a fixed order."""
     torch = _torch()
-    if x.dim() != 2:
-        raise ValueError(f"x: expected [rows, dim], got the shape {tuple(x.shape)}")
-    rows, dim = x.shape
-    f32 = (torch.float32,)
+    rows, dim = _rows_dim(x, "x")
+    f32, same = (torch.float32,), (x.dtype,)
     _operand(x, "x", (rows, dim), (torch.float32, torch.bfloat16))
     _operand(dy, "dy", (rows, dim), (torch.bfloat16,), x)
-    _operand(stats, "stats", (rows, 2), f32, x)
-    if not stats.is_contiguous():
-        raise ValueError("stats must be contiguous")
+    _dense(stats, "stats", (rows, 2), x)
     _operand(gamma, "gamma", (dim,), f32, x)
     if add is not None:
-        _operand(add, "add", (rows, dim), (x.dtype,), x)
+        _operand(add, "add", (rows, dim), same, x)
     with _on_device_of(x):
         if dx is None:
-            dx = torch.empty((rows, dim), dtype=x.dtype, device=x.device)
+            dx = x.new_empty((rows, dim))
         else:
-            _operand(dx, "dx", (rows, dim), (x.dtype,), x)
-        dgamma = _column_sums(dgamma, "dgamma", dim, x)
-        dbeta = _column_sums(dbeta, "dbeta", dim, x)
+            _operand(dx, "dx", (rows, dim), same, x)
+        if dgamma is None:
+            dgamma = x.new_empty(dim, dtype=torch.float32)
+        else:
+            _operand(dgamma, "dgamma", (dim,), f32, x)
+        if dbeta is None:
+            dbeta = x.new_empty(dim, dtype=torch.float32)
+        else:
+            _operand(dbeta, "dbeta", (dim,), f32, x)
         nb = _lib.load().i2pc_layernorm_backward_workspace_bytes(rows, dim)
-        ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(nb, dtype=torch.uint8) if nb else None
         e = x.element_size()
-        with _Timed("k_lnt_bwd", 0.0, rows * dim * (2.0 + 2.0 * e + (e if add is not None else 0)) + 12.0 * dim):
-            _lib.call("i2pc_layernorm_backward", _p(dy), _pitch(dy), _p(x), int(x.dtype == torch.float32), _pitch(x),
-                      _p(stats), _p(gamma), _p(add), 0 if add is None else _pitch(add), rows, dim, _p(dx), _pitch(dx),
-                      _p(dgamma), _p(dbeta), _p(ws), nb, _stream())
+        _launch("k_lnt_bwd", rows * dim * (2.0 + 2.0 * e + (e if add is not None else 0)) + 12.0 * dim,
+                "i2pc_layernorm_backward", x, _p(dy), _pitch(dy), _p(x), int(e == 4), _pitch(x), _p(stats), _p(gamma), _p(add),
+                0 if add is None else _pitch(add), rows, dim, _p(dx), _pitch(dx), _p(dgamma), _p(dbeta), _p(ws), nb)
     return dx, dgamma, dbeta
 
 
-def _column_sums(t, name, dim, like):
-    torch = _torch()
-    if t is None:
-        return torch.empty(dim, dtype=torch.float32, device=like.device)
-    _operand(t, name, (dim,), (torch.float32,), like)
-    return t
+def _dense(t, name, shape, like):
+    _operand(t, name, shape, (_torch().float32,), like)
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
 
 
 def gelu_fp8(x, out=None, kept=None):
     """GELU (the erf form) of bf16 rows x [rows, dim], dim % 32 == 0: (y, kept) with y bf16 and kept the Fp8 rows
     of x (quant_fp8's block rule) that gelu_fp8_backward works from: 1.03 bytes a value instead of two."""
     torch = _torch()
-    if x.dim() != 2:
-        raise ValueError(f"x: expected [rows, dim], got the shape {tuple(x.shape)}")
-    rows, dim = x.shape
-    _operand(x, "x", (rows, dim), (torch.bfloat16,))
+    rows, dim = _rows_dim(x, "x")
+    bf = (torch.bfloat16,)
+    _operand(x, "x", (rows, dim), bf)
     with _on_device_of(x):
         if out is None:
-            out = torch.empty((rows, dim), dtype=torch.bfloat16, device=x.device)
+            out = x.new_empty((rows, dim))
         else:
-            _operand(out, "out", (rows, dim), (torch.bfloat16,), x)
+            _operand(out, "out", (rows, dim), bf, x)
         if kept is None:
-            kept = empty_fp8((rows, dim), x.device)
+            kept = Fp8(x.new_empty((rows, dim), dtype=torch.uint8), x.new_empty((rows, dim // 32), dtype=torch.uint8))
         else:
             _kept_operand(kept, rows, dim, x)
-        with _Timed("k_gelu_keep", 0.0, rows * dim * (5.0 + 1.0 / 32)):
-            _lib.call("i2pc_gelu_fp8", _p(x), _pitch(x), rows, dim, _p(out), _pitch(out), _p(kept.data), _p(kept.scale),
-                      _stream())
+        _launch("k_gelu_keep", rows * dim * (5.0 + 1.0 / 32), "i2pc_gelu_fp8", x, _p(x), _pitch(x), rows, dim, _p(out),
+                _pitch(out), _p(kept.data), _p(kept.scale))
     return out, kept
 
 
@@ -988,35 +1000,33 @@ def gelu_fp8_backward(dy, kept, dx=None, again=None, recompute=False):
     (or an `again` to write to): (dx, again), again = GELU(x~) in bf16, for the next linear layer's weight
     gradient."""
     torch = _torch()
-    if dy.dim() != 2:
-        raise ValueError(f"dy: expected [rows, dim], got the shape {tuple(dy.shape)}")
-    rows, dim = dy.shape
-    _operand(dy, "dy", (rows, dim), (torch.bfloat16,))
+    rows, dim = _rows_dim(dy, "dy")
+    bf = (torch.bfloat16,)
+    _operand(dy, "dy", (rows, dim), bf)
     _kept_operand(kept, rows, dim, dy)
     with _on_device_of(dy):
         if dx is None:
-            dx = torch.empty((rows, dim), dtype=torch.bfloat16, device=dy.device)
+            dx = dy.new_empty((rows, dim))
         else:
-            _operand(dx, "dx", (rows, dim), (torch.bfloat16,), dy)
+            _operand(dx, "dx", (rows, dim), bf, dy)
         if again is not None:
-            _operand(again, "again", (rows, dim), (torch.bfloat16,), dy)
+            _operand(again, "again", (rows, dim), bf, dy)
         elif recompute:
-            again = torch.empty((rows, dim), dtype=torch.bfloat16, device=dy.device)
-        nbytes = rows * dim * (5.0 + 1.0 / 32 + (2.0 if again is not None else 0.0))
-        with _Timed("k_gelu_back", 0.0, nbytes):
-            _lib.call("i2pc_gelu_fp8_backward", _p(dy), _pitch(dy), _p(kept.data), _p(kept.scale), rows, dim, _p(dx),
-                      _pitch(dx), _p(again), 0 if again is None else _pitch(again), _stream())
+            again = dy.new_empty((rows, dim))
+        _launch("k_gelu_back", rows * dim * (5.0 + 1.0 / 32 + (2.0 if again is not None else 0.0)), "i2pc_gelu_fp8_backward", dy,
+                _p(dy), _pitch(dy), _p(kept.data), _p(kept.scale), rows, dim, _p(dx), _pitch(dx), _p(again),
+                0 if again is None else _pitch(again))
     return dx if again is None else (dx, again)
 
 
 def _kept_operand(kept, rows, dim, like):
-    torch = _torch()
+    u8 = (_torch().uint8,)
     if not isinstance(kept, Fp8):
         raise TypeError(f"kept: expected Fp8 rows, got {type(kept).__name__}")
     if dim % 32:
         raise ValueError(f"dim={dim} must be a multiple of 32")
-    _operand(kept.data, "kept.data", (rows, dim), (torch.uint8,), like)
-    _operand(kept.scale, "kept.scale", (rows, dim // 32), (torch.uint8,), like)
+    _operand(kept.data, "kept.data", (rows, dim), u8, like)
+    _operand(kept.scale, "kept.scale", (rows, dim // 32), u8, like)
     if not (kept.data.is_contiguous() and kept.scale.is_contiguous()):
         raise ValueError("kept must be contiguous")
 
@@ -1045,36 +1055,34 @@ _lib.register("i2pc_attention_packed_backward", ctypes.c_int, [ctypes.POINTER(At
                                                                c_void_p])
 
 
-def _attn_packed_desc(d, q, k, v, cu_q, cu_k, k_lens, scale, causal):
-    """Checks the operands of a packed attention call and fills the descriptor's input side."""
+def _attn_packed_desc(q, k, v, out, lse, cu_q, cu_k, k_lens, scale, causal, zero_tail):
+    """Checks the operands of a packed attention call and makes its descriptor."""
     torch = _torch()
-    bf = (torch.bfloat16,)
-    i32 = (torch.int32,)
+    bf, i32 = (torch.bfloat16,), (torch.int32,)
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"q, k: expected [tokens, heads, head_dim], got the shapes {tuple(q.shape)}, {tuple(k.shape)}")
     tq, heads, hd = q.shape
-    tk, kv = k.shape[0], k.shape[1]
-    _operand(q, "q", q.shape, bf)
+    tk, kv, _ = k.shape
+    _operand(q, "q", (tq, heads, hd), bf)
     _operand(k, "k", (tk, kv, hd), bf, q)
     _operand(v, "v", (tk, kv, hd), bf, q)
+    _operand(out, "out", (tq, heads, hd), bf, q)
+    _dense(lse, "lse", (tq, heads), q)
     if cu_q.dim() != 1 or cu_q.shape[0] < 2:
         raise ValueError(f"cu_q: expected int32 [sequences + 1] of one sequence at least, got the shape {tuple(cu_q.shape)}")
-    batch = cu_q.shape[0] - 1
-    _operand(cu_q, "cu_q", (batch + 1,), i32, q)
+    n = cu_q.shape[0]
+    _operand(cu_q, "cu_q", (n,), i32, q)
     if cu_k is None:
         if tk != tq:
             raise ValueError(f"k has {tk} rows and q {tq}: give cu_k")
         cu_k = cu_q
-    _operand(cu_k, "cu_k", (batch + 1,), i32, q)
+    else:
+        _operand(cu_k, "cu_k", (n,), i32, q)
     if k_lens is not None:
-        _operand(k_lens, "k_lens", (batch,), i32, q)
-    d.q, d.q_t, d.q_h = _p(q), q.stride(0), q.stride(1)
-    d.k, d.k_t, d.k_h = _p(k), k.stride(0), k.stride(1)
-    d.v, d.v_t, d.v_h = _p(v), v.stride(0), v.stride(1)
-    d.cu_q, d.cu_k, d.k_lens = _p(cu_q), _p(cu_k), _p(k_lens)
-    d.batch, d.total_q, d.total_k, d.heads, d.kv_heads, d.head_dim = batch, tq, tk, heads, kv, hd
-    d.causal = int(bool(causal))
-    d.scale = hd ** -0.5 if scale is None else float(scale)
+        _operand(k_lens, "k_lens", (n - 1,), i32, q)
+    (q_t, q_h, _), (k_t, k_h, _), (v_t, v_h, _), (o_t, o_h, _) = q.stride(), k.stride(), v.stride(), out.stride()
+    return AttnPackedDesc(_p(q), _p(k), _p(v), q_t, q_h, k_t, k_h, v_t, v_h, _p(out), o_t, o_h, _p(lse), _p(cu_q), _p(cu_k),
+                          _p(k_lens), n - 1, tq, tk, heads, kv, hd, bool(causal), zero_tail, hd ** -0.5 if scale is None else scale)
 
 
 def attention_packed(q, k, v, cu_q, cu_k=None, k_lens=None, scale=None, causal=False, out=None, lse=None):
@@ -1087,29 +1095,24 @@ def attention_packed(q, k, v, cu_q, cu_k=None, k_lens=None, scale=None, causal=F
     slab).  cu_k None: the keys are packed as the queries are.  The lengths are read on the device when the kernel
     runs.  causal: query i of lq sees the keys j <= i + lk - lq of lk.  scale defaults to 1 / 8.
     out bf16 [total_q, heads, 64]; lse fp32 [total_q, heads] = log(sum(exp(scores))).  A query that sees no key has
-    out 0, lse -inf.  Rows behind the last sequence keep what a given `out` / `lse` holds, and are 0 / -inf in new ones.
+    out 0, lse -inf.  Rows behind the last sequence keep what a given `out` / `lse` holds (give both, or neither), and
+    are 0 / -inf in new ones.
     """
     torch = _torch()
-    d = AttnPackedDesc()
-    _attn_packed_desc(d, q, k, v, cu_q, cu_k, k_lens, scale, causal)
+    if (out is None) != (lse is None):
+        raise ValueError("give both out and lse, or neither")
     with _on_device_of(q):
-        d.zero_tail = int(out is None)
-        if (out is None) != (lse is None):
-            raise ValueError("give both out and lse, or neither")
-        if out is None:
-            out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-        else:
-            _operand(out, "out", q.shape, (torch.bfloat16,), q)
-            _operand(lse, "lse", q.shape[:2], (torch.float32,), q)
-            if not lse.is_contiguous():
-                raise ValueError("lse must be contiguous")
-        d.out, d.o_t, d.o_h, d.lse = _p(out), out.stride(0), out.stride(1), _p(lse)
-        nb = _lib.load().i2pc_attention_packed_workspace_bytes(ctypes.byref(d))
-        ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
-        # flops of the dense bound are not known here (the lengths are on the device)
-        with _Timed("k_attnp_fwd", 0.0, 2.0 * (2 * q.numel() + k.numel() + v.numel()) + 4.0 * lse.numel()):
-            _lib.call("i2pc_attention_packed", ctypes.byref(d), _p(ws), nb, _stream())
+        fresh = out is None
+        if fresh:
+            out = q.new_empty(q.shape)
+            lse = q.new_empty(q.shape[:2], dtype=torch.float32)
+        d = _attn_packed_desc(q, k, v, out, lse, cu_q, cu_k, k_lens, scale, causal, fresh)
+        ref = ctypes.byref(d)
+        nb = _lib.load().i2pc_attention_packed_workspace_bytes(ref)
+        ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
+        # the lengths are on the device: the flops of the call are not known here
+        _launch("k_attnp_fwd", 2.0 * (2 * q.numel() + k.numel() + v.numel()) + 4.0 * lse.numel(), "i2pc_attention_packed", q, ref,
+                _p(ws), nb)
     return out, lse
 
 
@@ -1119,36 +1122,23 @@ def attention_packed_backward(dout, q, k, v, out, lse, cu_q, cu_k=None, scale=No
     head; all sums are fp32 in a fixed order.  Rows behind the last sequence keep what a given dq / dk / dv holds (give all
     three, or none), and are 0 in new ones."""
     torch = _torch()
-    g = AttnPackedGradDesc()
-    d = g.f
     bf = (torch.bfloat16,)
-    _attn_packed_desc(d, q, k, v, cu_q, cu_k, None, scale, causal)
-    _operand(dout, "dout", q.shape, bf, q)
-    _operand(out, "out", q.shape, bf, q)
-    _operand(lse, "lse", q.shape[:2], (torch.float32,), q)
-    if not lse.is_contiguous():
-        raise ValueError("lse must be contiguous")
-    given = [t is not None for t in (dq, dk, dv)]
-    if any(given) and not all(given):
+    fresh = dq is None
+    if (dk is None) != fresh or (dv is None) != fresh:
         raise ValueError("give all of dq, dk, dv, or none")
     with _on_device_of(q):
-        d.zero_tail = int(not any(given))
-        if any(given):
+        d = _attn_packed_desc(q, k, v, out, lse, cu_q, cu_k, None, scale, causal, fresh)
+        _operand(dout, "dout", q.shape, bf, q)
+        if fresh:
+            dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape)
+        else:
             _operand(dq, "dq", q.shape, bf, q)
             _operand(dk, "dk", k.shape, bf, q)
             _operand(dv, "dv", v.shape, bf, q)
-        else:
-            dq = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-            dk = torch.empty(k.shape, dtype=torch.bfloat16, device=q.device)
-            dv = torch.empty(v.shape, dtype=torch.bfloat16, device=q.device)
-        d.out, d.o_t, d.o_h, d.lse = _p(out), out.stride(0), out.stride(1), _p(lse)
-        g.dout, g.d_t, g.d_h = _p(dout), dout.stride(0), dout.stride(1)
-        g.dq, g.dq_t, g.dq_h = _p(dq), dq.stride(0), dq.stride(1)
-        g.dk, g.dk_t, g.dk_h = _p(dk), dk.stride(0), dk.stride(1)
-        g.dv, g.dv_t, g.dv_h = _p(dv), dv.stride(0), dv.stride(1)
-        nb = _lib.load().i2pc_attention_packed_backward_workspace_bytes(ctypes.byref(g))
-        ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
-        nbytes = 2.0 * (4 * q.numel() + 2 * k.numel() + 2 * v.numel()) + 4.0 * lse.numel()
-        with _Timed("k_attnp_bwd", 0.0, nbytes):
-            _lib.call("i2pc_attention_packed_backward", ctypes.byref(g), _p(ws), nb, _stream())
+        (d_t, d_h, _), (dq_t, dq_h, _), (dk_t, dk_h, _), (dv_t, dv_h, _) = dout.stride(), dq.stride(), dk.stride(), dv.stride()
+        ref = ctypes.byref(AttnPackedGradDesc(d, _p(dout), d_t, d_h, _p(dq), _p(dk), _p(dv), dq_t, dq_h, dk_t, dk_h, dv_t, dv_h))
+        nb = _lib.load().i2pc_attention_packed_backward_workspace_bytes(ref)
+        ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
+        _launch("k_attnp_bwd", 2.0 * (4 * q.numel() + 2 * k.numel() + 2 * v.numel()) + 4.0 * lse.numel(),
+                "i2pc_attention_packed_backward", q, ref, _p(ws), nb)
     return dq, dk, dv

@@ -40,7 +40,9 @@ class _Device:
 
     def __init__(self, t):
         self._t = t
-        self.is_cuda = True
+
+    def get_device(self):
+        return 0
 
     def __getattr__(self, n):
         return getattr(self._t, n)
@@ -50,6 +52,8 @@ def test_shapes_types_and_strides():
     bf = torch.bfloat16
     op = ops._operand
     op(_Device(torch.zeros(3, 4)), "t", (3, 4), (torch.float32,))
+    with pytest.raises(_lib.I2PCError):
+        op(torch.zeros(3, 4), "t", (3, 4), (torch.float32,))
     with pytest.raises(TypeError):
         op(_Device(torch.zeros(3, 4)), "t", (3, 4), (bf,))
     with pytest.raises(ValueError):
@@ -64,12 +68,25 @@ def test_shapes_types_and_strides():
         ops._kept_operand(torch.zeros(2, 32), 2, 32, None)
     with pytest.raises(ValueError):
         ops._kept_operand(ops.Fp8(None, None), 2, 33, None)
-    q = _Device(torch.zeros(4, 2, 64, dtype=bf))
-    for bad_cu in (torch.zeros(1, dtype=torch.int32), torch.zeros(2, 2, dtype=torch.int32)):
+    dev = lambda *shape, dtype=bf: _Device(torch.zeros(*shape, dtype=dtype))              # noqa: E731
+    q, lse, cu = dev(4, 2, 64), dev(4, 2, dtype=torch.float32), dev(2, dtype=torch.int32)
+    desc = lambda q=q, k=q, v=q, out=q, lse=lse, cu_q=cu, cu_k=None, k_lens=None: ops._attn_packed_desc(               # noqa: E731
+        q, k, v, out, lse, cu_q, cu_k, k_lens, None, True, False)
+    d = desc()
+    assert (d.batch, d.total_q, d.heads, d.causal, d.scale, d.q_t, d.o_h) == (1, 4, 2, 1, 0.125, 128, 64)
+    for kw in ({"q": dev(4, 128)}, {"k": dev(4, 2, 32)}, {"v": dev(5, 2, 64)}, {"out": dev(3, 2, 64)}, {"lse": dev(2, 4, dtype=torch.float32)},
+               {"cu_q": dev(1, dtype=torch.int32)}, {"cu_q": dev(2, 2, dtype=torch.int32)}, {"cu_k": dev(3, dtype=torch.int32)},
+               {"k": dev(5, 2, 64), "v": dev(5, 2, 64)}, {"k_lens": dev(2, dtype=torch.int32)},
+               {"lse": _Device(torch.zeros(2, 4).t())}):
         with pytest.raises(ValueError):
-            ops.attention_packed(q, q, q, bad_cu)
-    with pytest.raises(ValueError):                                      # other rows than q's need a cu_k
-        ops.attention_packed(q, *[_Device(torch.zeros(5, 2, 64, dtype=bf))] * 2, _Device(torch.zeros(2, dtype=torch.int32)))
+            desc(**kw)
+    for kw in ({"q": dev(4, 2, 64, dtype=torch.float16)}, {"cu_q": dev(2, dtype=torch.int64)}, {"k_lens": dev(1, dtype=torch.int64)}):
+        with pytest.raises(TypeError):
+            desc(**kw)
+    with pytest.raises(ValueError):
+        ops.attention_packed(q, q, q, cu, out=q)
+    with pytest.raises(ValueError):
+        ops.attention_packed_backward(q, q, q, q, q, lse, cu, dq=q)
 
 
 def _rc(name, *args):
@@ -89,11 +106,13 @@ def test_layernorm_refusals():
     lib = _lib.load()
     need = lib.i2pc_layernorm_backward_workspace_bytes(100, 384)
     assert need > 0 and lib.i2pc_layernorm_backward_workspace_bytes(100, 9000) == 0
+    assert lib.i2pc_layernorm_backward_workspace_bytes(8, 384) == 0            # one workgroup: no partial rows
 
     def backward(rows=100, dim=384, lda=384, ws=16, nb=need, dx=16):
         return _rc("i2pc_layernorm_backward", 16, dim, 16, 1, dim, 16, 16, 16, lda, rows, dim, dx, dim, 16, 16, ws, nb, None)
     assert backward(nb=need - 1)[0] == -2
-    for kw in ({"rows": -1}, {"dim": 9000}, {"lda": 100}, {"ws": None}, {"dx": None}):
+    assert backward(ws=None)[0] == -2
+    for kw in ({"rows": -1}, {"dim": 9000}, {"lda": 100}, {"dx": None}):
         assert backward(**kw)[0] == -1, kw
 
 

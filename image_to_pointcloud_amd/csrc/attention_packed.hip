@@ -33,7 +33,6 @@ using attn::tr_read;
 using attn::v4s;
 
 constexpr int kRows = 128;       // packed rows of a workgroup: 4 waves x 32
-constexpr int kKeys = 64;        // keys of a dK / dV workgroup
 
 struct Args {
   const bf16_t *q, *k, *v;
@@ -124,14 +123,24 @@ __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rs, uint32_t lds_bas
                : "memory", "m0");
 }
 
-// A descriptor over `rows` rows of `pitch` elements from p (64 values of the last row): reads behind it give
-// zero.  The base is 64 bits and moves with the tile, so a sequence may span more than 4 GiB.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* p, int64_t pitch, int rows) {
-  const int64_t bytes = rows > 0 ? ((rows - 1) * pitch + 64) * 2 : 0;
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)min(bytes, (int64_t)0x7fffffff), 0x00020000);
-}
+// Where a tile of rows is read from: its first row and the bytes from there through the last row's 64 values.  Reads
+// behind them give zero.  The base is 64 bits and moves with the tile, so a sequence may span more than 4 GiB; moving it
+// is a few scalar additions.
+struct Src {
+  const uint8_t* p;
+  int64_t left;
+  __device__ __forceinline__ Src(const bf16_t* row, int64_t pitch, int rows)
+      : p(reinterpret_cast<const uint8_t*>(row)), left(((rows - 1) * pitch + 64) * 2) {}
+  __device__ __forceinline__ void move(int64_t bytes) {
+    p += bytes;
+    left -= bytes;
+  }
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc() const {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, (int)min(left, (int64_t)0x7fffffff), 0x00020000);
+  }
+};
 
-// one wave's quarter of a 64-row tile: 2 instructions of 8 rows x 128 B
+// one wave's quarter of a 64-row tile: 2 instructions of 8 rows x 128 B, to `lds` and 1 KiB behind it
 struct Stage {
   uint32_t off[2];
   __device__ __forceinline__ Stage(int wid, int lane, int64_t pitch) {
@@ -141,9 +150,9 @@ struct Stage {
       off[j] = (uint32_t)((row * pitch + ((lane & 7) ^ swz(row)) * 8) * 2);
     }
   }
-  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, const uint8_t* tile, int wid) const {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) dma16(rs, __builtin_amdgcn_readfirstlane(lds_addr(tile + (wid * 2 + j) * 1024)), off[j]);
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t lds) const {
+    dma16(rs, lds, off[0]);
+    dma16(rs, lds + 1024, off[1]);
   }
 };
 
@@ -183,8 +192,10 @@ __device__ __forceinline__ float dot_row(const bf16_t* row, const bf16x8 (&f)[4]
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     const bf16x8 x = *reinterpret_cast<const bf16x8*>(row + 16 * t + 8 * hh);
+    bf16x8 y = f[t];
+    asm volatile("" : "+v"(y));                      // its conversion is not kept in registers from row to row
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s = fmaf((float)x[j], (float)f[t][j], s);
+    for (int j = 0; j < 8; ++j) s = fmaf((float)x[j], (float)y[j], s);
   }
   return s + __shfl_xor(s, 32);
 }
@@ -199,6 +210,14 @@ __device__ __forceinline__ void add_row(f32x16 (&acc)[2], float w, const bf16_t*
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[dt][4 * g + i] = fmaf(w, e[i], acc[dt][4 * g + i]);
     }
+}
+
+// whether this lane's part of rows base .. base + 31 of a tile has an infinity or NaN
+__device__ __forceinline__ int has_nonfinite(const uint8_t* tile, int base, int lane) {
+  int bad = 0;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) bad |= nonfinite(row_frag(tile, base + (lane & 31), t, lane >> 5));
+  return bad;
 }
 
 // 4 consecutive values a lane and register group of an accumulator, times f, as bf16: row[32 dt + 8 g + 4 hh ...]
@@ -261,9 +280,9 @@ __device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const uin
 #pragma unroll
   for (int t = 0; t < 4; ++t) st = mfma(kf[t], qf[t], t == 0 ? w.nm : st);
   if (partial) {
+    const int lim = left - 4 * hh;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if ((i & 3) + 8 * (i >> 2) + 4 * hh >= left) st[i] = -INFINITY;
+    for (int i = 0; i < 16; ++i) st[i] = (i & 3) + 8 * (i >> 2) < lim ? st[i] : -INFINITY;
   }
   float ls = 0.f;
   uint32_t pk[8];
@@ -310,10 +329,7 @@ __device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const uin
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt) vf[t][dt] = tr_frag(sV, base + 16 * t, dt, lane);
-  if (CAUSAL && partial) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) w.bad |= (int)nonfinite(vf[t][0]) | (int)nonfinite(vf[t][1]);
-  }
+  if (CAUSAL && partial) w.bad |= has_nonfinite(sV, base, lane);
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -344,15 +360,19 @@ __device__ __forceinline__ void attend_again(Rows& w, const bf16x8 (&qf)[4], con
   w.l = hh ? 0.f : l;                                // the whole sum; the halves' are added
 }
 
-// One workgroup: 128 packed rows of one key head, over all of their keys or (SPLIT) over one of nsplit shares of
+// One workgroup: 128 / KW packed rows of one key head, over all of their keys or (SPLIT) over one of nsplit shares of
 // them.  Each wave owns 32 rows, a row to a lane: S^T = K Q^T leaves a query's scores in one lane's
 // registers, which then are the B operand of O^T += V^T P^T.  K and V tiles of 64 keys go through LDS by
-// LDS-DMA, double-buffered.
-template <bool CAUSAL, bool SPLIT>
+// LDS-DMA, double-buffered.  KW 2: waves 2, 3 hold the rows of waves 0, 1 again and take the second 32 keys of each tile,
+// and the two states are joined at the end: twice the workgroups, of half the length.
+template <bool CAUSAL, bool SPLIT, int KW>
 __global__ __launch_bounds__(256, 3) void k_attnp_fwd(const Args a) {
+  constexpr int kWgRows = kRows / KW;
   __shared__ __attribute__((aligned(16))) uint8_t smem[4 * kTileBytes];
+  __shared__ float ml[2][KW == 2 ? 2 : 1][KW == 2 ? 64 : 1];
   const int lane = threadIdx.x & 63, hh = lane >> 5, lr = lane & 31;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rw = KW == 2 ? wid & 1 : wid, kw = KW == 2 ? wid >> 1 : 0;
   // key heads fastest: workgroups b and b + 8 share an XCD, so with 8 heads (4, 2) each XCD (pair, four) keeps to
   // one head's keys; later tiles, which a causal mask leaves the most keys, come first
   const int hk = blockIdx.x % a.Hk;
@@ -361,36 +381,41 @@ __global__ __launch_bounds__(256, 3) void k_attnp_fwd(const Args a) {
   if (SPLIT) rest /= a.nsplit;
   const int tiles = gridDim.x / (a.Hk * (SPLIT ? a.nsplit : 1));
   int tile;
-  const int b = find_tile(a.cu_q, a.Tq, a.G, kRows, a.B + a.zero_tail, tiles - 1 - rest, lane, tile);
+  const int b = find_tile(a.cu_q, a.Tq, a.G, kWgRows, a.B + a.zero_tail, tiles - 1 - rest, lane, tile);
   if (b == a.B) {                                    // the rows behind the last sequence
     const int t0 = cu_at(a.cu_q, a.B, a.Tq);
-    if (!SPLIT) zero_rows(a.out, a.o_t, a.o_h, t0, tile * kRows, (a.Tq - t0) * a.G, hk, a.G, a.lse, a.H);
+    if (!SPLIT) zero_rows(a.out, a.o_t, a.o_h, t0, tile * kWgRows, min((tile + 1) * kWgRows, (a.Tq - t0) * a.G), hk, a.G, a.lse, a.H);
     return;
   }
   const Seq s = sequence(a, b);
-  const int R = s.lq * a.G, r0 = tile * kRows;
+  const int R = s.lq * a.G, r0 = tile * kWgRows;
   if (r0 >= R) return;
-  const int r = r0 + wid * 32 + lr, rc = min(r, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
+  const int r = r0 + rw * 32 + lr, rc = min(r, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
   const int nk = seen(CAUSAL, qi, s);
   // first and last row of the wave, last row of the tile (uniform)
-  const int w0 = min(r0 + wid * 32, R - 1);
-  const bool wave_on = r0 + wid * 32 < R;
+  const int w0 = min(r0 + rw * 32, R - 1);
+  const bool wave_on = r0 + rw * 32 < R;
   const int nk_first = seen(CAUSAL, w0 / a.G, s), nk_last = seen(CAUSAL, min(w0 + 31, R - 1) / a.G, s);
-  int ks = 0, ke = seen(CAUSAL, (min(r0 + kRows, R) - 1) / a.G, s);
+  int ks = 0, ke = seen(CAUSAL, (min(r0 + kWgRows, R) - 1) / a.G, s);
   if (SPLIT) {
     const int chunk = ((s.lk + a.nsplit - 1) / a.nsplit + kKV - 1) / kKV * kKV;
-    ks = min((int64_t)split * chunk, (int64_t)ke);
+    ks = (int)min((int64_t)split * chunk, (int64_t)ke);
     ke = min(ke, ks + chunk);
   }
 
   const bf16_t* Kg = a.k + (s.k0 * a.k_t + hk * a.k_h);
   const bf16_t* Vg = a.v + (s.k0 * a.v_t + hk * a.v_h);
   const Stage stk(wid, lane, a.k_t), stv(wid, lane, a.v_t);
-  auto stage = [&](int buf, int key) {
-    stk.load(rows_rsrc(Kg + key * a.k_t, a.k_t, s.lk - key), smem + buf * 2 * kTileBytes, wid);
-    stv.load(rows_rsrc(Vg + key * a.v_t, a.v_t, s.lk - key), smem + (buf * 2 + 1) * kTileBytes, wid);
+  Src srck(Kg + ks * a.k_t, a.k_t, s.lk - ks), srcv(Vg + ks * a.v_t, a.v_t, s.lk - ks);
+  const int64_t stepk = a.k_t * kKV * 2, stepv = a.v_t * kKV * 2;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem)) + wid * 2048;
+  auto stage = [&](int buf) {                        // the next tile
+    stk.load(srck.rsrc(), lds0 + buf * 2 * kTileBytes);
+    stv.load(srcv.rsrc(), lds0 + (buf * 2 + 1) * kTileBytes);
+    srck.move(stepk);
+    srcv.move(stepv);
   };
-  if (ks < ke) stage(0, ks);
+  if (ks < ke) stage(0);
   bf16x8 qf[4];
   {
     const bf16_t* qr = a.q + (s.q0 + qi) * a.q_t + h * a.q_h;
@@ -404,24 +429,51 @@ __global__ __launch_bounds__(256, 3) void k_attnp_fwd(const Args a) {
   Rows w;
   w.clear();
   for (int key0 = ks, cur = 0; key0 < ke; key0 += kKV, cur ^= 1) {
-    if (key0 + kKV < ke) stage(cur ^ 1, key0 + kKV);
+    if (key0 + kKV < ke) stage(cur ^ 1);
     const uint8_t* sK = smem + cur * 2 * kTileBytes;
     if (wave_on) {
 #pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2) {
-        const int key = key0 + 32 * k2;
+      for (int k2 = 0; k2 < 2 / KW; ++k2) {
+        const int at = 32 * (k2 + kw), key = key0 + at;
         if (key >= nk_last) break;                   // no row of the wave sees these keys
-        attend<CAUSAL>(w, qf, sK, sK + kTileBytes, 32 * k2, key == ks, key + 32 > nk_first, nk - key, c, lane);
+        attend<CAUSAL>(w, qf, sK, sK + kTileBytes, at, key == ks + 32 * kw, key + 32 > nk_first, nk - key, c, lane);
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the next tile landed (this wave's part)
     __syncthreads();                                     // ... and every wave's
   }
-  if (CAUSAL && __ballot(w.bad) != 0) attend_again(w, qf, Kg, a.k_t, Vg, a.v_t, ks, min(ke, nk_last), 1, nk, c, hh);
-  const float l = w.l + __shfl_xor(w.l, 32);
+  if (CAUSAL && __ballot(w.bad) != 0)
+    attend_again(w, qf, Kg, a.k_t, Vg, a.v_t, ks + 32 * kw, min(ke, nk_last), KW == 2 ? 33 : 1, nk, c, hh);
+  float l = w.l + __shfl_xor(w.l, 32), m = -w.nm[0];
+  if constexpr (KW == 2) {
+    float* x = reinterpret_cast<float*>(smem) + rw * 32 * 64 + lane;
+    if (kw == 1) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x[i * 64] = w.o[0][i];
+        x[(16 + i) * 64] = w.o[1][i];
+      }
+      ml[0][rw][lane] = m;
+      ml[1][rw][lane] = l;
+    }
+    __syncthreads();
+    if (kw == 1) return;
+    const float m1 = ml[0][rw][lane], l1 = ml[1][rw][lane];
+    if (l1 != 0.f) {                                 // (NaN: joined too)
+      const float mm = l == 0.f ? m1 : fmaxf(m, m1);
+      const float f0 = m == mm ? 1.f : __builtin_amdgcn_exp2f((m - mm) * c), f1 = m1 == mm ? 1.f : __builtin_amdgcn_exp2f((m1 - mm) * c);
+      l = l == 0.f ? l1 * f1 : fmaf(l, f0, l1 * f1);
+      m = mm;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        w.o[0][i] = fmaf(w.o[0][i], f0, x[i * 64] * f1);
+        w.o[1][i] = fmaf(w.o[1][i], f0, x[(16 + i) * 64] * f1);
+      }
+    }
+  }
   if (r >= R) return;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  const float l2 = l == 0.f ? -INFINITY : fmaf(-w.nm[0], c, log2f(l));
+  const float l2 = l == 0.f ? -INFINITY : fmaf(m, c, log2f(l));
   if (SPLIT) {
     const int64_t row = ((int64_t)split * a.Hk + hk) * a.Tq * a.G + (int64_t)s.q0 * a.G + r;
     if (hh == 0) a.part_l[row] = l2;
@@ -481,13 +533,19 @@ __global__ __launch_bounds__(256, 2) void k_attnp_few(const Args a) {
     offv[j] = (uint32_t)((row * a.v_t + ch) * 2);
   }
   uint8_t* mine = smem + wid * 4 * kFewBlock;
-  auto stage = [&](int buf, int key) {
-    const auto rk = rows_rsrc(Kg + key * a.k_t, a.k_t, s.lk - key), rv = rows_rsrc(Vg + key * a.v_t, a.v_t, s.lk - key);
-    const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(mine + buf * 2 * kFewBlock));
+  const int first = ks + 32 * wid;
+  Src srck(Kg + first * a.k_t, a.k_t, s.lk - first), srcv(Vg + first * a.v_t, a.v_t, s.lk - first);
+  const int64_t stepk = a.k_t * 256, stepv = a.v_t * 256;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(mine));
+  auto stage = [&](int buf) {                        // the wave's next block
+    const auto rk = srck.rsrc(), rv = srcv.rsrc();
+    const uint32_t base = lds0 + buf * 2 * kFewBlock;
 #pragma unroll
     for (int j = 0; j < 4; ++j) dma16(rk, base + j * 1024, offk[j]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) dma16(rv, base + kFewBlock + j * 1024, offv[j]);
+    srck.move(stepk);
+    srcv.move(stepv);
   };
   bf16x8 qf[4];
   {
@@ -495,8 +553,7 @@ __global__ __launch_bounds__(256, 2) void k_attnp_few(const Args a) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) qf[t] = *reinterpret_cast<const bf16x8*>(qr + 16 * t + 8 * hh);
   }
-  const int first = ks + 32 * wid;
-  if (first < ke) stage(0, first);
+  if (first < ke) stage(0);
   const float c = a.c;
   Rows w;
   w.clear();
@@ -504,7 +561,7 @@ __global__ __launch_bounds__(256, 2) void k_attnp_few(const Args a) {
     if (key + 128 < ke) {
       // the other buffer's reads have returned before it is written again
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      stage(cur ^ 1, key + 128);
+      stage(cur ^ 1);
       asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // this block landed, the next one's 8 loads may be on their way
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -641,38 +698,46 @@ __global__ __launch_bounds__(256) void k_attnp_delta(const Args a) {
   }
 }
 
-// dQ: the forward's rows and tiles; per 32 keys S^T = K Q^T and dP^T = V dO^T, then dQ^T += K^T dS^T.
-template <bool CAUSAL>
+// dQ: the forward's rows and tiles; per 32 keys S^T = K Q^T and dP^T = V dO^T (which starts at -D), then
+// dQ^T += K^T dS^T.  KW 2 as in the forward pass.
+template <bool CAUSAL, int KW>
 __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
+  constexpr int kWgRows = kRows / KW;
   __shared__ __attribute__((aligned(16))) uint8_t smem[4 * kTileBytes];
   const int lane = threadIdx.x & 63, hh = lane >> 5, lr = lane & 31;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rw = KW == 2 ? wid & 1 : wid, kw = KW == 2 ? wid >> 1 : 0;
   const int hk = blockIdx.x % a.Hk, tiles = gridDim.x / a.Hk;
   int tile;
-  const int b = find_tile(a.cu_q, a.Tq, a.G, kRows, a.B + a.zero_tail, tiles - 1 - (int)(blockIdx.x / a.Hk), lane, tile);
+  const int b = find_tile(a.cu_q, a.Tq, a.G, kWgRows, a.B + a.zero_tail, tiles - 1 - (int)(blockIdx.x / a.Hk), lane, tile);
   if (b == a.B) {
     const int t0 = cu_at(a.cu_q, a.B, a.Tq);
-    zero_rows(a.dq, a.dq_t, a.dq_h, t0, tile * kRows, (a.Tq - t0) * a.G, hk, a.G, nullptr, 0);
+    zero_rows(a.dq, a.dq_t, a.dq_h, t0, tile * kWgRows, min((tile + 1) * kWgRows, (a.Tq - t0) * a.G), hk, a.G, nullptr, 0);
     return;
   }
   const Seq s = sequence(a, b);
-  const int R = s.lq * a.G, r0 = tile * kRows;
+  const int R = s.lq * a.G, r0 = tile * kWgRows;
   if (r0 >= R) return;
-  const int r = r0 + wid * 32 + lr, rc = min(r, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
+  const int r = r0 + rw * 32 + lr, rc = min(r, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
   const int nk = seen(CAUSAL, qi, s);
-  const int w0 = min(r0 + wid * 32, R - 1);
-  const bool wave_on = r0 + wid * 32 < R;
+  const int w0 = min(r0 + rw * 32, R - 1);
+  const bool wave_on = r0 + rw * 32 < R;
   const int nk_first = seen(CAUSAL, w0 / a.G, s), nk_last = seen(CAUSAL, min(w0 + 31, R - 1) / a.G, s);
-  const int ke = seen(CAUSAL, (min(r0 + kRows, R) - 1) / a.G, s);
+  const int ke = seen(CAUSAL, (min(r0 + kWgRows, R) - 1) / a.G, s);
 
   const bf16_t* Kg = a.k + (s.k0 * a.k_t + hk * a.k_h);
   const bf16_t* Vg = a.v + (s.k0 * a.v_t + hk * a.v_h);
   const Stage stk(wid, lane, a.k_t), stv(wid, lane, a.v_t);
-  auto stage = [&](int buf, int key) {
-    stk.load(rows_rsrc(Kg + key * a.k_t, a.k_t, s.lk - key), smem + buf * 2 * kTileBytes, wid);
-    stv.load(rows_rsrc(Vg + key * a.v_t, a.v_t, s.lk - key), smem + (buf * 2 + 1) * kTileBytes, wid);
+  Src srck(Kg, a.k_t, s.lk), srcv(Vg, a.v_t, s.lk);
+  const int64_t stepk = a.k_t * kKV * 2, stepv = a.v_t * kKV * 2;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem)) + wid * 2048;
+  auto stage = [&](int buf) {
+    stk.load(srck.rsrc(), lds0 + buf * 2 * kTileBytes);
+    stv.load(srcv.rsrc(), lds0 + (buf * 2 + 1) * kTileBytes);
+    srck.move(stepk);
+    srcv.move(stepv);
   };
-  if (ke > 0) stage(0, 0);
+  if (ke > 0) stage(0);
   bf16x8 qf[4], df[4];
   const bf16_t* qr = a.q + (s.q0 + qi) * a.q_t + h * a.q_h;
   const bf16_t* dr = a.dout + (s.q0 + qi) * a.d_t + h * a.d_h;
@@ -695,44 +760,35 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
 
   int bad = 0;
   for (int key0 = 0, cur = 0; key0 < ke; key0 += kKV, cur ^= 1) {
-    if (key0 + kKV < ke) stage(cur ^ 1, key0 + kKV);
+    if (key0 + kKV < ke) stage(cur ^ 1);
     const uint8_t* sK = smem + cur * 2 * kTileBytes;
     const uint8_t* sV = sK + kTileBytes;
     if (wave_on) {
 #pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2) {
-        if (key0 + 32 * k2 >= nk_last) break;
+      for (int k2 = 0; k2 < 2 / KW; ++k2) {
+        const int at = 32 * (k2 + kw), key = key0 + at;
+        if (key >= nk_last) break;
         f32x16 st, dp;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          st = mfma(row_frag(sK, 32 * k2 + lr, t, hh), qf[t], t == 0 ? f32x16{} : st);
-          dp = mfma(row_frag(sV, 32 * k2 + lr, t, hh), df[t], t == 0 ? nd : dp);
+          st = mfma(row_frag(sK, at + lr, t, hh), qf[t], t == 0 ? f32x16{} : st);
+          dp = mfma(row_frag(sV, at + lr, t, hh), df[t], t == 0 ? nd : dp);
         }
-        const bool partial = key0 + 32 * k2 + 32 > nk_first;
-        const int left = nk - key0 - 32 * k2;
 #pragma unroll
         for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(fmaf(st[i], c, nl));
-        if (partial) {
+        if (key + 32 > nk_first) {                   // some row of the wave does not see all of the block
+          const int lim = nk - key - 4 * hh;
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if ((i & 3) + 8 * (i >> 2) + 4 * hh >= left) dp[i] = 0.f;
+          for (int i = 0; i < 16; ++i) dp[i] = (i & 3) + 8 * (i >> 2) < lim ? dp[i] : 0.f;
+          if (CAUSAL) bad |= has_nonfinite(sK, at, lane);
         }
         uint32_t pk[8];
 #pragma unroll
         for (int i = 0; i < 16; i += 2) pk[i >> 1] = pack_bf16(dp[i], dp[i + 1]);
-        bf16x8 kt[2][2];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int dt = 0; dt < 2; ++dt) kt[t][dt] = tr_frag(sK, 32 * k2 + 16 * t, dt, lane);
-        if (CAUSAL && partial) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t) bad |= (int)nonfinite(kt[t][0]) + (int)nonfinite(kt[t][1]);
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int dt = 0; dt < 2; ++dt) dq[dt] = mfma(kt[t][dt], p_frag(pk, t), dq[dt]);
+          for (int dt = 0; dt < 2; ++dt) dq[dt] = mfma(tr_frag(sK, at + 16 * t, dt, lane), p_frag(pk, t), dq[dt]);
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -741,33 +797,54 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
   if (CAUSAL && __ballot(bad) != 0) {
     for (int i = 0; i < 16; ++i) dq[0][i] = dq[1][i] = 0.f;
 #pragma clang loop unroll(disable)
-    for (int j = 0; j < nk_last; ++j) {
+    for (int j = 32 * kw; j < nk_last; j += KW == 2 && (j & 31) == 31 ? 33 : 1) {
       const float x = dot_row(Kg + j * a.k_t, qf, hh), y = dot_row(Vg + j * a.v_t, df, hh);
       if (j < nk) add_row(dq, __builtin_amdgcn_exp2f(fmaf(x, c, nl)) * (y + nd[0]), Kg + j * a.k_t, hh);
+    }
+  }
+  if constexpr (KW == 2) {
+    float* x = reinterpret_cast<float*>(smem) + rw * 32 * 64 + lane;
+    if (kw == 1) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x[i * 64] = dq[0][i];
+        x[(16 + i) * 64] = dq[1][i];
+      }
+    }
+    __syncthreads();
+    if (kw == 1) return;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      dq[0][i] += x[i * 64];
+      dq[1][i] += x[(16 + i) * 64];
     }
   }
   if (r < R) store_acc(a.dq + (s.q0 + qi) * a.dq_t + h * a.dq_h, dq, a.scale, hh);
 }
 
-// dK, dV: 64 keys of one key head a workgroup, over the rows of its G query heads one after the other.  A key to a
-// lane: S = Q K^T and dP = dO V^T leave a key's column in one lane's registers, which then are the B operand of
-// dV^T += dO^T P and dK^T += Q^T dS.  Waves 0, 1 take rows 0-31 of each 64-row tile, waves 2, 3 rows 32-63; their sums
-// are added at the end.
-template <bool CAUSAL>
+// dK, dV: 32 KW keys of one key head a workgroup, over the rows of its query heads one after the other (of one of them
+// with a.nsplit = G: partial sums, joined by k_attnp_sum).  A key to a lane: S = Q K^T (which starts at -lse / scale) and
+// dP = dO V^T (at -D) leave a key's column in one lane's registers, which then are the B operand of dV^T += dO^T P and
+// dK^T += Q^T dS.  KW 4: every wave has 32 keys and takes all 64 rows of a tile; KW 2: waves 2, 3 hold the keys of waves 0,
+// 1 again and take rows 32-63 of each tile, their sums are added at the end.
+template <bool CAUSAL, int KW>
 __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
   // two buffers of Q tile, dO tile, 64 nlse, 64 ndelta
   constexpr int kBuf = 2 * kTileBytes + 512;
   __shared__ __attribute__((aligned(16))) uint8_t smem[2 * kBuf];
   const int lane = threadIdx.x & 63, hh = lane >> 5, lr = lane & 31;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kh = wid & 1, qh = wid >> 1;
+  const int kh = KW == 4 ? wid : wid & 1, qh = KW == 4 ? 0 : wid >> 1;
   const int hk = blockIdx.x % a.Hk;
+  int rest = blockIdx.x / a.Hk;
+  const int split = rest % a.nsplit;
+  rest /= a.nsplit;
   int tile;
-  const int b = find_tile(a.cu_k, a.Tk, 1, kKeys, a.B + a.zero_tail, blockIdx.x / a.Hk, lane, tile);
+  const int b = find_tile(a.cu_k, a.Tk, 1, 32 * KW, a.B + a.zero_tail, rest, lane, tile);
   if (b == a.B) {
     const int t0 = cu_at(a.cu_k, a.B, a.Tk);
-    for (int e = threadIdx.x; e < kKeys * 8; e += 256) {
-      const int64_t t = t0 + tile * kKeys + (e >> 3);
+    for (int e = threadIdx.x; a.nsplit == 1 && e < 32 * KW * 8; e += 256) {
+      const int64_t t = t0 + tile * 32 * KW + (e >> 3);
       if (t >= a.Tk) break;
       *reinterpret_cast<uint4*>(a.dk + t * a.dk_t + hk * a.dk_h + (e & 7) * 8) = make_uint4(0, 0, 0, 0);
       *reinterpret_cast<uint4*>(a.dv + t * a.dv_t + hk * a.dv_h + (e & 7) * 8) = make_uint4(0, 0, 0, 0);
@@ -775,28 +852,51 @@ __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
     return;
   }
   const Seq s = sequence(a, b);
-  const int key0 = tile * kKeys;
+  const int key0 = tile * 32 * KW;
   if (key0 >= s.lk) return;
   const int kw = key0 + 32 * kh;                       // the wave's first key
   const int key = kw + lr, kc = min(key, s.lk - 1);
   // causal: key j is seen by the queries from j - (lk - lq) on
   const int off = s.lk - s.lq;
   const int i_first = CAUSAL ? max(0, key0 - off) : 0;
-  const int tiles = s.lq > i_first ? (s.lq - i_first + 63) / 64 : 0, total = tiles * a.G;
+  const int g0 = a.nsplit == 1 ? 0 : split, g1 = a.nsplit == 1 ? a.G : split + 1;
+  const bool any = i_first < s.lq;
 
   const Stage stq(wid, lane, a.q_t), std_(wid, lane, a.d_t);
-  auto stage = [&](int buf, int n) {
-    const int g = n / tiles, h = hk * a.G + g, i = i_first + (n - g * tiles) * 64;
-    uint8_t* base = smem + buf * kBuf;
-    stq.load(rows_rsrc(a.q + ((s.q0 + i) * a.q_t + h * a.q_h), a.q_t, s.lq - i), base, wid);
-    std_.load(rows_rsrc(a.dout + ((s.q0 + i) * a.d_t + h * a.d_h), a.d_t, s.lq - i), base + kTileBytes, wid);
+  const bf16_t* Q0 = a.q + ((s.q0 + i_first) * a.q_t + (hk * a.G + g0) * a.q_h);
+  const bf16_t* D0 = a.dout + ((s.q0 + i_first) * a.d_t + (hk * a.G + g0) * a.d_h);
+  // waves 0 and 1 also load the tile's nlse and ndelta
+  const float* S0 = (wid ? a.ndelta : a.nlse) + (int64_t)(hk * a.G + g0) * a.Tq + s.q0 + i_first;
+  const float* S = S0;
+  Src srcq(Q0, a.q_t, s.lq - i_first), srcd(D0, a.d_t, s.lq - i_first);
+  const int64_t stepq = a.q_t * 128, stepd = a.d_t * 128;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem)) + wid * 2048;
+  const uint32_t ldss = lds0 - wid * 2048 + 2 * kTileBytes + wid * 256;
+  int next_i = i_first, next_g = g0;                   // the tile that is loaded next
+  auto stage = [&](int buf) {
+    stq.load(srcq.rsrc(), lds0 + buf * kBuf);
+    std_.load(srcd.rsrc(), lds0 + buf * kBuf + kTileBytes);
     if (wid < 2) {
-      const float* st = (wid ? a.ndelta : a.nlse) + (int64_t)h * a.Tq + s.q0 + i;
-      const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(st), 0, min(s.lq - i, 64) * 4, 0x00020000);
-      dma4(rs, __builtin_amdgcn_readfirstlane(lds_addr(base + 2 * kTileBytes + wid * 256)), lane * 4);
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(S), 0, min(s.lq - next_i, 64) * 4, 0x00020000);
+      dma4(rs, ldss + buf * kBuf, lane * 4);
+    }
+    next_i += 64;
+    if (next_i < s.lq) {
+      srcq.move(stepq);
+      srcd.move(stepd);
+      S += 64;
+    } else {                                           // the next query head
+      next_i = i_first;
+      ++next_g;
+      Q0 += a.q_h;
+      D0 += a.d_h;
+      S0 += a.Tq;
+      srcq = Src(Q0, a.q_t, s.lq - i_first);
+      srcd = Src(D0, a.d_t, s.lq - i_first);
+      S = S0;
     }
   };
-  if (total > 0) stage(0, 0);
+  if (any) stage(0);
   bf16x8 kf[4], vf[4];
   {
     const bf16_t* kr = a.k + (s.k0 + kc) * a.k_t + hk * a.k_h;
@@ -814,73 +914,72 @@ __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
   f32x16 dk[2], dv[2];
   for (int i = 0; i < 16; ++i) dk[0][i] = dk[1][i] = dv[0][i] = dv[1][i] = 0.f;
 
-  int bad = 0;
-  for (int n = 0, cur = 0; n < total; ++n, cur ^= 1) {
-    if (n + 1 < total) stage(cur ^ 1, n + 1);
-    const uint8_t* sQ = smem + cur * kBuf;
-    const uint8_t* sD = sQ + kTileBytes;
-    const float* stat = reinterpret_cast<const float*>(sQ + 2 * kTileBytes);
-    const int i0 = i_first + n % tiles * 64 + 32 * qh;      // the wave's first query
-    // some query of the block exists and sees some key of the wave
-    const bool on = i0 < s.lq && (!CAUSAL || i0 + 31 >= kw - off);
-    if (on) {
-      f32x16 st, dp;
+  int bad = 0, cur = 0;
+  for (int g = g0; any && g < g1; ++g)
+    for (int i1 = i_first; i1 < s.lq; i1 += 64, cur ^= 1) {
+      if (next_g < g1) stage(cur ^ 1);
+      const uint8_t* sQ = smem + cur * kBuf;
+      const uint8_t* sD = sQ + kTileBytes;
+      const float* stat = reinterpret_cast<const float*>(sQ + 2 * kTileBytes);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const float4 x = *reinterpret_cast<const float4*>(stat + 32 * qh + 8 * g + 4 * hh);
-        const float4 y = *reinterpret_cast<const float4*>(stat + 64 + 32 * qh + 8 * g + 4 * hh);
-        st[4 * g] = x.x, st[4 * g + 1] = x.y, st[4 * g + 2] = x.z, st[4 * g + 3] = x.w;
-        dp[4 * g] = y.x, dp[4 * g + 1] = y.y, dp[4 * g + 2] = y.z, dp[4 * g + 3] = y.w;
-      }
+      for (int u = 0; u < KW / 2; ++u) {
+        const int rb = 32 * (u + qh), i0 = i1 + rb;            // the block's first row in the tile, its first query
+        // some query of the block exists and sees some key of the wave
+        if (i0 < s.lq && (!CAUSAL || i0 + 31 >= kw - off)) {
+          f32x16 st, dp;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        st = mfma(row_frag(sQ, 32 * qh + lr, t, hh), kf[t], st);
-        dp = mfma(row_frag(sD, 32 * qh + lr, t, hh), vf[t], dp);
-      }
-      const bool partial = CAUSAL && i0 < kw + 31 - off;     // uniform
-      const int first = key - off - i0;                      // the block's rows below this do not see the lane's key
+          for (int q = 0; q < 4; ++q) {
+            const float4 x = *reinterpret_cast<const float4*>(stat + rb + 8 * q + 4 * hh);
+            const float4 y = *reinterpret_cast<const float4*>(stat + 64 + rb + 8 * q + 4 * hh);
+            st[4 * q] = x.x, st[4 * q + 1] = x.y, st[4 * q + 2] = x.z, st[4 * q + 3] = x.w;
+            dp[4 * q] = y.x, dp[4 * q + 1] = y.y, dp[4 * q + 2] = y.z, dp[4 * q + 3] = y.w;
+          }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        st[i] = __builtin_amdgcn_exp2f(st[i] * c);
-        dp[i] *= st[i];
-      }
-      if (partial) {
+          for (int t = 0; t < 4; ++t) {
+            st = mfma(row_frag(sQ, rb + lr, t, hh), kf[t], st);
+            dp = mfma(row_frag(sD, rb + lr, t, hh), vf[t], dp);
+          }
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if ((i & 3) + 8 * (i >> 2) + 4 * hh < first) st[i] = dp[i] = 0.f;
-      }
-      uint32_t pk[8], dsk[8];
+          for (int i = 0; i < 16; ++i) {
+            st[i] = __builtin_amdgcn_exp2f(st[i] * c);
+            dp[i] *= st[i];
+          }
+          if (CAUSAL && i0 < kw + 31 - off) {                  // some query of the block does not see some key of the wave
+            const int lim = key - off - i0 - 4 * hh;           // the rows below this do not see the lane's key
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        pk[i >> 1] = pack_bf16(st[i], st[i + 1]);
-        dsk[i >> 1] = pack_bf16(dp[i], dp[i + 1]);
-      }
-      if (partial) {
+            for (int i = 0; i < 16; ++i) {
+              const bool on = (i & 3) + 8 * (i >> 2) >= lim;
+              st[i] = on ? st[i] : 0.f;
+              dp[i] = on ? dp[i] : 0.f;
+            }
+            bad |= has_nonfinite(sQ, rb, lane) | has_nonfinite(sD, rb, lane);
+          }
+          uint32_t pk[8], dsk[8];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+          for (int i = 0; i < 16; i += 2) {
+            pk[i >> 1] = pack_bf16(st[i], st[i + 1]);
+            dsk[i >> 1] = pack_bf16(dp[i], dp[i + 1]);
+          }
 #pragma unroll
-          for (int dt = 0; dt < 2; ++dt)
-            bad |= (int)nonfinite(tr_frag(sD, 32 * qh + 16 * t, dt, lane)) + (int)nonfinite(tr_frag(sQ, 32 * qh + 16 * t, dt, lane));
-      }
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int dt = 0; dt < 2; ++dt) {
-          dv[dt] = mfma(tr_frag(sD, 32 * qh + 16 * t, dt, lane), p_frag(pk, t), dv[dt]);
-          dk[dt] = mfma(tr_frag(sQ, 32 * qh + 16 * t, dt, lane), p_frag(dsk, t), dk[dt]);
+            for (int dt = 0; dt < 2; ++dt) {
+              dv[dt] = mfma(tr_frag(sD, rb + 16 * t, dt, lane), p_frag(pk, t), dv[dt]);
+              dk[dt] = mfma(tr_frag(sQ, rb + 16 * t, dt, lane), p_frag(dsk, t), dk[dt]);
+            }
         }
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-  }
   if (CAUSAL && __ballot(bad) != 0) {
     for (int i = 0; i < 16; ++i) dk[0][i] = dk[1][i] = dv[0][i] = dv[1][i] = 0.f;
     const Args& w = again();
-    for (int g = 0; g < w.G; ++g) {
+    for (int g = g0; g < g1; ++g) {
       const int h = hk * w.G + g;
 #pragma clang loop unroll(disable)
       for (int i = i_first; i < s.lq; ++i) {
-        if (((i - i_first) >> 5 & 1) != qh) continue;         // the other waves' rows
+        if (KW == 2 && ((i - i_first) >> 5 & 1) != qh) continue;      // the other waves' rows
         const bf16_t* qr = w.q + (s.q0 + i) * w.q_t + h * w.q_h;
         const bf16_t* dr = w.dout + (s.q0 + i) * w.d_t + h * w.d_h;
         const float x = dot_row(qr, kf, hh), y = dot_row(dr, vf, hh);
@@ -893,53 +992,101 @@ __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
       }
     }
   }
-  // the two row halves' sums: 64 floats x 64 lanes of waves 2, 3 through LDS (32 KiB, the buffers' own)
-  float* x = reinterpret_cast<float*>(smem) + kh * 64 * 64;
-  if (qh == 1) {
+  if constexpr (KW == 2) {
+    // the two row halves' sums: 64 floats x 64 lanes of waves 2, 3 through LDS (32 KiB, the buffers' own)
+    float* x = reinterpret_cast<float*>(smem) + kh * 64 * 64 + lane;
+    if (qh == 1) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x[i * 64] = dk[0][i];
+        x[(16 + i) * 64] = dk[1][i];
+        x[(32 + i) * 64] = dv[0][i];
+        x[(48 + i) * 64] = dv[1][i];
+      }
+    }
+    __syncthreads();
+    if (qh == 1) return;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      x[i * 64 + lane] = dk[0][i];
-      x[(16 + i) * 64 + lane] = dk[1][i];
-      x[(32 + i) * 64 + lane] = dv[0][i];
-      x[(48 + i) * 64 + lane] = dv[1][i];
+      dk[0][i] += x[i * 64];
+      dk[1][i] += x[(16 + i) * 64];
+      dv[0][i] += x[(32 + i) * 64];
+      dv[1][i] += x[(48 + i) * 64];
     }
   }
-  __syncthreads();
-  if (qh == 1 || key >= s.lk) return;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    dk[0][i] += x[i * 64 + lane];
-    dk[1][i] += x[(16 + i) * 64 + lane];
-    dv[0][i] += x[(32 + i) * 64 + lane];
-    dv[1][i] += x[(48 + i) * 64 + lane];
+  if (key >= s.lk) return;
+  if (a.nsplit == 1) {
+    store_acc(a.dk + (s.k0 + key) * a.dk_t + hk * a.dk_h, dk, a.scale, hh);
+    store_acc(a.dv + (s.k0 + key) * a.dv_t + hk * a.dv_h, dv, 1.0f, hh);
+    return;
   }
-  store_acc(a.dk + (s.k0 + key) * a.dk_t + hk * a.dk_h, dk, a.scale, hh);
-  store_acc(a.dv + (s.k0 + key) * a.dv_t + hk * a.dv_h, dv, 1.0f, hh);
+  float* pk = a.part_o + (((int64_t)split * a.Tk + s.k0 + key) * a.Hk + hk) * 128;       // 64 of dK, 64 of dV
+#pragma unroll
+  for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * dt + 8 * g + 4 * hh;
+      *reinterpret_cast<float4*>(pk + d) = make_float4(dk[dt][4 * g], dk[dt][4 * g + 1], dk[dt][4 * g + 2], dk[dt][4 * g + 3]);
+      *reinterpret_cast<float4*>(pk + 64 + d) = make_float4(dv[dt][4 * g], dv[dt][4 * g + 1], dv[dt][4 * g + 2], dv[dt][4 * g + 3]);
+    }
+}
+
+// The query heads' partial sums of dK and dV added, in their order: 32 lanes a key row, four values each.
+__global__ __launch_bounds__(256) void k_attnp_sum(const Args a) {
+  const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = (int64_t)a.Tk * a.Hk;
+  if (n >= rows) return;
+  const int64_t t = n / a.Hk;
+  const int hk = (int)(n - t * a.Hk), e = threadIdx.x & 31;
+  const bool tail = t >= cu_at(a.cu_k, a.B, a.Tk);
+  if (tail && !a.zero_tail) return;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int g = 0; !tail && g < a.nsplit; ++g) {
+    const float4 x = *reinterpret_cast<const float4*>(a.part_o + (g * rows + n) * 128 + 4 * e);
+    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+  }
+  const float f = e < 16 ? a.scale : 1.0f;
+  bf16_t* out = e < 16 ? a.dk + t * a.dk_t + hk * a.dk_h + 4 * e : a.dv + t * a.dv_t + hk * a.dv_h + 4 * (e - 16);
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
 }
 
 // ------------------------------------------------------------------ host side
-inline int64_t row_tiles(const i2pc_attn_packed_desc& d) {
-  return (int64_t)d.total_q * (d.heads / d.kv_heads) / kRows + d.batch + (d.zero_tail ? 1 : 0);
+inline int64_t row_tiles(const i2pc_attn_packed_desc& d, int rows) {
+  return (int64_t)d.total_q * (d.heads / d.kv_heads) / rows + d.batch + (d.zero_tail ? 1 : 0);
 }
+// Waves over the keys of a tile (the kernels' KW): two while 128-row workgroups would not fill the chip's 768 places twice.
+// Measured forward, KW 1 / 2: 7200 tokens of six heads (372 workgroups) 38 / 32 us, 8700 causal rows of 16 heads over 4
+// (1000) 80 / 71 us, 12000 of twelve heads (1250) 65 / 67 us, 32 x 577 of 16 heads (2800) 75 / 95 us.
+inline int key_waves(const i2pc_attn_packed_desc& d) { return row_tiles(d, kRows) * d.kv_heads < 1200 ? 2 : 1; }
 
 // Sequences of 32 packed rows or fewer on average take the kernel for few rows.  (Right for any lengths: the rule only
 // decides the speed.)
 inline bool few_rows(const i2pc_attn_packed_desc& d) {
   return (int64_t)d.total_q * (d.heads / d.kv_heads) <= (int64_t)d.batch * kFew;
 }
-inline int64_t few_tiles(const i2pc_attn_packed_desc& d) {
-  return (int64_t)d.total_q * (d.heads / d.kv_heads) / kFew + d.batch + (d.zero_tail ? 1 : 0);
-}
 
 // Shares of the keys: one where the row tiles fill the chip, else so many that they do, of 256 keys at least (an
 // upper bound: a share may be empty).
 inline int splits(const i2pc_attn_packed_desc& d) {
   if (d.total_k == 0) return 1;
-  const int64_t tiles = (few_rows(d) ? few_tiles(d) : row_tiles(d)) * d.kv_heads;
-  const int64_t most = (d.total_k + 255) / 256;
-  static const int target = [] { const char* e = getenv("I2PC_FEW"); return e ? atoi(e) : 1024; }();
-  const int64_t want = few_rows(d) ? target / tiles : tiles >= 512 ? 1 : (1024 + tiles - 1) / tiles;
+  const bool few = few_rows(d);
+  const int64_t tiles = row_tiles(d, few ? kFew : kRows / 2) * d.kv_heads;
+  const int64_t most = few ? (d.total_k + 1023) / 1024 : (d.total_k + 255) / 256;
+  const int64_t want = few ? 2048 / tiles : key_waves(d) == 1 || tiles >= 512 ? 1 : 1024 / tiles;
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 512}));
+}
+
+// The dK / dV call: keys of a workgroup / 32, and whether each query head of a group has workgroups of its own.
+struct KeySplit {
+  int kw, heads;
+};
+inline int64_t key_tiles(const i2pc_attn_packed_desc& d, int keys) {
+  return (int64_t)d.total_k / keys + d.batch + (d.zero_tail ? 1 : 0);
+}
+inline KeySplit key_split(const i2pc_attn_packed_desc& d) {
+  const int G = d.heads / d.kv_heads;
+  const int64_t wide = key_tiles(d, 128) * d.kv_heads;
+  const int heads = wide < 4096 ? G : 1;
+  return {wide * heads < 768 ? 2 : 4, heads};
 }
 
 // Rows apart (the range checks of the tiles' loads go by the row stride), heads apart too where they are written.
@@ -958,7 +1105,7 @@ int check(const char* what, const i2pc_attn_packed_desc* d) {
   // grids of 256-thread workgroups hold 2^24 of them
   const int64_t most = (int64_t)1 << 24;
   if ((int64_t)d->total_q * d->heads >= most * 32 || ((int64_t)d->total_q / kRows + 2 * (int64_t)d->batch + 2) * d->heads >= most ||
-      ((int64_t)d->total_k / kKeys + (int64_t)d->batch + 1) * d->kv_heads >= most)
+      ((int64_t)d->total_k / 64 + (int64_t)d->batch + 1) * d->kv_heads >= most)
     return set_error(I2PC_EUNSUPPORTED, "%s: total_q * heads must stay below 2^29, (total_k / 64 + batch) * kv_heads below 2^24", what);
   I2PC_REQUIRE(std::isfinite(d->scale) && d->scale > 0.f, "%s: scale=%g must be finite and above zero", what, (double)d->scale);
   I2PC_REQUIRE(d->batch == 0 || (d->cu_q && d->cu_k), "%s: NULL cu_q or cu_k", what);
@@ -1009,17 +1156,20 @@ extern "C" int i2pc_attention_packed(const i2pc_attn_packed_desc* d, void* works
   hipStream_t s = as_stream(stream);
   a.nsplit = attnp::splits(*d);
   const bool few = attnp::few_rows(*d);
-  const dim3 block(256), grid((uint32_t)((few ? attnp::few_tiles(*d) : attnp::row_tiles(*d)) * a.Hk * a.nsplit));
+  const int kw = attnp::key_waves(*d);
+  const dim3 block(256), grid((uint32_t)(attnp::row_tiles(*d, few ? attnp::kFew : attnp::kRows / kw) * a.Hk * a.nsplit));
   if (a.nsplit > 1) {
     a.part_o = static_cast<float*>(workspace);
     a.part_l = a.part_o + (size_t)a.nsplit * a.H * a.Tq * 64;
   }
   if (few && d->causal) hipLaunchKernelGGL(attnp::k_attnp_few<true>, grid, block, 0, s, a);
   else if (few) hipLaunchKernelGGL(attnp::k_attnp_few<false>, grid, block, 0, s, a);
-  else if (a.nsplit == 1 && d->causal) hipLaunchKernelGGL((attnp::k_attnp_fwd<true, false>), grid, block, 0, s, a);
-  else if (a.nsplit == 1) hipLaunchKernelGGL((attnp::k_attnp_fwd<false, false>), grid, block, 0, s, a);
-  else if (d->causal) hipLaunchKernelGGL((attnp::k_attnp_fwd<true, true>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((attnp::k_attnp_fwd<false, true>), grid, block, 0, s, a);
+  else if (kw == 1 && d->causal) hipLaunchKernelGGL((attnp::k_attnp_fwd<true, false, 1>), grid, block, 0, s, a);
+  else if (kw == 1) hipLaunchKernelGGL((attnp::k_attnp_fwd<false, false, 1>), grid, block, 0, s, a);
+  else if (a.nsplit == 1 && d->causal) hipLaunchKernelGGL((attnp::k_attnp_fwd<true, false, 2>), grid, block, 0, s, a);
+  else if (a.nsplit == 1) hipLaunchKernelGGL((attnp::k_attnp_fwd<false, false, 2>), grid, block, 0, s, a);
+  else if (d->causal) hipLaunchKernelGGL((attnp::k_attnp_fwd<true, true, 2>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((attnp::k_attnp_fwd<false, true, 2>), grid, block, 0, s, a);
   const int64_t rows = (int64_t)a.Tq * a.H;
   if (a.nsplit > 32)
     hipLaunchKernelGGL(attnp::k_attnp_join<16>, dim3((uint32_t)rows), dim3(1024), 0, s, a);
@@ -1045,7 +1195,10 @@ static int check_grad(const i2pc_attn_packed_grad_desc* g) {
 
 extern "C" size_t i2pc_attention_packed_backward_workspace_bytes(const i2pc_attn_packed_grad_desc* g) {
   if (check_grad(g) != I2PC_OK) return 0;
-  return (size_t)2 * g->f.total_q * g->f.heads * sizeof(float);
+  // -lse / scale and -D of every row, and the query heads' partial sums where they are split
+  const attnp::KeySplit k = attnp::key_split(g->f);
+  return ((size_t)2 * g->f.total_q * g->f.heads + 3) / 4 * 4 * sizeof(float) +
+         (k.heads == 1 ? 0 : (size_t)k.heads * g->f.total_k * g->f.kv_heads * 128 * sizeof(float));
 }
 
 extern "C" int i2pc_attention_packed_backward(const i2pc_attn_packed_grad_desc* g, void* workspace, size_t workspace_bytes,
@@ -1071,14 +1224,24 @@ extern "C" int i2pc_attention_packed_backward(const i2pc_attn_packed_grad_desc* 
   const dim3 block(256);
   if (a.Tq > 0) {
     hipLaunchKernelGGL(attnp::k_attnp_delta, dim3((uint32_t)(((int64_t)a.Tq * a.H + 31) / 32)), block, 0, s, a);
-    const dim3 grid((uint32_t)(attnp::row_tiles(d) * a.Hk));
-    if (d.causal) hipLaunchKernelGGL(attnp::k_attnp_dq<true>, grid, block, 0, s, a);
-    else hipLaunchKernelGGL(attnp::k_attnp_dq<false>, grid, block, 0, s, a);
+    const int kw = attnp::key_waves(d);
+    const dim3 grid((uint32_t)(attnp::row_tiles(d, attnp::kRows / kw) * a.Hk));
+    if (kw == 1 && d.causal) hipLaunchKernelGGL((attnp::k_attnp_dq<true, 1>), grid, block, 0, s, a);
+    else if (kw == 1) hipLaunchKernelGGL((attnp::k_attnp_dq<false, 1>), grid, block, 0, s, a);
+    else if (d.causal) hipLaunchKernelGGL((attnp::k_attnp_dq<true, 2>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((attnp::k_attnp_dq<false, 2>), grid, block, 0, s, a);
   }
   if (a.Tk > 0) {
-    const dim3 grid((uint32_t)(((int64_t)a.Tk / attnp::kKeys + a.B + a.zero_tail) * a.Hk));
-    if (d.causal) hipLaunchKernelGGL(attnp::k_attnp_dkdv<true>, grid, block, 0, s, a);
-    else hipLaunchKernelGGL(attnp::k_attnp_dkdv<false>, grid, block, 0, s, a);
+    const attnp::KeySplit k = attnp::key_split(d);
+    a.nsplit = k.heads;
+    a.part_o = a.nlse + ((size_t)2 * a.Tq * a.H + 3) / 4 * 4;
+    const dim3 grid((uint32_t)(attnp::key_tiles(d, 32 * k.kw) * a.Hk * a.nsplit));
+    if (k.kw == 4 && d.causal) hipLaunchKernelGGL((attnp::k_attnp_dkdv<true, 4>), grid, block, 0, s, a);
+    else if (k.kw == 4) hipLaunchKernelGGL((attnp::k_attnp_dkdv<false, 4>), grid, block, 0, s, a);
+    else if (d.causal) hipLaunchKernelGGL((attnp::k_attnp_dkdv<true, 2>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((attnp::k_attnp_dkdv<false, 2>), grid, block, 0, s, a);
+    if (a.nsplit > 1)
+      hipLaunchKernelGGL(attnp::k_attnp_sum, dim3((uint32_t)(((int64_t)a.Tk * a.Hk + 7) / 8)), block, 0, s, a);
   }
   return check_launch("attention_packed_backward");
 }

@@ -13,35 +13,35 @@
 namespace i2pc {
 namespace gelu8 {
 
-// Phi(x) and exp(-x^2 / 2) for finite x; erfc by Abramowitz & Stegun 7.1.26, which needs that exponential
-// anyway.  The approximation is of the tail, so Phi keeps its size for negative x: |error| <= 0.75e-7.
-__device__ __forceinline__ void normal_cdf(float x, float& cdf, float& ex) {
-  const float z = fabsf(x) * 0.70710678118654752f;
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
-  ex = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);           // exp(-x^2 / 2)
-  float p = fmaf(t, 1.061405429f, -1.453152027f);
-  p = fmaf(t, p, 1.421413741f);
-  p = fmaf(t, p, -0.284496736f);
-  p = fmaf(t, p, 0.254829592f);
-  const float tail = 0.5f * p * t * ex;                                  // Phi(-|x|)
-  cdf = x < 0.f ? tail : 1.0f - tail;
+// Phi(-|x|) and exp(-x^2 / 2): erfc by Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7, halved here), which needs that
+// exponential anyway.  Its constants are scaled by sqrt(1/2) and 1/2.
+__device__ __forceinline__ float normal_tail(float x, float& ex) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.23164188f, fabsf(x), 1.0f));
+  ex = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);
+  float p = fmaf(t, 0.5307027145f, -0.7265760135f);
+  p = fmaf(t, p, 0.7107068705f);
+  p = fmaf(t, p, -0.142248368f);
+  p = fmaf(t, p, 0.127414796f);
+  return p * t * ex;
 }
-__device__ __forceinline__ float gelu(float x) {
-  float c, e;
-  normal_cdf(x, c, e);
-  // x Phi(x) at the ends: +inf -> +inf, -inf -> 0 (not inf * 0); NaN stays
-  return x == -INFINITY ? 0.f : x * c;
+// GELU(x) = max(x, 0) - |x| Phi(-|x|).  ENDS: +-inf may come in (inf * 0 otherwise).  NaN stays NaN in both forms.
+template <bool ENDS>
+__device__ __forceinline__ float gelu(float x, float tail) {
+  const float y = fmaf(-fabsf(x), tail, fmaxf(x, 0.f));
+  return ENDS && fabsf(x) == INFINITY ? fmaxf(x, 0.f) : y;
 }
-__device__ __forceinline__ float gelu_slope(float x, float& act) {
-  float c, e;
-  normal_cdf(x, c, e);
-  const bool inf = fabsf(x) == INFINITY;
-  act = x == -INFINITY ? 0.f : x * c;
-  return inf ? c : fmaf(x * 0.39894228040143268f, e, c);
+// Phi(x) + x phi(x)
+template <bool ENDS>
+__device__ __forceinline__ float gelu_slope(float x, float tail, float ex) {
+  const float c = 0.5f + __builtin_copysignf(0.5f - tail, x);
+  return ENDS && fabsf(x) == INFINITY ? c : fmaf(x * 0.39894228040143268f, ex, c);
 }
 
-// float -> e4m3 pairs; NaN stays NaN (the clamp is for +-inf, which only blocks of scale 2^127 hold)
-__device__ __forceinline__ float clamp448(float v) { return v != v ? v : fminf(fmaxf(v, -448.f), 448.f); }
+// x / 2^e within e4m3's range, which only infinities of a block of scale 2^127 leave
+template <bool ENDS>
+__device__ __forceinline__ float within(float v) {
+  return !ENDS || v != v ? v : fminf(fmaxf(v, -448.f), 448.f);
+}
 
 __device__ __forceinline__ float lo16(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi16(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
@@ -70,8 +70,20 @@ __global__ __launch_bounds__(256) void k_gelu_keep(const uint16_t* __restrict__ 
   float q[8], g[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    q[j] = clamp448(v[j] * mul);
-    g[j] = gelu(v[j]);
+    float ex;
+    const float tail = normal_tail(v[j], ex);
+    q[j] = within<false>(v[j] * mul);
+    g[j] = gelu<false>(v[j], tail);
+  }
+  if (__builtin_expect(am == INFINITY, 0)) {
+    asm volatile("");                                  // a branch, not selects: hardly ever taken
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float ex;
+      const float tail = normal_tail(v[j], ex);
+      q[j] = within<true>(v[j] * mul);
+      g[j] = gelu<true>(v[j], tail);
+    }
   }
   int d0 = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false), d1 = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
   d0 = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], d0, true);
@@ -91,16 +103,32 @@ __global__ __launch_bounds__(256) void k_gelu_back(const uint16_t* __restrict__ 
   if (c >= chunks) return;
   const uint4 w = *reinterpret_cast<const uint4*>(dy + at(c, per_row, lddy));
   const int2 k = *reinterpret_cast<const int2*>(kept + (int64_t)c * 8);
-  const float mul = mx::exp2i((int)scale[c >> 2] - 127);
+  const int e = scale[c >> 2];
+  const float mul = mx::exp2i(e - 127);
   const float d[8] = {lo16(w.x), hi16(w.x), lo16(w.y), hi16(w.y), lo16(w.z), hi16(w.z), lo16(w.w), hi16(w.w)};
-  float g[8], a[8];
+  float x[8], g[8], a[8];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int word = h ? k.y : k.x;
     const auto p0 = __builtin_amdgcn_cvt_pk_f32_fp8(word, false), p1 = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);
-    const float q[4] = {p0[0], p0[1], p1[0], p1[1]};
+    x[4 * h] = p0[0] * mul, x[4 * h + 1] = p0[1] * mul, x[4 * h + 2] = p1[0] * mul, x[4 * h + 3] = p1[1] * mul;
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) g[4 * h + j] = d[4 * h + j] * gelu_slope(q[j] * mul, a[4 * h + j]);
+  for (int j = 0; j < 8; ++j) {
+    float ex;
+    const float tail = normal_tail(x[j], ex);
+    a[j] = gelu<false>(x[j], tail);
+    g[j] = d[j] * gelu_slope<false>(x[j], tail, ex);
+  }
+  if (__builtin_expect(e >= 127 + 120, 0)) {           // 448 * 2^120 is above the largest float
+    asm volatile("");                                  // a branch, not selects
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float ex;
+      const float tail = normal_tail(x[j], ex);
+      a[j] = gelu<true>(x[j], tail);
+      g[j] = d[j] * gelu_slope<true>(x[j], tail, ex);
+    }
   }
   *reinterpret_cast<uint4*>(dx + at(c, per_row, lddx)) =
       make_uint4(pk2bf(g[0], g[1]), pk2bf(g[2], g[3]), pk2bf(g[4], g[5]), pk2bf(g[6], g[7]));

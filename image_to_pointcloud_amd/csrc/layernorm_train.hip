@@ -59,6 +59,24 @@ struct Vec<bf16_t, E> {
   }
 };
 
+// E bf16 values as they are in memory, widened where they are used: half the registers of their floats.
+template <int E>
+struct Packed {
+  uint32_t w[(E + 1) / 2];
+  __device__ __forceinline__ void load(const bf16_t* p) {
+    if constexpr (E == 1) w[0] = *p;
+    else __builtin_memcpy(w, p, E * 2);
+  }
+  // to be widened anew: the floats are not kept from one use to the next
+  __device__ __forceinline__ void renew() {
+#pragma unroll
+    for (int j = 0; j < (E + 1) / 2; ++j) asm volatile("" : "+v"(w[j]));
+  }
+  __device__ __forceinline__ float operator[](int j) const {
+    return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+  }
+};
+
 // A row's columns over WPR waves: chunk i of a lane starts at column (i * 64 * WPR + wave * 64 + lane) * E.
 // The last chunk of a row whose width is no multiple of E starts at dim - E instead and repeats columns of
 // the chunk before it: every load is a whole vector, `live` keeps the repeated columns out of the row
@@ -100,7 +118,7 @@ __global__ __launch_bounds__(WPR == 8 ? 512 : 256) void k_lnt_fwd(const T* __res
                                                  const float* __restrict__ beta, float eps, int rows, int dim,
                                                  bf16_t* __restrict__ y, int64_t ldy, float2* __restrict__ stats) {
   __shared__ float red[8];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // scalar row addresses
   const Cols<E, V, WPR> c(lane, wave % WPR, dim);
   constexpr int R = WPR == 1 ? 4 : 1;              // WPR > 1: one row a workgroup, all its waves or none
   for (int64_t row = (int64_t)blockIdx.x * R + (WPR == 1 ? wave : 0); row < rows; row += (int64_t)gridDim.x * R) {
@@ -140,14 +158,14 @@ __global__ __launch_bounds__(WPR == 8 ? 512 : 256) void k_lnt_fwd(const T* __res
 // Rows blockIdx.x * R + k * gridDim.x * R for the R = 8 / WPR rows a workgroup takes at a time.  Partial row p of the
 // column sums goes to dgamma + p * 2 * dim and dbeta + p * 2 * dim: with one partial row, the outputs themselves.
 template <typename T, int E, int V, int WPR>
-__global__ __launch_bounds__(kThreads) void k_lnt_bwd(const bf16_t* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
+__global__ __launch_bounds__(kThreads, 4) void k_lnt_bwd(const bf16_t* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
                                                       int64_t ldx, const float2* __restrict__ stats,
                                                       const float* __restrict__ gamma, const T* add, int64_t lda, int rows,
                                                       int dim, T* dx, int64_t lddx, float* __restrict__ dgamma,
                                                       float* __restrict__ dbeta) {
   __shared__ float red[8];
-  extern __shared__ float sums[];                  // [2][dim], rows of one wave only
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  extern __shared__ float sums[];                  // [2][dim] (R > 1)
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // scalar row addresses
   constexpr int R = 8 / WPR;
   const Cols<E, V, WPR> c(lane, wave % WPR, dim);
   float g[V][E], dg[V][E], db[V][E];
@@ -164,11 +182,12 @@ __global__ __launch_bounds__(kThreads) void k_lnt_bwd(const bf16_t* __restrict__
     const bool on = row < rows;
     if (WPR == 1 && !on) break;
     const int64_t rc = on ? row : rows - 1;
-    float xv[V][E], gy[V][E], av[V][E];
+    float xv[V][E], av[V][E];
+    Packed<E> gy[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       Vec<T, E>::load(x + rc * ldx + c.col[i], xv[i]);
-      Vec<bf16_t, E>::load(dy + rc * lddy + c.col[i], gy[i]);
+      gy[i].load(dy + rc * lddy + c.col[i]);
     }
     if (add) {
 #pragma unroll
@@ -182,7 +201,6 @@ __global__ __launch_bounds__(kThreads) void k_lnt_bwd(const bf16_t* __restrict__
       for (int j = 0; j < E; ++j) {
         const float h = (xv[i][j] - st.x) * st.y, d = gy[i][j], gd = d * g[i][j];
         xv[i][j] = h;
-        gy[i][j] = gd;
         a += c.live(i, j) ? gd : 0.f;
         b += c.live(i, j) ? gd * h : 0.f;
         if (WPR == 1 || on) {
@@ -196,17 +214,18 @@ __global__ __launch_bounds__(kThreads) void k_lnt_bwd(const bf16_t* __restrict__
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         float o[E];
+        gy[i].renew();
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          o[j] = st.y * (gy[i][j] - a - xv[i][j] * b);
+          o[j] = st.y * (gy[i][j] * g[i][j] - a - xv[i][j] * b);
           if (add) o[j] += av[i][j];
         }
         if (c.first[i] < (uint32_t)E) Vec<T, E>::store(dx + row * lddx + c.col[i], o);
       }
     }
   }
-  if constexpr (WPR > 1) {                         // wide rows: a partial row for each row group
-    const int64_t p = (int64_t)(blockIdx.x * R + wave / WPR) * 2 * dim;
+  const int64_t p = (int64_t)blockIdx.x * 2 * dim;
+  if constexpr (R == 1) {
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (c.first[i] < (uint32_t)E) {
@@ -216,7 +235,7 @@ __global__ __launch_bounds__(kThreads) void k_lnt_bwd(const bf16_t* __restrict__
   } else {                                         // the row groups' column sums, one after the other
     for (int w = 0; w < R; ++w) {
       __syncthreads();
-      if (wave == w) {
+      if (wave / WPR == w) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
 #pragma unroll
@@ -229,7 +248,6 @@ __global__ __launch_bounds__(kThreads) void k_lnt_bwd(const bf16_t* __restrict__
       }
     }
     __syncthreads();
-    const int64_t p = (int64_t)blockIdx.x * 2 * dim;
     for (int i = threadIdx.x; i < dim; i += kThreads) {
       dgamma[p + i] = sums[i];
       dbeta[p + i] = sums[dim + i];
@@ -237,40 +255,39 @@ __global__ __launch_bounds__(kThreads) void k_lnt_bwd(const bf16_t* __restrict__
   }
 }
 
-// dgamma | dbeta [2 * dim] = the sum of `parts` partial rows: 64 columns a workgroup, 16 waves over the
-// rows, eight loads in flight each.
+// dgamma | dbeta [2 * dim] = the sum of `parts` partial rows: 32 columns a workgroup, 32 row groups, sixteen loads in
+// flight each -- 512 partial rows are one round trip.
 __global__ __launch_bounds__(1024) void k_lnt_cols(const float* __restrict__ part, int parts, int dim,
                                                    float* __restrict__ dgamma, float* __restrict__ dbeta) {
-  __shared__ float s[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = blockIdx.x * 64 + lane, n = 2 * dim, cc = min(col, n - 1);
+  __shared__ float s[32][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + x, n = 2 * dim, cc = min(col, n - 1);
   float a = 0.f;
-  for (int p0 = wave; p0 < parts; p0 += 128) {
-    float v[8];
+  for (int p0 = y; p0 < parts; p0 += 512) {
+    float v[16];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = part[(int64_t)min(p0 + 16 * u, parts - 1) * n + cc];
+    for (int u = 0; u < 16; ++u) v[u] = part[(int64_t)min(p0 + 32 * u, parts - 1) * n + cc];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) a += p0 + 16 * u < parts ? v[u] : 0.f;
+    for (int u = 0; u < 16; ++u) a += p0 + 32 * u < parts ? v[u] : 0.f;
   }
-  s[wave][lane] = a;
+  s[y][x] = a;
   __syncthreads();
-  if (wave == 0 && col < n) {
-    a = 0.f;
+  a = s[x][y];                                     // row group x of column y
 #pragma unroll
-    for (int w = 0; w < 16; ++w) a += s[w][lane];
-    if (col < dim) dgamma[col] = a;
-    else dbeta[col - dim] = a;
+  for (int o = 16; o > 0; o >>= 1) a += __shfl_xor(a, o);
+  const int c = blockIdx.x * 32 + y;
+  if (x == 0 && c < n) {
+    if (c < dim) dgamma[c] = a;
+    else dbeta[c - dim] = a;
   }
 }
 
-// Rows a backward workgroup takes at a time (LNT_DISPATCH's 8 / WPR), its workgroups (one round each while
-// there are few rows) and their partial rows.
-inline int rows_at_once(int dim) { return dim <= 1024 ? 8 : dim <= 4096 ? 2 : 1; }
-inline int groups_for(int rows, int dim) {
-  const int r = rows_at_once(dim);
+// Workgroups (and partial rows) of the backward pass: as many as a round of R = 8 / WPR rows each takes while there
+// are few rows.
+inline int parts_for(int rows, int dim) {
+  const int r = dim <= 1024 ? 8 : dim <= 4096 ? 2 : 1;
   return std::max(1, std::min(kMaxGroups, (rows - 1) / r + 1));
 }
-inline int parts_for(int rows, int dim) { return groups_for(rows, dim) * (dim <= 1024 ? 1 : rows_at_once(dim)); }
 
 template <typename T, int E, int V, int WPR>
 void launch_fwd(const T* x, int64_t ldx, const float* gamma, const float* beta, float eps, int rows, int dim, bf16_t* y,
@@ -282,15 +299,15 @@ void launch_fwd(const T* x, int64_t ldx, const float* gamma, const float* beta, 
 template <typename T, int E, int V, int WPR>
 void launch_bwd(const bf16_t* dy, int64_t lddy, const T* x, int64_t ldx, const float2* stats, const float* gamma,
                 const T* add, int64_t lda, int rows, int dim, T* dx, int64_t lddx, float* dgamma, float* dbeta, hipStream_t s) {
-  hipLaunchKernelGGL((k_lnt_bwd<T, E, V, WPR>), dim3(groups_for(rows, dim)), dim3(kThreads),
-                     WPR == 1 ? 2 * dim * sizeof(float) : 0, s, dy,
+  hipLaunchKernelGGL((k_lnt_bwd<T, E, V, WPR>), dim3(parts_for(rows, dim)), dim3(kThreads),
+                     WPR < 8 ? 2 * dim * sizeof(float) : 0, s, dy,
                      lddy, x, ldx, stats, gamma, add, lda, rows, dim, dx, lddx, dgamma, dbeta);
 }
 
-// The narrowest instance that holds the row: E elements a load, V loads a lane, WPR waves a row.  Rows above
-// 1024 take four waves or eight: the backward pass holds four values and two sums a column, and one wave's
-// registers would leave two waves a SIMD (200 to 256 VGPRs at 1536 and 2048).
-#define LNT_DISPATCH(FN, T, ...)                       \
+// The narrowest instance that holds the row: E elements a load, V loads a lane, WPR waves a row.  The backward pass
+// holds four values and two sums a column: above 1024 a row takes four waves there, where one wave's registers would
+// leave two waves a SIMD (200 to 256 VGPRs at 1536 and 2048); the forward pass takes four above 2048.
+#define LNT_DISPATCH(FN, T, WIDE1, WIDE2, ...)         \
   do {                                                 \
     if (dim <= 64) FN<T, 1, 1, 1>(__VA_ARGS__);        \
     else if (dim <= 128) FN<T, 2, 1, 1>(__VA_ARGS__);  \
@@ -299,10 +316,14 @@ void launch_bwd(const bf16_t* dy, int64_t lddy, const T* x, int64_t ldx, const f
     else if (dim <= 512) FN<T, 4, 2, 1>(__VA_ARGS__);  \
     else if (dim <= 768) FN<T, 4, 3, 1>(__VA_ARGS__);  \
     else if (dim <= 1024) FN<T, 4, 4, 1>(__VA_ARGS__); \
-    else if (dim <= 2048) FN<T, 4, 2, 4>(__VA_ARGS__); \
+    else if (dim <= 1536) FN<T, WIDE1>(__VA_ARGS__);   \
+    else if (dim <= 2048) FN<T, WIDE2>(__VA_ARGS__);   \
     else if (dim <= 4096) FN<T, 8, 2, 4>(__VA_ARGS__); \
     else FN<T, 8, 2, 8>(__VA_ARGS__);                  \
   } while (0)
+#define LNT_F1 8, 3, 1
+#define LNT_F2 8, 4, 1
+#define LNT_B 8, 1, 4
 
 }  // namespace lnt
 }  // namespace i2pc
@@ -322,9 +343,9 @@ extern "C" int i2pc_layernorm_train(const void* x, int x_f32, int64_t ldx, const
   auto* st = reinterpret_cast<float2*>(stats);
   using namespace lnt;
   if (x_f32)
-    LNT_DISPATCH(launch_fwd, float, static_cast<const float*>(x), ldx, gamma, beta, eps, rows, dim, yy, ldy, st, s);
+    LNT_DISPATCH(launch_fwd, float, LNT_F1, LNT_F2, static_cast<const float*>(x), ldx, gamma, beta, eps, rows, dim, yy, ldy, st, s);
   else
-    LNT_DISPATCH(launch_fwd, bf16_t, static_cast<const bf16_t*>(x), ldx, gamma, beta, eps, rows, dim, yy, ldy, st, s);
+    LNT_DISPATCH(launch_fwd, bf16_t, LNT_F1, LNT_F2, static_cast<const bf16_t*>(x), ldx, gamma, beta, eps, rows, dim, yy, ldy, st, s);
   return check_launch("layernorm_train");
 }
 
@@ -354,12 +375,12 @@ extern "C" int i2pc_layernorm_backward(const void* dy, int64_t lddy, const void*
   auto* g = static_cast<const bf16_t*>(dy);
   auto* st = reinterpret_cast<const float2*>(stats);
   if (x_f32)
-    LNT_DISPATCH(launch_bwd, float, g, lddy, static_cast<const float*>(x), ldx, st, gamma, static_cast<const float*>(add),
+    LNT_DISPATCH(launch_bwd, float, LNT_B, LNT_B, g, lddy, static_cast<const float*>(x), ldx, st, gamma, static_cast<const float*>(add),
                  lda, rows, dim, static_cast<float*>(dx), lddx, pg, pb, s);
   else
-    LNT_DISPATCH(launch_bwd, bf16_t, g, lddy, static_cast<const bf16_t*>(x), ldx, st, gamma, static_cast<const bf16_t*>(add),
+    LNT_DISPATCH(launch_bwd, bf16_t, LNT_B, LNT_B, g, lddy, static_cast<const bf16_t*>(x), ldx, st, gamma, static_cast<const bf16_t*>(add),
                  lda, rows, dim, static_cast<bf16_t*>(dx), lddx, pg, pb, s);
   if (need)
-    hipLaunchKernelGGL(k_lnt_cols, dim3((2 * dim + 63) / 64), dim3(1024), 0, s, part, parts_for(rows, dim), dim, dgamma, dbeta);
+    hipLaunchKernelGGL(k_lnt_cols, dim3((2 * dim + 31) / 32), dim3(1024), 0, s, part, parts_for(rows, dim), dim, dgamma, dbeta);
   return check_launch("layernorm_backward");
 }

@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace i2pc {
 namespace attnp {
@@ -56,10 +57,11 @@ struct Args {
 
 // The kernel's arguments, read again where they are used: for code that is hardly ever reached, so that its
 // pointers and strides do not occupy scalar registers throughout.
-__device__ __forceinline__ const Args& again() {
-  const Args* p = (const Args*)(const __attribute__((address_space(4))) void*)__builtin_amdgcn_kernarg_segment_ptr();
+typedef const __attribute__((address_space(4))) Args ConstArgs;
+__device__ __forceinline__ ConstArgs* again() {
+  ConstArgs* p = (ConstArgs*)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(p));
-  return *p;
+  return p;
 }
 
 // ------------------------------------------------------------------ lookup of a tile
@@ -123,20 +125,18 @@ __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rs, uint32_t lds_bas
                : "memory", "m0");
 }
 
-// Where a tile of rows is read from: its first row and the bytes from there through the last row's 64 values.  Reads
-// behind them give zero.  The base is 64 bits and moves with the tile, so a sequence may span more than 4 GiB; moving it
-// is a few scalar additions.
+// Where a tile of rows is read from.  The base is 64 bits and moves with the tile, so a sequence may span more than
+// 4 GiB; moving it is a scalar addition, and so is the next tile's range: `rows` rows are left, and reads behind the
+// 64 values of the last of them give zero.
+template <int TILE>
 struct Src {
   const uint8_t* p;
-  int64_t left;
-  __device__ __forceinline__ Src(const bf16_t* row, int64_t pitch, int rows)
-      : p(reinterpret_cast<const uint8_t*>(row)), left(((rows - 1) * pitch + 64) * 2) {}
-  __device__ __forceinline__ void move(int64_t bytes) {
-    p += bytes;
-    left -= bytes;
-  }
-  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc() const {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, (int)min(left, (int64_t)0x7fffffff), 0x00020000);
+  uint32_t pitch;                // bytes from row to row
+  __device__ __forceinline__ Src(const bf16_t* row, int64_t row_stride)
+      : p(reinterpret_cast<const uint8_t*>(row)), pitch((uint32_t)row_stride * 2) {}
+  __device__ __forceinline__ void move() { p += (uint64_t)pitch * TILE; }
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(int rows) const {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, (min(rows, TILE) - 1) * pitch + 128, 0x00020000);
   }
 };
 
@@ -156,18 +156,43 @@ struct Stage {
   }
 };
 
-__device__ __forceinline__ bf16x8 row_frag(const uint8_t* tile, int row, int s, int hh) {
-  return *reinterpret_cast<const bf16x8*>(tile + row * 128 + (((2 * s + hh) ^ swz(row)) << 4));
-}
-// columns 32 dt .. + 31 of rows base + {0-3, 8-11} + 4 (lane >> 5) as the A operand of a product over the rows
-__device__ __forceinline__ bf16x8 tr_frag(const uint8_t* tile, int base, int dt, int lane) {
-  const int tg = lane >> 4, tq = (lane >> 2) & 3, tp = lane & 3;
-  const int d0 = 32 * dt + 16 * (tg & 1) + 4 * tp, ch = d0 >> 3, within = (d0 & 7) * 2;
-  const int r0 = base + 4 * (tg >> 1) + tq, r1 = r0 + 8;
-  const v4s lo = tr_read(tile + r0 * 128 + ((ch ^ swz(r0)) << 4) + within);
-  const v4s hi = tr_read(tile + r1 * 128 + ((ch ^ swz(r1)) << 4) + within);
-  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
+// Where a lane reads its operands from a tile of 128-byte rows at LDS address `tile`: the A operand of a product over d
+// (row lane & 31 of a 32-row block, chunk t of four) and of a product over the block's rows (columns 32 dt .. + 31 of rows
+// {0-3, 8-11} + 4 (lane >> 5), by two transposing reads).  The swizzle repeats every 16 rows, so that other blocks,
+// tiles and buffers are these addresses plus constants -- the offsets of the read instructions where the loops are
+// unrolled over the two buffers, and no vector additions.
+struct Lanes {
+  uint32_t row[4], lo[2], hi[2];
+  __device__ __forceinline__ Lanes(uint32_t tile, int lane) {
+    const int lr = lane & 31, hh = lane >> 5;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) row[t] = tile + lr * 128 + (((2 * t + hh) ^ swz(lr)) << 4);
+    const int tg = lane >> 4, tq = (lane >> 2) & 3, tp = lane & 3, r0 = 4 * (tg >> 1) + tq, r1 = r0 + 8;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) {
+      const int d0 = 32 * dt + 16 * (tg & 1) + 4 * tp, ch = d0 >> 3, within = (d0 & 7) * 2;
+      lo[dt] = tile + r0 * 128 + ((ch ^ swz(r0)) << 4) + within;
+      hi[dt] = tile + r1 * 128 + ((ch ^ swz(r1)) << 4) + within;
+    }
+  }
+  __device__ __forceinline__ Lanes behind(uint32_t bytes) const {      // the addresses of another buffer
+    Lanes x = *this;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) x.row[t] += bytes;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) x.lo[dt] += bytes, x.hi[dt] += bytes;
+    return x;
+  }
+  // `at`: bytes from `tile` to the block's first row (rows: 16 of them for a column read)
+  __device__ __forceinline__ bf16x8 rows(int t, uint32_t at) const {
+    return *(const __attribute__((address_space(3))) bf16x8*)(row[t] + at);
+  }
+  __device__ __forceinline__ bf16x8 columns(int dt, uint32_t at) const {
+    const v4s l = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(lo[dt] + at));
+    const v4s h = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(hi[dt] + at));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(l, h, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
 __device__ __forceinline__ bf16x8 p_frag(const uint32_t (&pk)[8], int s) {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   return __builtin_bit_cast(bf16x8, u32x4{pk[4 * s], pk[4 * s + 1], pk[4 * s + 2], pk[4 * s + 3]});
@@ -212,12 +237,18 @@ __device__ __forceinline__ void add_row(f32x16 (&acc)[2], float w, const bf16_t*
     }
 }
 
-// whether this lane's part of rows base .. base + 31 of a tile has an infinity or NaN
-__device__ __forceinline__ int has_nonfinite(const uint8_t* tile, int base, int lane) {
+// whether this lane's part of the 32 rows at `at` has an infinity or NaN
+__device__ __forceinline__ int has_nonfinite(const Lanes& ad, uint32_t at) {
   int bad = 0;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) bad |= nonfinite(row_frag(tile, base + (lane & 31), t, lane >> 5));
+  for (int t = 0; t < 4; ++t) bad |= nonfinite(ad.rows(t, at));
   return bad;
+}
+
+// a bound that the compiler does not take apart: it would keep sixteen of its sums with constants in registers instead
+__device__ __forceinline__ int whole(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 // 4 consecutive values a lane and register group of an accumulator, times f, as bf16: row[32 dt + 8 g + 4 hh ...]
@@ -254,52 +285,49 @@ __device__ __forceinline__ void zero_rows(bf16_t* out, int64_t o_t, int64_t o_h,
 // A row's running state, a row to a lane (its two lane halves hold different keys' probabilities and different d of O).
 struct Rows {
   f32x16 o[2];                   // O^T, not normalised
-  f32x16 nm;                     // minus the reference m, in units of the raw scores, all 16 alike
-  float l;                       // this half's sum of 2^(c (s - m))
+  float m;                       // the reference, c times a raw score
+  float l;                       // this half's sum of 2^(c s - m)
   int bad;                       // met an infinity or NaN in a partly masked block
   __device__ __forceinline__ void clear() {
-    for (int i = 0; i < 16; ++i) o[0][i] = o[1][i] = nm[i] = 0.f;
-    l = 0.f;
+    for (int i = 0; i < 16; ++i) o[0][i] = o[1][i] = 0.f;
+    m = l = 0.f;
     bad = 0;
   }
 };
 
-// 32 keys (rows base .. base + 31 of the K and V tiles) for 32 rows.  S^T = K Q^T starts at -m (the accumulator's start
-// value), so p = 2^(c s); m moves only when a probability could pass 2^8 (harmless for the bf16 operand and the fp32
-// sums), so the usual block has no maximum and no rescale.  `first`: the rows' first block, which sets m.  left: how many
-// of the block's keys the lane's row sees; partial (uniform): not all of them for some row of the wave.
+// 32 keys (at bytes atK, atV behind the addresses' tile) for 32 rows: p = 2^(c s - m), one FMA and one exponential a
+// score.  m moves only when a probability could pass 2^8 (harmless for the bf16 operand and the fp32 sums), so the usual
+// block has no maximum and no rescale.  `first`: the rows' first block, which sets m.  left: how many of the block's keys
+// the lane's row sees; partial (uniform): not all of them for some row of the wave.
 template <bool CAUSAL>
-__device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const uint8_t* sK, const uint8_t* sV, int base, bool first,
-                                       bool partial, int left, float c, int lane) {
+__device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const Lanes& ad, uint32_t atK, uint32_t atV, bool first,
+                                       bool partial, int left, float c, int hh) {
   constexpr float kThresh = 256.f;
-  const int hh = lane >> 5, lr = lane & 31;
   bf16x8 kf[4];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) kf[t] = row_frag(sK, base + lr, t, hh);
+  for (int t = 0; t < 4; ++t) kf[t] = ad.rows(t, atK);
   f32x16 st;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) st = mfma(kf[t], qf[t], t == 0 ? w.nm : st);
+  for (int t = 0; t < 4; ++t) st = mfma(kf[t], qf[t], t == 0 ? f32x16{} : st);
   if (partial) {
-    const int lim = left - 4 * hh;
+    const int lim = whole(left - 4 * hh);
 #pragma unroll
     for (int i = 0; i < 16; ++i) st[i] = (i & 3) + 8 * (i >> 2) < lim ? st[i] : -INFINITY;
   }
   float ls = 0.f;
   uint32_t pk[8];
-  auto probs = [&](float sub) {                      // sub: in units of the raw scores
-    ls = 0.f;
-    const float nsub = -sub * c;
+  auto probs = [&]() {
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
-      const float p0 = __builtin_amdgcn_exp2f(fmaf(st[i], c, nsub));
-      const float p1 = __builtin_amdgcn_exp2f(fmaf(st[i + 1], c, nsub));
-      ls += p0 + p1;
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(st[i], c, -w.m));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(st[i + 1], c, -w.m));
+      ls = i ? ls + (p0 + p1) : p0 + p1;
       pk[i >> 1] = pack_bf16(p0, p1);
     }
   };
   bool full = first;
   if (!full) {
-    probs(0.f);
+    probs();
     full = __ballot(ls >= kThresh) != 0;
   }
   if (full) {
@@ -307,12 +335,11 @@ __device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const uin
 #pragma unroll
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[i]);
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-    mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+    mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * c;
     // a row that sees nothing here keeps its reference
-    const float delta = first ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, 0.f);
-    probs(delta);
+    const float m_new = first ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, w.m);
     if (!first) {
-      const float alpha = __builtin_amdgcn_exp2f(-delta * c);
+      const float alpha = __builtin_amdgcn_exp2f(w.m - m_new);
       w.l *= alpha;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -320,16 +347,16 @@ __device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const uin
         w.o[1][i] *= alpha;
       }
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w.nm[i] -= delta;
+    w.m = m_new;
+    probs();
   }
   w.l += ls;
   bf16x8 vf[2][2];
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
-    for (int dt = 0; dt < 2; ++dt) vf[t][dt] = tr_frag(sV, base + 16 * t, dt, lane);
-  if (CAUSAL && partial) w.bad |= has_nonfinite(sV, base, lane);
+    for (int dt = 0; dt < 2; ++dt) vf[t][dt] = ad.columns(dt, atV + 2048 * t);
+  if (CAUSAL && partial) w.bad |= has_nonfinite(ad, atV);
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -343,10 +370,10 @@ __device__ __forceinline__ void attend_again(Rows& w, const bf16x8 (&qf)[4], con
   w.clear();
 #pragma clang loop unroll(disable)
   for (int j = from; j < to; j += (j & 31) == 31 ? step : 1) {
-    const float x = dot_row(K + j * k_t, qf, hh);
+    const float x = dot_row(K + j * k_t, qf, hh) * c;
     if (j < nk) {
-      const float m_new = fmaxf(m, x), alpha = m == m_new ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
-      const float p = __builtin_amdgcn_exp2f((x - m_new) * c);
+      const float m_new = fmaxf(m, x), alpha = m == m_new ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+      const float p = __builtin_amdgcn_exp2f(x - m_new);
       m = m_new;
       l = fmaf(l, alpha, p);
       for (int i = 0; i < 16; ++i) {
@@ -356,7 +383,7 @@ __device__ __forceinline__ void attend_again(Rows& w, const bf16x8 (&qf)[4], con
       add_row(w.o, p, V + j * v_t, hh);
     }
   }
-  for (int i = 0; i < 16; ++i) w.nm[i] = m == -INFINITY ? 0.f : -m;
+  w.m = m == -INFINITY ? 0.f : m;
   w.l = hh ? 0.f : l;                                // the whole sum; the halves' are added
 }
 
@@ -366,7 +393,7 @@ __device__ __forceinline__ void attend_again(Rows& w, const bf16x8 (&qf)[4], con
 // LDS-DMA, double-buffered.  KW 2: waves 2, 3 hold the rows of waves 0, 1 again and take the second 32 keys of each tile,
 // and the two states are joined at the end: twice the workgroups, of half the length.
 template <bool CAUSAL, bool SPLIT, int KW>
-__global__ __launch_bounds__(256, 3) void k_attnp_fwd(const Args a) {
+__global__ __launch_bounds__(256, 4) void k_attnp_fwd(const Args a) {
   constexpr int kWgRows = kRows / KW;
   __shared__ __attribute__((aligned(16))) uint8_t smem[4 * kTileBytes];
   __shared__ float ml[2][KW == 2 ? 2 : 1][KW == 2 ? 64 : 1];
@@ -406,16 +433,15 @@ __global__ __launch_bounds__(256, 3) void k_attnp_fwd(const Args a) {
   const bf16_t* Kg = a.k + (s.k0 * a.k_t + hk * a.k_h);
   const bf16_t* Vg = a.v + (s.k0 * a.v_t + hk * a.v_h);
   const Stage stk(wid, lane, a.k_t), stv(wid, lane, a.v_t);
-  Src srck(Kg + ks * a.k_t, a.k_t, s.lk - ks), srcv(Vg + ks * a.v_t, a.v_t, s.lk - ks);
-  const int64_t stepk = a.k_t * kKV * 2, stepv = a.v_t * kKV * 2;
+  Src<kKV> srck(Kg + ks * a.k_t, a.k_t), srcv(Vg + ks * a.v_t, a.v_t);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem)) + wid * 2048;
-  auto stage = [&](int buf) {                        // the next tile
-    stk.load(srck.rsrc(), lds0 + buf * 2 * kTileBytes);
-    stv.load(srcv.rsrc(), lds0 + (buf * 2 + 1) * kTileBytes);
-    srck.move(stepk);
-    srcv.move(stepv);
+  auto stage = [&](int buf, int key) {               // the next tile, which starts at key
+    stk.load(srck.rsrc(s.lk - key), lds0 + buf * 2 * kTileBytes);
+    stv.load(srcv.rsrc(s.lk - key), lds0 + (buf * 2 + 1) * kTileBytes);
+    srck.move();
+    srcv.move();
   };
-  if (ks < ke) stage(0);
+  if (ks < ke) stage(0, ks);
   bf16x8 qf[4];
   {
     const bf16_t* qr = a.q + (s.q0 + qi) * a.q_t + h * a.q_h;
@@ -428,23 +454,29 @@ __global__ __launch_bounds__(256, 3) void k_attnp_fwd(const Args a) {
   const float c = a.c;
   Rows w;
   w.clear();
-  for (int key0 = ks, cur = 0; key0 < ke; key0 += kKV, cur ^= 1) {
-    if (key0 + kKV < ke) stage(cur ^ 1);
-    const uint8_t* sK = smem + cur * 2 * kTileBytes;
+  const Lanes ad(lds_addr(smem) + kw * 4096, lane);
+  auto step = [&](int key0, auto buffer) {
+    constexpr int cur = decltype(buffer)::value;
+    if (key0 + kKV < ke) stage(cur ^ 1, key0 + kKV);
     if (wave_on) {
 #pragma unroll
       for (int k2 = 0; k2 < 2 / KW; ++k2) {
-        const int at = 32 * (k2 + kw), key = key0 + at;
+        const int key = key0 + 32 * (k2 + kw);
         if (key >= nk_last) break;                   // no row of the wave sees these keys
-        attend<CAUSAL>(w, qf, sK, sK + kTileBytes, at, key == ks + 32 * kw, key + 32 > nk_first, nk - key, c, lane);
+        attend<CAUSAL>(w, qf, ad, cur * 2 * kTileBytes + k2 * 4096, (cur * 2 + 1) * kTileBytes + k2 * 4096, key == ks + 32 * kw,
+                       key + 32 > nk_first, nk - key, c, hh);
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the next tile landed (this wave's part)
     __syncthreads();                                     // ... and every wave's
+  };
+  for (int key0 = ks; key0 < ke; key0 += 2 * kKV) {
+    step(key0, std::integral_constant<int, 0>{});
+    if (key0 + kKV < ke) step(key0 + kKV, std::integral_constant<int, 1>{});
   }
   if (CAUSAL && __ballot(w.bad) != 0)
     attend_again(w, qf, Kg, a.k_t, Vg, a.v_t, ks + 32 * kw, min(ke, nk_last), KW == 2 ? 33 : 1, nk, c, hh);
-  float l = w.l + __shfl_xor(w.l, 32), m = -w.nm[0];
+  float l = w.l + __shfl_xor(w.l, 32), m = w.m;
   if constexpr (KW == 2) {
     float* x = reinterpret_cast<float*>(smem) + rw * 32 * 64 + lane;
     if (kw == 1) {
@@ -461,7 +493,7 @@ __global__ __launch_bounds__(256, 3) void k_attnp_fwd(const Args a) {
     const float m1 = ml[0][rw][lane], l1 = ml[1][rw][lane];
     if (l1 != 0.f) {                                 // (NaN: joined too)
       const float mm = l == 0.f ? m1 : fmaxf(m, m1);
-      const float f0 = m == mm ? 1.f : __builtin_amdgcn_exp2f((m - mm) * c), f1 = m1 == mm ? 1.f : __builtin_amdgcn_exp2f((m1 - mm) * c);
+      const float f0 = m == mm ? 1.f : __builtin_amdgcn_exp2f(m - mm), f1 = m1 == mm ? 1.f : __builtin_amdgcn_exp2f(m1 - mm);
       l = l == 0.f ? l1 * f1 : fmaf(l, f0, l1 * f1);
       m = mm;
 #pragma unroll
@@ -473,7 +505,7 @@ __global__ __launch_bounds__(256, 3) void k_attnp_fwd(const Args a) {
   }
   if (r >= R) return;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  const float l2 = l == 0.f ? -INFINITY : fmaf(m, c, log2f(l));
+  const float l2 = l == 0.f ? -INFINITY : m + log2f(l);
   if (SPLIT) {
     const int64_t row = ((int64_t)split * a.Hk + hk) * a.Tq * a.G + (int64_t)s.q0 * a.G + r;
     if (hh == 0) a.part_l[row] = l2;
@@ -534,18 +566,17 @@ __global__ __launch_bounds__(256, 2) void k_attnp_few(const Args a) {
   }
   uint8_t* mine = smem + wid * 4 * kFewBlock;
   const int first = ks + 32 * wid;
-  Src srck(Kg + first * a.k_t, a.k_t, s.lk - first), srcv(Vg + first * a.v_t, a.v_t, s.lk - first);
-  const int64_t stepk = a.k_t * 256, stepv = a.v_t * 256;
+  Src<128> srck(Kg + first * a.k_t, a.k_t), srcv(Vg + first * a.v_t, a.v_t);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(mine));
-  auto stage = [&](int buf) {                        // the wave's next block
-    const auto rk = srck.rsrc(), rv = srcv.rsrc();
+  auto stage = [&](int buf, int key) {               // the wave's next block, which starts at key
+    const auto rk = srck.rsrc(s.lk - key), rv = srcv.rsrc(s.lk - key);
     const uint32_t base = lds0 + buf * 2 * kFewBlock;
 #pragma unroll
     for (int j = 0; j < 4; ++j) dma16(rk, base + j * 1024, offk[j]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) dma16(rv, base + kFewBlock + j * 1024, offv[j]);
-    srck.move(stepk);
-    srcv.move(stepv);
+    srck.move();
+    srcv.move();
   };
   bf16x8 qf[4];
   {
@@ -553,26 +584,31 @@ __global__ __launch_bounds__(256, 2) void k_attnp_few(const Args a) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) qf[t] = *reinterpret_cast<const bf16x8*>(qr + 16 * t + 8 * hh);
   }
-  if (first < ke) stage(0);
+  if (first < ke) stage(0, first);
   const float c = a.c;
   Rows w;
   w.clear();
-  for (int key = first, cur = 0; key < ke; key += 128, cur ^= 1) {
+  const Lanes ad(lds_addr(mine), lane);
+  auto step = [&](int key, auto buffer) {
+    constexpr int cur = decltype(buffer)::value;
     if (key + 128 < ke) {
       // the other buffer's reads have returned before it is written again
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      stage(cur ^ 1);
+      stage(cur ^ 1, key + 128);
       asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // this block landed, the next one's 8 loads may be on their way
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    const uint8_t* sK = mine + cur * 2 * kFewBlock;
-    attend<CAUSAL>(w, qf, sK, sK + kFewBlock, 0, key == first, key + 32 > nk_first, nk - key, c, lane);
+    attend<CAUSAL>(w, qf, ad, cur * 2 * kFewBlock, (cur * 2 + 1) * kFewBlock, key == first, key + 32 > nk_first, nk - key, c, hh);
+  };
+  for (int key = first; key < ke; key += 256) {
+    step(key, std::integral_constant<int, 0>{});
+    if (key + 128 < ke) step(key + 128, std::integral_constant<int, 1>{});
   }
   if (CAUSAL && __ballot(w.bad) != 0) attend_again(w, qf, Kg, a.k_t, Vg, a.v_t, first, ke, 97, nk, c, hh);
   const float l = w.l + __shfl_xor(w.l, 32);
 
-  // the four waves' sums: sum_w f_w O_w, f_w = 2^(c (m_w - m))
+  // the four waves' sums: sum_w f_w O_w, f_w = 2^(m_w - m)
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   float* ow = reinterpret_cast<float*>(mine);
 #pragma unroll
@@ -582,7 +618,7 @@ __global__ __launch_bounds__(256, 2) void k_attnp_few(const Args a) {
       *reinterpret_cast<float4*>(ow + lr * 68 + 32 * dt + 8 * g + 4 * hh) =
           make_float4(w.o[dt][4 * g], w.o[dt][4 * g + 1], w.o[dt][4 * g + 2], w.o[dt][4 * g + 3]);
   if (hh == 0) {
-    ml[0][wid][lr] = l == 0.f ? -INFINITY : -w.nm[0];
+    ml[0][wid][lr] = l == 0.f ? -INFINITY : w.m;
     ml[1][wid][lr] = l;
   }
   __syncthreads();
@@ -595,14 +631,14 @@ __global__ __launch_bounds__(256, 2) void k_attnp_few(const Args a) {
   for (int v = 0; v < 4; ++v) {
     const float lv = ml[1][v][row];
     if (lv == 0.f) continue;                         // saw nothing (a NaN sum is not skipped)
-    const float mv = ml[0][v][row], f = mv == m ? 1.f : __builtin_amdgcn_exp2f((mv - m) * c);
+    const float mv = ml[0][v][row], f = mv == m ? 1.f : __builtin_amdgcn_exp2f(mv - m);
     total = fmaf(f, lv, total);
     const float* x = reinterpret_cast<const float*>(smem + v * 4 * kFewBlock) + row * 68 + d;
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = fmaf(f, x[i], acc[i]);
   }
   const float inv = total == 0.f ? 0.f : 1.0f / total;
-  const float l2 = total == 0.f ? -INFINITY : fmaf(m, c, log2f(total));
+  const float l2 = total == 0.f ? -INFINITY : m + log2f(total);
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] *= inv;
   const int i = r / a.G, hq = hk * a.G + r - i * a.G;
@@ -728,16 +764,15 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
   const bf16_t* Kg = a.k + (s.k0 * a.k_t + hk * a.k_h);
   const bf16_t* Vg = a.v + (s.k0 * a.v_t + hk * a.v_h);
   const Stage stk(wid, lane, a.k_t), stv(wid, lane, a.v_t);
-  Src srck(Kg, a.k_t, s.lk), srcv(Vg, a.v_t, s.lk);
-  const int64_t stepk = a.k_t * kKV * 2, stepv = a.v_t * kKV * 2;
+  Src<kKV> srck(Kg, a.k_t), srcv(Vg, a.v_t);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem)) + wid * 2048;
-  auto stage = [&](int buf) {
-    stk.load(srck.rsrc(), lds0 + buf * 2 * kTileBytes);
-    stv.load(srcv.rsrc(), lds0 + (buf * 2 + 1) * kTileBytes);
-    srck.move(stepk);
-    srcv.move(stepv);
+  auto stage = [&](int buf, int key) {
+    stk.load(srck.rsrc(s.lk - key), lds0 + buf * 2 * kTileBytes);
+    stv.load(srcv.rsrc(s.lk - key), lds0 + (buf * 2 + 1) * kTileBytes);
+    srck.move();
+    srcv.move();
   };
-  if (ke > 0) stage(0);
+  if (ke > 0) stage(0, 0);
   bf16x8 qf[4], df[4];
   const bf16_t* qr = a.q + (s.q0 + qi) * a.q_t + h * a.q_h;
   const bf16_t* dr = a.dout + (s.q0 + qi) * a.d_t + h * a.d_h;
@@ -759,28 +794,29 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
   __syncthreads();
 
   int bad = 0;
-  for (int key0 = 0, cur = 0; key0 < ke; key0 += kKV, cur ^= 1) {
-    if (key0 + kKV < ke) stage(cur ^ 1);
-    const uint8_t* sK = smem + cur * 2 * kTileBytes;
-    const uint8_t* sV = sK + kTileBytes;
+  const Lanes ad(lds_addr(smem) + kw * 4096, lane);
+  auto step = [&](int key0, auto buffer) {
+    constexpr int cur = decltype(buffer)::value;
+    if (key0 + kKV < ke) stage(cur ^ 1, key0 + kKV);
     if (wave_on) {
 #pragma unroll
       for (int k2 = 0; k2 < 2 / KW; ++k2) {
-        const int at = 32 * (k2 + kw), key = key0 + at;
+        const int key = key0 + 32 * (k2 + kw);
+        const uint32_t atK = cur * 2 * kTileBytes + k2 * 4096, atV = atK + kTileBytes;
         if (key >= nk_last) break;
         f32x16 st, dp;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          st = mfma(row_frag(sK, at + lr, t, hh), qf[t], t == 0 ? f32x16{} : st);
-          dp = mfma(row_frag(sV, at + lr, t, hh), df[t], t == 0 ? nd : dp);
+          st = mfma(ad.rows(t, atK), qf[t], t == 0 ? f32x16{} : st);
+          dp = mfma(ad.rows(t, atV), df[t], t == 0 ? nd : dp);
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(fmaf(st[i], c, nl));
         if (key + 32 > nk_first) {                   // some row of the wave does not see all of the block
-          const int lim = nk - key - 4 * hh;
+          const int lim = whole(nk - key - 4 * hh);
 #pragma unroll
           for (int i = 0; i < 16; ++i) dp[i] = (i & 3) + 8 * (i >> 2) < lim ? dp[i] : 0.f;
-          if (CAUSAL) bad |= has_nonfinite(sK, at, lane);
+          if (CAUSAL) bad |= has_nonfinite(ad, atK);
         }
         uint32_t pk[8];
 #pragma unroll
@@ -788,11 +824,15 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int dt = 0; dt < 2; ++dt) dq[dt] = mfma(tr_frag(sK, at + 16 * t, dt, lane), p_frag(pk, t), dq[dt]);
+          for (int dt = 0; dt < 2; ++dt) dq[dt] = mfma(ad.columns(dt, atK + 2048 * t), p_frag(pk, t), dq[dt]);
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
+  };
+  for (int key0 = 0; key0 < ke; key0 += 2 * kKV) {
+    step(key0, std::integral_constant<int, 0>{});
+    if (key0 + kKV < ke) step(key0 + kKV, std::integral_constant<int, 1>{});
   }
   if (CAUSAL && __ballot(bad) != 0) {
     for (int i = 0; i < 16; ++i) dq[0][i] = dq[1][i] = 0.f;
@@ -825,12 +865,15 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
 // dK, dV: 32 KW keys of one key head a workgroup, over the rows of its query heads one after the other (of one of them
 // with a.nsplit = G: partial sums, joined by k_attnp_sum).  A key to a lane: S = Q K^T (which starts at -lse / scale) and
 // dP = dO V^T (at -D) leave a key's column in one lane's registers, which then are the B operand of dV^T += dO^T P and
-// dK^T += Q^T dS.  KW 4: every wave has 32 keys and takes all 64 rows of a tile; KW 2: waves 2, 3 hold the keys of waves 0,
-// 1 again and take rows 32-63 of each tile, their sums are added at the end.
+// dK^T += Q^T dS.  Tiles are of RT = 256 / KW rows: with KW 4 every wave has 32 keys and takes both 32-row blocks of a tile;
+// with KW 2 waves 2, 3 hold the keys of waves 0, 1 again, a wave takes two of the four blocks and the sums are added at the
+// end.  A wave's two blocks are independent: while one's exponentials are on the vector unit the other's products are on
+// the matrix unit.
 template <bool CAUSAL, int KW>
 __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
-  // two buffers of Q tile, dO tile, 64 nlse, 64 ndelta
-  constexpr int kBuf = 2 * kTileBytes + 512;
+  constexpr int RT = 256 / KW, kRowBytes = RT * 128;
+  // two buffers of Q tile, dO tile, RT nlse, RT ndelta
+  constexpr int kBuf = 2 * kRowBytes + 8 * RT;
   __shared__ __attribute__((aligned(16))) uint8_t smem[2 * kBuf];
   const int lane = threadIdx.x & 63, hh = lane >> 5, lr = lane & 31;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -862,38 +905,50 @@ __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
   const int g0 = a.nsplit == 1 ? 0 : split, g1 = a.nsplit == 1 ? a.G : split + 1;
   const bool any = i_first < s.lq;
 
-  const Stage stq(wid, lane, a.q_t), std_(wid, lane, a.d_t);
-  const bf16_t* Q0 = a.q + ((s.q0 + i_first) * a.q_t + (hk * a.G + g0) * a.q_h);
-  const bf16_t* D0 = a.dout + ((s.q0 + i_first) * a.d_t + (hk * a.G + g0) * a.d_h);
-  // waves 0 and 1 also load the tile's nlse and ndelta
-  const float* S0 = (wid ? a.ndelta : a.nlse) + (int64_t)(hk * a.G + g0) * a.Tq + s.q0 + i_first;
-  const float* S = S0;
-  Src srcq(Q0, a.q_t, s.lq - i_first), srcd(D0, a.d_t, s.lq - i_first);
-  const int64_t stepq = a.q_t * 128, stepd = a.d_t * 128;
-  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem)) + wid * 2048;
-  const uint32_t ldss = lds0 - wid * 2048 + 2 * kTileBytes + wid * 256;
+  // a wave loads RT / 4 rows of Q and of dO, 8 an instruction
+  constexpr int kOps = RT / 32;
+  uint32_t offq[kOps], offd[kOps];
+#pragma unroll
+  for (int j = 0; j < kOps; ++j) {
+    const int row = (wid * kOps + j) * 8 + (lane >> 3), ch = ((lane & 7) ^ swz(row)) * 8;
+    offq[j] = (uint32_t)((row * a.q_t + ch) * 2);
+    offd[j] = (uint32_t)((row * a.d_t + ch) * 2);
+  }
+  // and 64 of the tile's 2 RT statistics (waves 0, 1 of four with 64-row tiles)
+  const bool stat_on = wid < RT / 32;
+  const int stat_at = KW == 4 ? 0 : (wid & 1) * 64;
+  auto q_of = [&](auto* w, int g) { return w->q + ((s.q0 + i_first) * w->q_t + (hk * w->G + g) * w->q_h); };
+  auto d_of = [&](auto* w, int g) { return w->dout + ((s.q0 + i_first) * w->d_t + (hk * w->G + g) * w->d_h); };
+  auto s_of = [&](auto* w, int g) {
+    return ((KW == 4 ? wid : wid >> 1) ? w->ndelta : w->nlse) + (int64_t)(hk * w->G + g) * w->Tq + s.q0 + i_first + stat_at;
+  };
+  Src<RT> srcq(q_of(&a, g0), a.q_t), srcd(d_of(&a, g0), a.d_t);
+  const float* stats = s_of(&a, g0);
+  const uint32_t ldsb = __builtin_amdgcn_readfirstlane(lds_addr(smem));
+  const uint32_t lds0 = ldsb + wid * kOps * 1024, ldss = ldsb + 2 * kRowBytes + wid * 256;
   int next_i = i_first, next_g = g0;                   // the tile that is loaded next
   auto stage = [&](int buf) {
-    stq.load(srcq.rsrc(), lds0 + buf * kBuf);
-    std_.load(srcd.rsrc(), lds0 + buf * kBuf + kTileBytes);
-    if (wid < 2) {
-      const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(S), 0, min(s.lq - next_i, 64) * 4, 0x00020000);
-      dma4(rs, ldss + buf * kBuf, lane * 4);
+    const auto rq = srcq.rsrc(s.lq - next_i), rd = srcd.rsrc(s.lq - next_i);
+#pragma unroll
+    for (int j = 0; j < kOps; ++j) dma16(rq, lds0 + buf * kBuf + j * 1024, offq[j]);
+#pragma unroll
+    for (int j = 0; j < kOps; ++j) dma16(rd, lds0 + buf * kBuf + kRowBytes + j * 1024, offd[j]);
+    if (stat_on) {
+      const int n = __builtin_amdgcn_readfirstlane(max(0, min(s.lq - next_i - stat_at, 64)));
+      dma4(__builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(stats), 0, n * 4, 0x00020000), ldss + buf * kBuf, lane * 4);
     }
-    next_i += 64;
+    next_i += RT;
     if (next_i < s.lq) {
-      srcq.move(stepq);
-      srcd.move(stepd);
-      S += 64;
+      srcq.move();
+      srcd.move();
+      stats += RT;
     } else {                                           // the next query head
       next_i = i_first;
       ++next_g;
-      Q0 += a.q_h;
-      D0 += a.d_h;
-      S0 += a.Tq;
-      srcq = Src(Q0, a.q_t, s.lq - i_first);
-      srcd = Src(D0, a.d_t, s.lq - i_first);
-      S = S0;
+      ConstArgs* w = again();
+      srcq.p = reinterpret_cast<const uint8_t*>(q_of(w, next_g));
+      srcd.p = reinterpret_cast<const uint8_t*>(d_of(w, next_g));
+      stats = s_of(w, next_g);
     }
   };
   if (any) stage(0);
@@ -915,79 +970,160 @@ __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
   for (int i = 0; i < 16; ++i) dk[0][i] = dk[1][i] = dv[0][i] = dv[1][i] = 0.f;
 
   int bad = 0, cur = 0;
-  for (int g = g0; any && g < g1; ++g)
-    for (int i1 = i_first; i1 < s.lq; i1 += 64, cur ^= 1) {
-      if (next_g < g1) stage(cur ^ 1);
-      const uint8_t* sQ = smem + cur * kBuf;
-      const uint8_t* sD = sQ + kTileBytes;
-      const float* stat = reinterpret_cast<const float*>(sQ + 2 * kTileBytes);
+  // the wave's blocks: rows ra and ra + kApart of a tile
+  constexpr int kApart = KW == 2 ? 64 : 32;
+  const int ra = 32 * qh;
+  const Lanes ad0(ldsb + ra * 128, lane);
+  const uint32_t stat0 = ldsb + 2 * kRowBytes + (ra + 4 * hh) * 4;
+  // One tile, whose first query is i1.  EDGE: some of its queries may not see some of the workgroup's keys.  (Rows behind
+  // the sequence are zero, with statistics of zero: they add nothing.)
+  auto tile_step = [&](int i1, auto edge) {
+    constexpr bool EDGE = decltype(edge)::value;
+    constexpr uint32_t atQ = 0, atD = kRowBytes;
+    if (next_g < g1) stage(cur ^ 1);
+    const Lanes ad = ad0.behind(cur * kBuf);
+    const uint32_t stat = stat0 + cur * kBuf;
+    // What a block's products need is read a phase ahead of them: the rows of Q and dO, with -lse / scale and -D as the
+    // accumulators' start values, then their transposes.
+    struct Block {
+      bf16x8 q[4], d[4];
+      f32x16 st, dp;
+    };
+    auto read_rows = [&](int r, Block& x) {            // r: rows behind ra
 #pragma unroll
-      for (int u = 0; u < KW / 2; ++u) {
-        const int rb = 32 * (u + qh), i0 = i1 + rb;            // the block's first row in the tile, its first query
-        // some query of the block exists and sees some key of the wave
-        if (i0 < s.lq && (!CAUSAL || i0 + 31 >= kw - off)) {
-          f32x16 st, dp;
+      for (int t = 0; t < 4; ++t) {
+        x.q[t] = ad.rows(t, atQ + r * 128);
+        x.d[t] = ad.rows(t, atD + r * 128);
+      }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float4 x = *reinterpret_cast<const float4*>(stat + rb + 8 * q + 4 * hh);
-            const float4 y = *reinterpret_cast<const float4*>(stat + 64 + rb + 8 * q + 4 * hh);
-            st[4 * q] = x.x, st[4 * q + 1] = x.y, st[4 * q + 2] = x.z, st[4 * q + 3] = x.w;
-            dp[4 * q] = y.x, dp[4 * q + 1] = y.y, dp[4 * q + 2] = y.z, dp[4 * q + 3] = y.w;
-          }
+      for (int q = 0; q < 4; ++q) {
+        typedef float f32x4 __attribute__((ext_vector_type(4)));
+        const f32x4 u = *(const __attribute__((address_space(3))) f32x4*)(stat + (r + 8 * q) * 4);
+        const f32x4 v = *(const __attribute__((address_space(3))) f32x4*)(stat + (RT + r + 8 * q) * 4);
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            st = mfma(row_frag(sQ, rb + lr, t, hh), kf[t], st);
-            dp = mfma(row_frag(sD, rb + lr, t, hh), vf[t], dp);
-          }
+        for (int i = 0; i < 4; ++i) x.st[4 * q + i] = u[i], x.dp[4 * q + i] = v[i];
+      }
+    };
+    auto read_columns = [&](int r, Block& x) {         // in place of the rows
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            st[i] = __builtin_amdgcn_exp2f(st[i] * c);
-            dp[i] *= st[i];
-          }
-          if (CAUSAL && i0 < kw + 31 - off) {                  // some query of the block does not see some key of the wave
-            const int lim = key - off - i0 - 4 * hh;           // the rows below this do not see the lane's key
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const bool on = (i & 3) + 8 * (i >> 2) >= lim;
-              st[i] = on ? st[i] : 0.f;
-              dp[i] = on ? dp[i] : 0.f;
-            }
-            bad |= has_nonfinite(sQ, rb, lane) | has_nonfinite(sD, rb, lane);
-          }
-          uint32_t pk[8], dsk[8];
+        for (int dt = 0; dt < 2; ++dt) {
+          x.d[2 * t + dt] = ad.columns(dt, atD + r * 128 + 2048 * t);
+          x.q[2 * t + dt] = ad.columns(dt, atQ + r * 128 + 2048 * t);
+        }
+    };
+    auto scores = [&](int r, Block& x) {               // S - lse / scale and dP - D
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            pk[i >> 1] = pack_bf16(st[i], st[i + 1]);
-            dsk[i >> 1] = pack_bf16(dp[i], dp[i + 1]);
-          }
+      for (int t = 0; t < 4; ++t) {
+        x.st = mfma(x.q[t], kf[t], x.st);
+        x.dp = mfma(x.d[t], vf[t], x.dp);
+      }
+      if (EDGE) {
+        const int lim = whole(key - off - i1 - ra - r - 4 * hh);  // the rows below this do not see the lane's key
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int dt = 0; dt < 2; ++dt) {
-              dv[dt] = mfma(tr_frag(sD, rb + 16 * t, dt, lane), p_frag(pk, t), dv[dt]);
-              dk[dt] = mfma(tr_frag(sQ, rb + 16 * t, dt, lane), p_frag(dsk, t), dk[dt]);
-            }
+        for (int i = 0; i < 16; ++i) {
+          const bool on = (i & 3) + 8 * (i >> 2) >= lim;
+          x.st[i] = on ? x.st[i] : -INFINITY;
+          x.dp[i] = on ? x.dp[i] : 0.f;
         }
       }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
+    };
+    auto probs = [&](Block& x) {                       // P and dS in place of them
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x.st[i] = __builtin_amdgcn_exp2f(x.st[i] * c);
+        x.dp[i] *= x.st[i];
+      }
+    };
+    auto sums = [&](const Block& x) {
+      uint32_t pk[8], dsk[8];
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        pk[i >> 1] = pack_bf16(x.st[i], x.st[i + 1]);
+        dsk[i >> 1] = pack_bf16(x.dp[i], x.dp[i + 1]);
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt) {
+          dv[dt] = mfma(x.d[2 * t + dt], p_frag(pk, t), dv[dt]);
+          dk[dt] = mfma(x.q[2 * t + dt], p_frag(dsk, t), dk[dt]);
+        }
+    };
+    // a phase: `reads` LDS reads, then eight products between the other block's exponentials
+    auto mix = [](auto reads) {
+      __builtin_amdgcn_sched_group_barrier(0x100, decltype(reads)::value, 0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x400, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+      }
+    };
+    if constexpr (EDGE) {
+      // one block after the other, where some query sees some key of the wave
+#pragma unroll
+      for (int r = 0; r <= kApart; r += kApart) {
+        if (i1 + ra + r + 31 < kw - off) continue;
+        Block x;
+        read_rows(r, x);
+        scores(r, x);
+        __builtin_amdgcn_sched_barrier(0);
+        bad |= has_nonfinite(ad, atQ + r * 128) | has_nonfinite(ad, atD + r * 128);
+        __builtin_amdgcn_sched_barrier(0);
+        read_columns(r, x);
+        probs(x);
+        sums(x);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      Block x, y;
+      read_rows(0, x);
+      __builtin_amdgcn_sched_barrier(0);
+      read_rows(kApart, y);
+      scores(0, x);
+      __builtin_amdgcn_sched_barrier(0);
+      read_columns(0, x);
+      scores(kApart, y);
+      probs(x);
+      mix(std::integral_constant<int, 16>{});
+      __builtin_amdgcn_sched_barrier(0);
+      read_columns(kApart, y);
+      sums(x);
+      probs(y);
+      mix(std::integral_constant<int, 16>{});
+      __builtin_amdgcn_sched_barrier(0);
+      sums(y);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    cur ^= 1;
+  };
+  const int i_edge = CAUSAL ? min(s.lq, key0 + 32 * KW - 1 - off) : i_first;   // from here on all keys are seen
+  for (int g = g0; any && g < g1; ++g) {
+    int i1 = i_first;
+    if (CAUSAL)
+      for (; i1 < i_edge; i1 += RT) tile_step(i1, std::true_type{});
+    for (; i1 < s.lq; i1 += RT) tile_step(i1, std::false_type{});
+  }
   if (CAUSAL && __ballot(bad) != 0) {
     for (int i = 0; i < 16; ++i) dk[0][i] = dk[1][i] = dv[0][i] = dv[1][i] = 0.f;
-    const Args& w = again();
+    ConstArgs* w = again();
     for (int g = g0; g < g1; ++g) {
-      const int h = hk * w.G + g;
+      const int h = hk * w->G + g;
 #pragma clang loop unroll(disable)
       for (int i = i_first; i < s.lq; ++i) {
         if (KW == 2 && ((i - i_first) >> 5 & 1) != qh) continue;      // the other waves' rows
-        const bf16_t* qr = w.q + (s.q0 + i) * w.q_t + h * w.q_h;
-        const bf16_t* dr = w.dout + (s.q0 + i) * w.d_t + h * w.d_h;
+        const bf16_t* qr = w->q + (s.q0 + i) * w->q_t + h * w->q_h;
+        const bf16_t* dr = w->dout + (s.q0 + i) * w->d_t + h * w->d_h;
         const float x = dot_row(qr, kf, hh), y = dot_row(dr, vf, hh);
         if (i >= key - off) {
-          const int64_t st = (int64_t)h * w.Tq + s.q0 + i;
-          const float p = __builtin_amdgcn_exp2f((x + w.nlse[st]) * c);
+          const int64_t st = (int64_t)h * w->Tq + s.q0 + i;
+          const float p = __builtin_amdgcn_exp2f((x + w->nlse[st]) * c);
           add_row(dv, p, dr, hh);
-          add_row(dk, p * (y + w.ndelta[st]), qr, hh);
+          add_row(dk, p * (y + w->ndelta[st]), qr, hh);
         }
       }
     }
@@ -1053,10 +1189,13 @@ __global__ __launch_bounds__(256) void k_attnp_sum(const Args a) {
 inline int64_t row_tiles(const i2pc_attn_packed_desc& d, int rows) {
   return (int64_t)d.total_q * (d.heads / d.kv_heads) / rows + d.batch + (d.zero_tail ? 1 : 0);
 }
-// Waves over the keys of a tile (the kernels' KW): two while 128-row workgroups would not fill the chip's 768 places twice.
-// Measured forward, KW 1 / 2: 7200 tokens of six heads (372 workgroups) 38 / 32 us, 8700 causal rows of 16 heads over 4
-// (1000) 80 / 71 us, 12000 of twelve heads (1250) 65 / 67 us, 32 x 577 of 16 heads (2800) 75 / 95 us.
-inline int key_waves(const i2pc_attn_packed_desc& d) { return row_tiles(d, kRows) * d.kv_heads < 1200 ? 2 : 1; }
+// Waves over the keys of a tile (the kernels' KW): two while there are few 128-row workgroups for the chip's 1024 places,
+// or not many of the different lengths that a causal mask gives them.  Measured forward, KW 1 / 2: 7200 tokens of six
+// heads (380 workgroups) 38 / 31 us, 9400 of twelve heads (1010) 62 / 65 us; causal, 16 heads over 4, 7300 tokens (940)
+// 76 / 65 us, 8700 tokens (1110) 112 / 108 us.
+inline int key_waves(const i2pc_attn_packed_desc& d) {
+  return row_tiles(d, kRows) * d.kv_heads < (d.causal ? 1200 : 700) ? 2 : 1;
+}
 
 // Sequences of 32 packed rows or fewer on average take the kernel for few rows.  (Right for any lengths: the rule only
 // decides the speed.)

@@ -91,14 +91,41 @@ __device__ __forceinline__ int find_tile(const int32_t* cu, int total, int mult,
 struct Seq {
   int q0, lq, k0, lk;
 };
-__device__ __forceinline__ Seq sequence(const Args& a, int b) {
-  Seq s;
+// The sequence b and the tile within it that index t of a grid over `cu` (cu_q, or cu_k with BY_KEY) stands for; b = B: the
+// rows behind the last sequence (zero_tail).  Up to 64 sequences everything is read at once, a sequence to a lane.
+template <bool BY_KEY>
+__device__ __forceinline__ int locate(const Args& a, int mult, int rows, int t, int lane, int& tile, Seq& s) {
+  const int32_t* cu = BY_KEY ? a.cu_k : a.cu_q;
+  const int total = BY_KEY ? a.Tk : a.Tq;
+  if (a.B <= 64) {
+    const int i = min(lane, a.B - 1);
+    const int q0 = i ? min(max(a.cu_q[i], 0), a.Tq) : 0, q1 = min(max(a.cu_q[i + 1], 0), a.Tq);
+    const int k0 = i ? min(max(a.cu_k[i], 0), a.Tk) : 0, k1 = min(max(a.cu_k[i + 1], 0), a.Tk);
+    const int most = a.k_lens ? max(0, a.k_lens[i]) : INT_MAX;
+    const int f = (BY_KEY ? k0 : q0) * mult / rows + i;
+    if (a.zero_tail) {
+      const int end = __builtin_amdgcn_readlane(BY_KEY ? k1 : q1, a.B - 1) * mult / rows + a.B;
+      if (t >= end) {
+        tile = t - end;
+        return a.B;
+      }
+    }
+    const int b = max(__popcll(__ballot(lane < a.B && f <= t)) - 1, 0);
+    tile = t - __builtin_amdgcn_readlane(f, b);
+    s.q0 = __builtin_amdgcn_readlane(q0, b);
+    s.lq = __builtin_amdgcn_readlane(max(0, q1 - q0), b);
+    s.k0 = __builtin_amdgcn_readlane(k0, b);
+    s.lk = __builtin_amdgcn_readlane(min(max(0, k1 - k0), most), b);
+    return b;
+  }
+  const int b = find_tile(cu, total, mult, rows, a.B + a.zero_tail, t, lane, tile);
+  if (b == a.B) return b;
   s.q0 = __builtin_amdgcn_readfirstlane(cu_at(a.cu_q, b, a.Tq));
   s.lq = max(0, __builtin_amdgcn_readfirstlane(cu_at(a.cu_q, b + 1, a.Tq)) - s.q0);
   s.k0 = __builtin_amdgcn_readfirstlane(cu_at(a.cu_k, b, a.Tk));
   s.lk = max(0, __builtin_amdgcn_readfirstlane(cu_at(a.cu_k, b + 1, a.Tk)) - s.k0);
   if (a.k_lens) s.lk = min(s.lk, max(0, __builtin_amdgcn_readfirstlane(a.k_lens[b])));
-  return s;
+  return b;
 }
 
 // ------------------------------------------------------------------ tiles in LDS
@@ -309,6 +336,12 @@ __device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const Lan
   f32x16 st;
 #pragma unroll
   for (int t = 0; t < 4; ++t) st = mfma(kf[t], qf[t], t == 0 ? f32x16{} : st);
+  // V's columns are on their way while the exponentials are taken
+  bf16x8 vf[2][2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) vf[t][dt] = ad.columns(dt, atV + 2048 * t);
   if (partial) {
     const int lim = whole(left - 4 * hh);
 #pragma unroll
@@ -351,11 +384,6 @@ __device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const Lan
     probs();
   }
   w.l += ls;
-  bf16x8 vf[2][2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int dt = 0; dt < 2; ++dt) vf[t][dt] = ad.columns(dt, atV + 2048 * t);
   if (CAUSAL && partial) w.bad |= has_nonfinite(ad, atV);
 #pragma unroll
   for (int t = 0; t < 2; ++t)
@@ -408,13 +436,13 @@ __global__ __launch_bounds__(256, 4) void k_attnp_fwd(const Args a) {
   if (SPLIT) rest /= a.nsplit;
   const int tiles = gridDim.x / (a.Hk * (SPLIT ? a.nsplit : 1));
   int tile;
-  const int b = find_tile(a.cu_q, a.Tq, a.G, kWgRows, a.B + a.zero_tail, tiles - 1 - rest, lane, tile);
+  Seq s;
+  const int b = locate<false>(a, a.G, kWgRows, tiles - 1 - rest, lane, tile, s);
   if (b == a.B) {                                    // the rows behind the last sequence
     const int t0 = cu_at(a.cu_q, a.B, a.Tq);
     if (!SPLIT) zero_rows(a.out, a.o_t, a.o_h, t0, tile * kWgRows, min((tile + 1) * kWgRows, (a.Tq - t0) * a.G), hk, a.G, a.lse, a.H);
     return;
   }
-  const Seq s = sequence(a, b);
   const int R = s.lq * a.G, r0 = tile * kWgRows;
   if (r0 >= R) return;
   const int r = r0 + rw * 32 + lr, rc = min(r, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
@@ -539,13 +567,13 @@ __global__ __launch_bounds__(256, 2) void k_attnp_few(const Args a) {
   int rest = blockIdx.x / a.Hk;
   const int split = rest % a.nsplit;
   int tile;
-  const int b = find_tile(a.cu_q, a.Tq, a.G, kFew, a.B + a.zero_tail, rest / a.nsplit, lane, tile);
+  Seq s;
+  const int b = locate<false>(a, a.G, kFew, rest / a.nsplit, lane, tile, s);
   if (b == a.B) {
     const int t0 = cu_at(a.cu_q, a.B, a.Tq);
     if (split == 0 && a.nsplit == 1) zero_rows(a.out, a.o_t, a.o_h, t0, tile * kFew, min((tile + 1) * kFew, (a.Tq - t0) * a.G), hk, a.G, a.lse, a.H);
     return;
   }
-  const Seq s = sequence(a, b);
   const int R = s.lq * a.G, r0 = tile * kFew;
   if (r0 >= R) return;
   const int rc = min(r0 + lr, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
@@ -709,33 +737,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_attnp_join(const Args
 }
 
 // ------------------------------------------------------------------ backward
-// nlse = -lse / scale (a row that saw nothing: -inf, so that its probabilities are 0) and ndelta = -D, both [H][Tq]:
-// 8 lanes a row.
-__global__ __launch_bounds__(256) void k_attnp_delta(const Args a) {
-  const int64_t n = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
-  if (n >= (int64_t)a.Tq * a.H) return;
-  const int t = (int)(n / a.H), h = (int)(n - (int64_t)t * a.H), ch = threadIdx.x & 7;
-  const uint4 x = *reinterpret_cast<const uint4*>(a.dout + t * a.d_t + h * a.d_h + ch * 8);
-  const uint4 y = *reinterpret_cast<const uint4*>(a.out + t * a.o_t + h * a.o_h + ch * 8);
-  const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-  float d = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    d = fmaf(__uint_as_float(xs[i] << 16), __uint_as_float(ys[i] << 16), d);
-    d = fmaf(__uint_as_float(xs[i] & 0xffff0000u), __uint_as_float(ys[i] & 0xffff0000u), d);
-  }
-  d += __shfl_xor(d, 1);
-  d += __shfl_xor(d, 2);
-  d += __shfl_xor(d, 4);
-  if (ch == 0) {
-    const float lse = a.lse[n];
-    a.nlse[(int64_t)h * a.Tq + t] = lse == -INFINITY ? -INFINITY : -lse / a.scale;
-    a.ndelta[(int64_t)h * a.Tq + t] = lse == -INFINITY ? 0.f : -d;
-  }
-}
-
 // dQ: the forward's rows and tiles; per 32 keys S^T = K Q^T and dP^T = V dO^T (which starts at -D), then
-// dQ^T += K^T dS^T.  KW 2 as in the forward pass.
+// dQ^T += K^T dS^T.  KW 2 as in the forward pass.  D = rowsum(dO O) is taken on the way from the rows that the kernel holds
+// anyway, and left for the dK / dV kernel: ndelta = -D, nlse = -lse / scale (-inf for a row that saw nothing, so that its
+// probabilities are 0), both [H][Tq].
 template <bool CAUSAL, int KW>
 __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
   constexpr int kWgRows = kRows / KW;
@@ -745,13 +750,13 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
   const int rw = KW == 2 ? wid & 1 : wid, kw = KW == 2 ? wid >> 1 : 0;
   const int hk = blockIdx.x % a.Hk, tiles = gridDim.x / a.Hk;
   int tile;
-  const int b = find_tile(a.cu_q, a.Tq, a.G, kWgRows, a.B + a.zero_tail, tiles - 1 - (int)(blockIdx.x / a.Hk), lane, tile);
+  Seq s;
+  const int b = locate<false>(a, a.G, kWgRows, tiles - 1 - (int)(blockIdx.x / a.Hk), lane, tile, s);
   if (b == a.B) {
     const int t0 = cu_at(a.cu_q, a.B, a.Tq);
     zero_rows(a.dq, a.dq_t, a.dq_h, t0, tile * kWgRows, min((tile + 1) * kWgRows, (a.Tq - t0) * a.G), hk, a.G, nullptr, 0);
     return;
   }
-  const Seq s = sequence(a, b);
   const int R = s.lq * a.G, r0 = tile * kWgRows;
   if (r0 >= R) return;
   const int r = r0 + rw * 32 + lr, rc = min(r, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
@@ -781,13 +786,22 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
     qf[t] = *reinterpret_cast<const bf16x8*>(qr + 16 * t + 8 * hh);
     df[t] = *reinterpret_cast<const bf16x8*>(dr + 16 * t + 8 * hh);
   }
-  const float c = a.c, nl = a.nlse[(int64_t)h * a.Tq + s.q0 + qi] * c;
+  const float c = a.c;
+  float nl;
   f32x16 nd, dq[2];
   {
-    const float d = a.ndelta[(int64_t)h * a.Tq + s.q0 + qi];
+    const float d = dot_row(a.out + (s.q0 + qi) * a.o_t + h * a.o_h, df, hh), lse = a.lse[(int64_t)(s.q0 + qi) * a.H + h];
+    const bool none = lse == -INFINITY;
+    const float neg = none ? -INFINITY : -lse / a.scale;
+    nl = neg * c;
     for (int i = 0; i < 16; ++i) {
-      nd[i] = d;
+      nd[i] = none ? 0.f : -d;
       dq[0][i] = dq[1][i] = 0.f;
+    }
+    if (r < R && kw == 0 && hh == 0) {
+      const int64_t at = (int64_t)h * a.Tq + s.q0 + qi;
+      a.nlse[at] = neg;
+      a.ndelta[at] = nd[0];
     }
   }
   __builtin_amdgcn_s_waitcnt(0xF70);
@@ -883,7 +897,8 @@ __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
   const int split = rest % a.nsplit;
   rest /= a.nsplit;
   int tile;
-  const int b = find_tile(a.cu_k, a.Tk, 1, 32 * KW, a.B + a.zero_tail, rest, lane, tile);
+  Seq s;
+  const int b = locate<true>(a, 1, 32 * KW, rest, lane, tile, s);
   if (b == a.B) {
     const int t0 = cu_at(a.cu_k, a.B, a.Tk);
     for (int e = threadIdx.x; a.nsplit == 1 && e < 32 * KW * 8; e += 256) {
@@ -894,7 +909,6 @@ __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
     }
     return;
   }
-  const Seq s = sequence(a, b);
   const int key0 = tile * 32 * KW;
   if (key0 >= s.lk) return;
   const int kw = key0 + 32 * kh;                       // the wave's first key
@@ -1209,7 +1223,7 @@ inline int splits(const i2pc_attn_packed_desc& d) {
   if (d.total_k == 0) return 1;
   const bool few = few_rows(d);
   const int64_t tiles = row_tiles(d, few ? kFew : kRows / 2) * d.kv_heads;
-  const int64_t most = few ? (d.total_k + 1023) / 1024 : (d.total_k + 255) / 256;
+  const int64_t most = few ? (d.total_k + 2047) / 2048 : (d.total_k + 255) / 256;
   const int64_t want = few ? 2048 / tiles : key_waves(d) == 1 || tiles >= 512 ? 1 : 1024 / tiles;
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 512}));
 }
@@ -1362,7 +1376,6 @@ extern "C" int i2pc_attention_packed_backward(const i2pc_attn_packed_grad_desc* 
   hipStream_t s = as_stream(stream);
   const dim3 block(256);
   if (a.Tq > 0) {
-    hipLaunchKernelGGL(attnp::k_attnp_delta, dim3((uint32_t)(((int64_t)a.Tq * a.H + 31) / 32)), block, 0, s, a);
     const int kw = attnp::key_waves(d);
     const dim3 grid((uint32_t)(attnp::row_tiles(d, attnp::kRows / kw) * a.Hk));
     if (kw == 1 && d.causal) hipLaunchKernelGGL((attnp::k_attnp_dq<true, 1>), grid, block, 0, s, a);

@@ -92,8 +92,10 @@ struct Seq {
   int q0, lq, k0, lk;
 };
 // The sequence b and the tile within it that index t of a grid over `cu` (cu_q, or cu_k with BY_KEY) stands for; b = B: the
-// rows behind the last sequence (zero_tail).  Up to 64 sequences everything is read at once, a sequence to a lane.
-template <bool BY_KEY>
+// rows behind the last sequence (zero_tail); tile < 0: nothing.  Up to 64 sequences everything is read at once, a sequence
+// to a lane.  LONGEST: of up to 16 sequences those with the most keys come first, so that what ends last is short (ten
+// images of 1 to 2305 tokens, twelve heads: 60 -> 56 us; the pass over the lengths costs more than that for 32 or 64).
+template <bool BY_KEY, bool LONGEST>
 __device__ __forceinline__ int locate(const Args& a, int mult, int rows, int t, int lane, int& tile, Seq& s) {
   const int32_t* cu = BY_KEY ? a.cu_k : a.cu_q;
   const int total = BY_KEY ? a.Tk : a.Tq;
@@ -102,20 +104,38 @@ __device__ __forceinline__ int locate(const Args& a, int mult, int rows, int t, 
     const int q0 = i ? min(max(a.cu_q[i], 0), a.Tq) : 0, q1 = min(max(a.cu_q[i + 1], 0), a.Tq);
     const int k0 = i ? min(max(a.cu_k[i], 0), a.Tk) : 0, k1 = min(max(a.cu_k[i + 1], 0), a.Tk);
     const int most = a.k_lens ? max(0, a.k_lens[i]) : INT_MAX;
-    const int f = (BY_KEY ? k0 : q0) * mult / rows + i;
-    if (a.zero_tail) {
-      const int end = __builtin_amdgcn_readlane(BY_KEY ? k1 : q1, a.B - 1) * mult / rows + a.B;
-      if (t >= end) {
-        tile = t - end;
-        return a.B;
+    const int lq = max(0, q1 - q0), lk = min(max(0, k1 - k0), most);
+    int b;
+    if (LONGEST && a.B <= 16) {
+      const int n = lane < a.B ? ((BY_KEY ? lk : lq) * mult + rows - 1) / rows : 0;    // the lane's tiles
+      int first = 0, all = 0;
+      for (int j = 0; j < a.B; ++j) {
+        const int nj = __builtin_amdgcn_readlane(n, j), cj = __builtin_amdgcn_readlane(lk, j);
+        first += cj > lk || (cj == lk && j < lane) ? nj : 0;
+        all += nj;
       }
+      if (t >= all) {
+        tile = a.zero_tail ? t - all : -1;
+        return a.zero_tail ? a.B : 0;
+      }
+      b = max((int)__ffsll((unsigned long long)__ballot(t >= first && t < first + n)) - 1, 0);
+      tile = t - __builtin_amdgcn_readlane(first, b);
+    } else {
+      const int f = (BY_KEY ? k0 : q0) * mult / rows + i;
+      if (a.zero_tail) {
+        const int end = __builtin_amdgcn_readlane(BY_KEY ? k1 : q1, a.B - 1) * mult / rows + a.B;
+        if (t >= end) {
+          tile = t - end;
+          return a.B;
+        }
+      }
+      b = max(__popcll(__ballot(lane < a.B && f <= t)) - 1, 0);
+      tile = t - __builtin_amdgcn_readlane(f, b);
     }
-    const int b = max(__popcll(__ballot(lane < a.B && f <= t)) - 1, 0);
-    tile = t - __builtin_amdgcn_readlane(f, b);
     s.q0 = __builtin_amdgcn_readlane(q0, b);
-    s.lq = __builtin_amdgcn_readlane(max(0, q1 - q0), b);
+    s.lq = __builtin_amdgcn_readlane(lq, b);
     s.k0 = __builtin_amdgcn_readlane(k0, b);
-    s.lk = __builtin_amdgcn_readlane(min(max(0, k1 - k0), most), b);
+    s.lk = __builtin_amdgcn_readlane(lk, b);
     return b;
   }
   const int b = find_tile(cu, total, mult, rows, a.B + a.zero_tail, t, lane, tile);
@@ -429,7 +449,7 @@ __global__ __launch_bounds__(256, 4) void k_attnp_fwd(const Args a) {
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rw = KW == 2 ? wid & 1 : wid, kw = KW == 2 ? wid >> 1 : 0;
   // key heads fastest: workgroups b and b + 8 share an XCD, so with 8 heads (4, 2) each XCD (pair, four) keeps to
-  // one head's keys; later tiles, which a causal mask leaves the most keys, come first
+  // one head's keys; with a causal mask later tiles, which have the most keys, come first
   const int hk = blockIdx.x % a.Hk;
   int rest = blockIdx.x / a.Hk;
   const int split = SPLIT ? rest % a.nsplit : 0;
@@ -437,14 +457,14 @@ __global__ __launch_bounds__(256, 4) void k_attnp_fwd(const Args a) {
   const int tiles = gridDim.x / (a.Hk * (SPLIT ? a.nsplit : 1));
   int tile;
   Seq s;
-  const int b = locate<false>(a, a.G, kWgRows, tiles - 1 - rest, lane, tile, s);
+  const int b = locate<false, !CAUSAL>(a, a.G, kWgRows, CAUSAL ? tiles - 1 - rest : rest, lane, tile, s);
   if (b == a.B) {                                    // the rows behind the last sequence
     const int t0 = cu_at(a.cu_q, a.B, a.Tq);
     if (!SPLIT) zero_rows(a.out, a.o_t, a.o_h, t0, tile * kWgRows, min((tile + 1) * kWgRows, (a.Tq - t0) * a.G), hk, a.G, a.lse, a.H);
     return;
   }
   const int R = s.lq * a.G, r0 = tile * kWgRows;
-  if (r0 >= R) return;
+  if (tile < 0 || r0 >= R) return;
   const int r = r0 + rw * 32 + lr, rc = min(r, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
   const int nk = seen(CAUSAL, qi, s);
   // first and last row of the wave, last row of the tile (uniform)
@@ -568,14 +588,14 @@ __global__ __launch_bounds__(256, 2) void k_attnp_few(const Args a) {
   const int split = rest % a.nsplit;
   int tile;
   Seq s;
-  const int b = locate<false>(a, a.G, kFew, rest / a.nsplit, lane, tile, s);
+  const int b = locate<false, false>(a, a.G, kFew, rest / a.nsplit, lane, tile, s);
   if (b == a.B) {
     const int t0 = cu_at(a.cu_q, a.B, a.Tq);
     if (split == 0 && a.nsplit == 1) zero_rows(a.out, a.o_t, a.o_h, t0, tile * kFew, min((tile + 1) * kFew, (a.Tq - t0) * a.G), hk, a.G, a.lse, a.H);
     return;
   }
   const int R = s.lq * a.G, r0 = tile * kFew;
-  if (r0 >= R) return;
+  if (tile < 0 || r0 >= R) return;
   const int rc = min(r0 + lr, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
   const int nk = seen(CAUSAL, qi, s), nk_first = seen(CAUSAL, r0 / a.G, s);
   int ke = seen(CAUSAL, (min(r0 + kFew, R) - 1) / a.G, s);
@@ -748,17 +768,17 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
   const int lane = threadIdx.x & 63, hh = lane >> 5, lr = lane & 31;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rw = KW == 2 ? wid & 1 : wid, kw = KW == 2 ? wid >> 1 : 0;
-  const int hk = blockIdx.x % a.Hk, tiles = gridDim.x / a.Hk;
+  const int hk = blockIdx.x % a.Hk, rest = blockIdx.x / a.Hk, tiles = gridDim.x / a.Hk;
   int tile;
   Seq s;
-  const int b = locate<false>(a, a.G, kWgRows, tiles - 1 - (int)(blockIdx.x / a.Hk), lane, tile, s);
+  const int b = locate<false, !CAUSAL>(a, a.G, kWgRows, CAUSAL ? tiles - 1 - rest : rest, lane, tile, s);
   if (b == a.B) {
     const int t0 = cu_at(a.cu_q, a.B, a.Tq);
     zero_rows(a.dq, a.dq_t, a.dq_h, t0, tile * kWgRows, min((tile + 1) * kWgRows, (a.Tq - t0) * a.G), hk, a.G, nullptr, 0);
     return;
   }
   const int R = s.lq * a.G, r0 = tile * kWgRows;
-  if (r0 >= R) return;
+  if (tile < 0 || r0 >= R) return;
   const int r = r0 + rw * 32 + lr, rc = min(r, R - 1), qi = rc / a.G, h = hk * a.G + rc - qi * a.G;
   const int nk = seen(CAUSAL, qi, s);
   const int w0 = min(r0 + rw * 32, R - 1);
@@ -898,7 +918,7 @@ __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
   rest /= a.nsplit;
   int tile;
   Seq s;
-  const int b = locate<true>(a, 1, 32 * KW, rest, lane, tile, s);
+  const int b = locate<true, false>(a, 1, 32 * KW, rest, lane, tile, s);
   if (b == a.B) {
     const int t0 = cu_at(a.cu_k, a.B, a.Tk);
     for (int e = threadIdx.x; a.nsplit == 1 && e < 32 * KW * 8; e += 256) {
@@ -910,7 +930,7 @@ __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
     return;
   }
   const int key0 = tile * 32 * KW;
-  if (key0 >= s.lk) return;
+  if (tile < 0 || key0 >= s.lk) return;
   const int kw = key0 + 32 * kh;                       // the wave's first key
   const int key = kw + lr, kc = min(key, s.lk - 1);
   // causal: key j is seen by the queries from j - (lk - lq) on

@@ -11,6 +11,9 @@
 // same read: a wave keeps the partial sums of its columns in registers over all the rows it takes, a
 // workgroup adds its waves' through LDS and writes one partial row, and k_lnt_cols adds the partial rows
 // -- fixed assignment and order, so the result does not change from run to run (no atomics).
+// Measured: 18464 x 1024 fp32 forward 24.5 us (4.6 TB/s), backward with add 54 us (4.9 TB/s; a copy of 2 GiB
+// reaches 4.9), the partial rows' sum 3 us of it; 4099 x 1111 bf16 8.1 and 16.7 us (its rows start at odd
+// addresses); 5 x 384: the launches.
 #include "common.h"
 
 #include <algorithm>
@@ -22,11 +25,23 @@ typedef uint16_t bf16_t;
 
 constexpr int kThreads = 512;                 // 8 waves
 constexpr int kMaxDim = 8192;
-constexpr int kMaxGroups = 512;               // two workgroups of 8 waves on each of 256 CUs
+constexpr int kCUs = 256;
 
+// The sum over a wave, in every lane: four DPP additions within 16 lanes, two swaps of rows -- all on the vector unit, where
+// shuffles through LDS would add their latency six times to every row sum.
+template <int CTRL>
+__device__ __forceinline__ float plus_dpp(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float wave_sum(float x) {
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-  return x;
+  x = plus_dpp<0xB1>(x);                           // quad_perm 1, 0, 3, 2
+  x = plus_dpp<0x4E>(x);                           // quad_perm 2, 3, 0, 1
+  x = plus_dpp<0x141>(x);                          // row_half_mirror
+  x = plus_dpp<0x140>(x);                          // row_mirror
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
 
 // E consecutive elements as floats, from / to an address with the element's own alignment only (rows of
@@ -77,10 +92,26 @@ struct Packed {
   }
 };
 
+// E values of T as they are in memory
+template <int E>
+struct Floats {
+  float v[E];
+  __device__ __forceinline__ void load(const float* p) { __builtin_memcpy(v, p, E * 4); }
+  __device__ __forceinline__ float operator[](int j) const { return v[j]; }
+};
+template <typename T, int E>
+struct Raw {
+  typedef Packed<E> type;
+};
+template <int E>
+struct Raw<float, E> {
+  typedef Floats<E> type;
+};
+
 // A row's columns over WPR waves: chunk i of a lane starts at column (i * 64 * WPR + wave * 64 + lane) * E.
 // The last chunk of a row whose width is no multiple of E starts at dim - E instead and repeats columns of
-// the chunk before it: every load is a whole vector, `live` keeps the repeated columns out of the row
-// sums, and what is stored for them is stored twice with the same value.
+// the chunk before it: every load is a whole vector, and `live` keeps the repeated columns out of the row
+// sums.  The forward pass stores them twice with the same value.
 template <int E, int V, int WPR>
 struct Cols {
   int col[V];
@@ -96,30 +127,41 @@ struct Cols {
   __device__ __forceinline__ bool live(int i, int j) const { return (uint32_t)j >= first[i]; }
 };
 
-// sum of a over the row's WPR waves (every lane gets it)
+// Sums over the row's WPR waves, in every lane of them.  The waves' parts meet in LDS, in one of two slots in turn: a wave
+// that writes a slot again has passed the other slot's barrier, which no wave reaches before it has read the first.
 template <int WPR>
-__device__ __forceinline__ float row_sum(float a, float* red, int wave) {
-  a = wave_sum(a);
-  if constexpr (WPR > 1) {
-    __syncthreads();                               // the slots' last readers are done
-    if ((threadIdx.x & 63) == 0) red[wave] = a;
-    __syncthreads();
-    const int w0 = wave / WPR * WPR;
-    a = 0.f;
+struct RowSum {
+  float2 (*slot)[8];
+  int wave, turn;
+  __device__ __forceinline__ float2 operator()(float a, float b) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if constexpr (WPR > 1) {
+      if ((threadIdx.x & 63) == 0) slot[turn][wave] = make_float2(a, b);
+      __syncthreads();
+      const int w0 = wave / WPR * WPR;
+      a = b = 0.f;
 #pragma unroll
-    for (int w = 0; w < WPR; ++w) a += red[w0 + w];
+      for (int w = 0; w < WPR; ++w) {
+        const float2 x = slot[turn][w0 + w];
+        a += x.x;
+        b += x.y;
+      }
+      turn ^= 1;
+    }
+    return make_float2(a, b);
   }
-  return a;
-}
+};
 
 // One row per WPR waves of a workgroup of four waves (eight for the widest rows).
 template <typename T, int E, int V, int WPR>
 __global__ __launch_bounds__(WPR == 8 ? 512 : 256) void k_lnt_fwd(const T* __restrict__ x, int64_t ldx, const float* __restrict__ gamma,
                                                  const float* __restrict__ beta, float eps, int rows, int dim,
                                                  bf16_t* __restrict__ y, int64_t ldy, float2* __restrict__ stats) {
-  __shared__ float red[8];
+  __shared__ float2 red[2][8];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // scalar row addresses
   const Cols<E, V, WPR> c(lane, wave % WPR, dim);
+  RowSum<WPR> row_sum{red, wave, 0};
   constexpr int R = WPR == 1 ? 4 : 1;              // WPR > 1: one row a workgroup, all its waves or none
   for (int64_t row = (int64_t)blockIdx.x * R + (WPR == 1 ? wave : 0); row < rows; row += (int64_t)gridDim.x * R) {
     const T* xr = x + row * ldx;
@@ -131,7 +173,7 @@ __global__ __launch_bounds__(WPR == 8 ? 512 : 256) void k_lnt_fwd(const T* __res
     for (int i = 0; i < V; ++i)
 #pragma unroll
       for (int j = 0; j < E; ++j) s += c.live(i, j) ? v[i][j] : 0.f;
-    const float mean = row_sum<WPR>(s, red, wave) / (float)dim;
+    const float mean = row_sum(s, 0.f).x / (float)dim;
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i)
@@ -140,7 +182,7 @@ __global__ __launch_bounds__(WPR == 8 ? 512 : 256) void k_lnt_fwd(const T* __res
         v[i][j] -= mean;
         q += c.live(i, j) ? v[i][j] * v[i][j] : 0.f;
       }
-    const float rstd = 1.0f / sqrtf(row_sum<WPR>(q, red, wave) / (float)dim + eps);
+    const float rstd = 1.0f / sqrtf(row_sum(q, 0.f).x / (float)dim + eps);
     if (lane == 0 && wave % WPR == 0) stats[row] = make_float2(mean, rstd);
     bf16_t* yr = y + row * ldy;
 #pragma unroll
@@ -158,16 +200,17 @@ __global__ __launch_bounds__(WPR == 8 ? 512 : 256) void k_lnt_fwd(const T* __res
 // Rows blockIdx.x * R + k * gridDim.x * R for the R = 8 / WPR rows a workgroup takes at a time.  Partial row p of the
 // column sums goes to dgamma + p * 2 * dim and dbeta + p * 2 * dim: with one partial row, the outputs themselves.
 template <typename T, int E, int V, int WPR>
-__global__ __launch_bounds__(kThreads, 4) void k_lnt_bwd(const bf16_t* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
+__global__ __launch_bounds__(kThreads, E * V <= 8 ? 4 : 2) void k_lnt_bwd(const bf16_t* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
                                                       int64_t ldx, const float2* __restrict__ stats,
                                                       const float* __restrict__ gamma, const T* add, int64_t lda, int rows,
                                                       int dim, T* dx, int64_t lddx, float* __restrict__ dgamma,
                                                       float* __restrict__ dbeta) {
-  __shared__ float red[8];
+  __shared__ float2 red[2][8];
   extern __shared__ float sums[];                  // [2][dim] (R > 1)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // scalar row addresses
   constexpr int R = 8 / WPR;
   const Cols<E, V, WPR> c(lane, wave % WPR, dim);
+  RowSum<WPR> row_sum{red, wave, 0};
   float g[V][E], dg[V][E], db[V][E];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -176,31 +219,49 @@ __global__ __launch_bounds__(kThreads, 4) void k_lnt_bwd(const bf16_t* __restric
     for (int j = 0; j < E; ++j) dg[i][j] = db[i][j] = 0.f;
   }
   const float inv = 1.0f / (float)dim;
-  // WPR > 1 meets barriers inside: every wave runs the same number of rounds
-  for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < rows; row0 += (int64_t)gridDim.x * R) {
-    const int64_t row = row0 + wave / WPR;
-    const bool on = row < rows;
-    if (WPR == 1 && !on) break;
-    const int64_t rc = on ? row : rows - 1;
-    float xv[V][E], av[V][E];
-    Packed<E> gy[V];
+  // A row as it is read.  AHEAD: the next row's loads go out before this row's sums (where the registers allow it)
+  struct Row {
+    typename Raw<T, E>::type x[V], a[V];
+    Packed<E> dy[V];
+    float2 st;
+  };
+  constexpr bool AHEAD = E * V <= 8;
+  auto load = [&](int64_t row, Row& w) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      Vec<T, E>::load(x + rc * ldx + c.col[i], xv[i]);
-      gy[i].load(dy + rc * lddy + c.col[i]);
+      w.x[i].load(x + row * ldx + c.col[i]);
+      w.dy[i].load(dy + row * lddy + c.col[i]);
     }
     if (add) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) Vec<T, E>::load(add + rc * lda + c.col[i], av[i]);
+      for (int i = 0; i < V; ++i) w.a[i].load(add + row * lda + c.col[i]);
     }
-    const float2 st = stats[rc];
+    w.st = stats[row];
+  };
+  // WPR > 1 meets barriers inside: every wave runs the same number of rounds
+  const int64_t step = (int64_t)gridDim.x * R;
+  Row next;
+  const int64_t row0 = (int64_t)blockIdx.x * R, mine = row0 + wave / WPR;
+  if (AHEAD && row0 < rows) load(min(mine, (int64_t)rows - 1), next);
+  for (int64_t at = row0; at < rows; at += step) {
+    const int64_t row = at + wave / WPR;
+    const bool on = row < rows;
+    if (WPR == 1 && !on) break;
+    Row w;
+    if (AHEAD) {
+      w = next;
+      if (at + step < rows) load(min(row + step, (int64_t)rows - 1), next);
+    } else {
+      load(on ? row : (int64_t)rows - 1, w);
+    }
+    const float2 st = w.st;
     float a = 0.f, b = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const float h = (xv[i][j] - st.x) * st.y, d = gy[i][j], gd = d * g[i][j];
-        xv[i][j] = h;
+        const float h = (w.x[i][j] - st.x) * st.y, d = w.dy[i][j], gd = d * g[i][j];
+        if constexpr (sizeof(T) == 4) w.x[i].v[j] = h;
         a += c.live(i, j) ? gd : 0.f;
         b += c.live(i, j) ? gd * h : 0.f;
         if (WPR == 1 || on) {
@@ -208,19 +269,34 @@ __global__ __launch_bounds__(kThreads, 4) void k_lnt_bwd(const bf16_t* __restric
           db[i][j] += d;
         }
       }
-    a = row_sum<WPR>(a, red, wave) * inv;
-    b = row_sum<WPR>(b, red, wave) * inv;
+    const float2 ab = row_sum(a, b);
+    a = ab.x * inv;
+    b = ab.y * inv;
     if (WPR == 1 || on) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         float o[E];
-        gy[i].renew();
+        w.dy[i].renew();
+        if constexpr (sizeof(T) == 2) w.x[i].renew();
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          o[j] = st.y * (gy[i][j] * g[i][j] - a - xv[i][j] * b);
-          if (add) o[j] += av[i][j];
+          const float h = sizeof(T) == 4 ? w.x[i][j] : (w.x[i][j] - st.x) * st.y;
+          o[j] = st.y * (w.dy[i][j] * g[i][j] - a - h * b);
+          if (add) o[j] += w.a[i][j];
         }
-        if (c.first[i] < (uint32_t)E) Vec<T, E>::store(dx + row * lddx + c.col[i], o);
+        T* to = dx + row * lddx + c.col[i];
+        if (c.first[i] == 0) {
+          Vec<T, E>::store(to, o);
+        } else if (c.first[i] < (uint32_t)E) {
+          // dx may be add, and another wave of the row may have stored the repeated columns before this one's add came:
+          // they are its alone
+#pragma unroll
+          for (int j = 1; j < E; ++j)
+            if (c.live(i, j)) {
+              const float one[1] = {o[j]};
+              Vec<T, 1>::store(to + j, one);
+            }
+        }
       }
     }
   }
@@ -282,48 +358,65 @@ __global__ __launch_bounds__(1024) void k_lnt_cols(const float* __restrict__ par
   }
 }
 
-// Workgroups (and partial rows) of the backward pass: as many as a round of R = 8 / WPR rows each takes while there
-// are few rows.
-inline int parts_for(int rows, int dim) {
-  const int r = dim <= 1024 ? 8 : dim <= 4096 ? 2 : 1;
-  return std::max(1, std::min(kMaxGroups, (rows - 1) / r + 1));
+// How a row lies in registers: E elements a load, V loads a lane, WPR waves a row -- the narrowest that holds it.
+template <int E_, int V_, int WPR_>
+struct Shape {
+  static constexpr int E = E_, V = V_, WPR = WPR_;
+};
+template <bool BACK, class F>
+auto with_shape(int dim, F f) {
+  if (dim <= 64) return f(Shape<1, 1, 1>{});
+  if (dim <= 128) return f(Shape<2, 1, 1>{});
+  if (dim <= 256) return f(Shape<4, 1, 1>{});
+  if (dim <= 384) return f(Shape<2, 3, 1>{});
+  if (dim <= 512) return f(Shape<4, 2, 1>{});
+  if constexpr (BACK) {
+    // eight columns a lane while eight waves hold the row: the backward pass holds four values and two sums a column, and
+    // with sixteen there are two waves a SIMD and no registers to read a row ahead (18464 x 1024, one wave a row: 65 us,
+    // two: 54 us; 12000 x 768 bf16 23.5 and 19.5 us)
+    if (dim <= 1024) return f(Shape<4, 2, 2>{});
+    if (dim <= 2048) return f(Shape<8, 1, 4>{});
+    if (dim <= 4096) return f(Shape<8, 1, 8>{});
+  } else {
+    if (dim <= 768) return f(Shape<4, 3, 1>{});
+    if (dim <= 1024) return f(Shape<4, 4, 1>{});
+    if (dim <= 1536) return f(Shape<8, 3, 1>{});
+    if (dim <= 2048) return f(Shape<8, 4, 1>{});
+    if (dim <= 4096) return f(Shape<8, 2, 4>{});
+  }
+  return f(Shape<8, 2, 8>{});
 }
 
-template <typename T, int E, int V, int WPR>
+// Workgroups (and partial rows) of the backward pass: as many as fit the CUs at once -- two, one of the widest shape -- or
+// as a round of 8 / WPR rows each takes while there are few rows.  (A third and a fourth workgroup a CU that wait, which
+// even out the last round, cost more in partial rows than they gave.)
+inline int parts_for(int rows, int dim) {
+  return with_shape<true>(dim, [&](auto s) {
+    typedef decltype(s) H;
+    return std::max(1, std::min(H::E * H::V <= 8 ? 2 * kCUs : kCUs, (rows - 1) / (8 / H::WPR) + 1));
+  });
+}
+
+template <typename T>
 void launch_fwd(const T* x, int64_t ldx, const float* gamma, const float* beta, float eps, int rows, int dim, bf16_t* y,
                 int64_t ldy, float2* stats, hipStream_t s) {
-  constexpr int R = WPR == 1 ? 4 : 1;
-  hipLaunchKernelGGL((k_lnt_fwd<T, E, V, WPR>), dim3(std::min((rows - 1) / R + 1, 1 << 22)), dim3(WPR == 8 ? 512 : 256), 0, s, x, ldx, gamma, beta, eps, rows,
-                     dim, y, ldy, stats);
+  with_shape<false>(dim, [&](auto h) {
+    typedef decltype(h) H;
+    constexpr int R = H::WPR == 1 ? 4 : 1;
+    hipLaunchKernelGGL((k_lnt_fwd<T, H::E, H::V, H::WPR>), dim3(std::min((rows - 1) / R + 1, 1 << 22)), dim3(H::WPR == 8 ? 512 : 256),
+                       0, s, x, ldx, gamma, beta, eps, rows, dim, y, ldy, stats);
+  });
 }
-template <typename T, int E, int V, int WPR>
-void launch_bwd(const bf16_t* dy, int64_t lddy, const T* x, int64_t ldx, const float2* stats, const float* gamma,
-                const T* add, int64_t lda, int rows, int dim, T* dx, int64_t lddx, float* dgamma, float* dbeta, hipStream_t s) {
-  hipLaunchKernelGGL((k_lnt_bwd<T, E, V, WPR>), dim3(parts_for(rows, dim)), dim3(kThreads),
-                     WPR < 8 ? 2 * dim * sizeof(float) : 0, s, dy,
-                     lddy, x, ldx, stats, gamma, add, lda, rows, dim, dx, lddx, dgamma, dbeta);
+template <typename T>
+void launch_bwd(const bf16_t* dy, int64_t lddy, const T* x, int64_t ldx, const float2* stats, const float* gamma, const T* add,
+                int64_t lda, int rows, int dim, T* dx, int64_t lddx, float* dgamma, float* dbeta, hipStream_t s) {
+  with_shape<true>(dim, [&](auto h) {
+    typedef decltype(h) H;
+    hipLaunchKernelGGL((k_lnt_bwd<T, H::E, H::V, H::WPR>), dim3(parts_for(rows, dim)), dim3(kThreads),
+                       H::WPR < 8 ? 2 * dim * sizeof(float) : 0, s, dy, lddy, x, ldx, stats, gamma, add, lda, rows, dim, dx, lddx,
+                       dgamma, dbeta);
+  });
 }
-
-// The narrowest instance that holds the row: E elements a load, V loads a lane, WPR waves a row.  The backward pass
-// holds four values and two sums a column: above 1024 a row takes four waves there, where one wave's registers would
-// leave two waves a SIMD (200 to 256 VGPRs at 1536 and 2048); the forward pass takes four above 2048.
-#define LNT_DISPATCH(FN, T, WIDE1, WIDE2, ...)         \
-  do {                                                 \
-    if (dim <= 64) FN<T, 1, 1, 1>(__VA_ARGS__);        \
-    else if (dim <= 128) FN<T, 2, 1, 1>(__VA_ARGS__);  \
-    else if (dim <= 256) FN<T, 4, 1, 1>(__VA_ARGS__);  \
-    else if (dim <= 384) FN<T, 2, 3, 1>(__VA_ARGS__);  \
-    else if (dim <= 512) FN<T, 4, 2, 1>(__VA_ARGS__);  \
-    else if (dim <= 768) FN<T, 4, 3, 1>(__VA_ARGS__);  \
-    else if (dim <= 1024) FN<T, 4, 4, 1>(__VA_ARGS__); \
-    else if (dim <= 1536) FN<T, WIDE1>(__VA_ARGS__);   \
-    else if (dim <= 2048) FN<T, WIDE2>(__VA_ARGS__);   \
-    else if (dim <= 4096) FN<T, 8, 2, 4>(__VA_ARGS__); \
-    else FN<T, 8, 2, 8>(__VA_ARGS__);                  \
-  } while (0)
-#define LNT_F1 8, 3, 1
-#define LNT_F2 8, 4, 1
-#define LNT_B 8, 1, 4
 
 }  // namespace lnt
 }  // namespace i2pc
@@ -343,9 +436,9 @@ extern "C" int i2pc_layernorm_train(const void* x, int x_f32, int64_t ldx, const
   auto* st = reinterpret_cast<float2*>(stats);
   using namespace lnt;
   if (x_f32)
-    LNT_DISPATCH(launch_fwd, float, LNT_F1, LNT_F2, static_cast<const float*>(x), ldx, gamma, beta, eps, rows, dim, yy, ldy, st, s);
+    launch_fwd(static_cast<const float*>(x), ldx, gamma, beta, eps, rows, dim, yy, ldy, st, s);
   else
-    LNT_DISPATCH(launch_fwd, bf16_t, LNT_F1, LNT_F2, static_cast<const bf16_t*>(x), ldx, gamma, beta, eps, rows, dim, yy, ldy, st, s);
+    launch_fwd(static_cast<const bf16_t*>(x), ldx, gamma, beta, eps, rows, dim, yy, ldy, st, s);
   return check_launch("layernorm_train");
 }
 
@@ -375,10 +468,10 @@ extern "C" int i2pc_layernorm_backward(const void* dy, int64_t lddy, const void*
   auto* g = static_cast<const bf16_t*>(dy);
   auto* st = reinterpret_cast<const float2*>(stats);
   if (x_f32)
-    LNT_DISPATCH(launch_bwd, float, LNT_B, LNT_B, g, lddy, static_cast<const float*>(x), ldx, st, gamma, static_cast<const float*>(add),
+    launch_bwd(g, lddy, static_cast<const float*>(x), ldx, st, gamma, static_cast<const float*>(add),
                  lda, rows, dim, static_cast<float*>(dx), lddx, pg, pb, s);
   else
-    LNT_DISPATCH(launch_bwd, bf16_t, LNT_B, LNT_B, g, lddy, static_cast<const bf16_t*>(x), ldx, st, gamma, static_cast<const bf16_t*>(add),
+    launch_bwd(g, lddy, static_cast<const bf16_t*>(x), ldx, st, gamma, static_cast<const bf16_t*>(add),
                  lda, rows, dim, static_cast<bf16_t*>(dx), lddx, pg, pb, s);
   if (need)
     hipLaunchKernelGGL(k_lnt_cols, dim3((2 * dim + 31) / 32), dim3(1024), 0, s, part, parts_for(rows, dim), dim, dgamma, dbeta);

@@ -7,7 +7,6 @@ Layouts: activations bf16 NHWC / [rows][features]; residual stream fp32.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import Optional
 
@@ -863,44 +862,56 @@ _lib.register("i2pc_gelu_fp8_backward", ctypes.c_int, [c_void_p, c_int64, c_void
                                                        c_int64, c_void_p, c_int64, c_void_p])
 
 
-def _operand(t, name, shape, dtypes, like=None):
-    """Refuses a tensor that is not on the device, not of `shape` / one of `dtypes`, or whose last axis is not
-    dense; `like`: the tensor whose device it has to share."""
-    at = t.get_device()
-    if at < 0:
+def _operand(t, name, shape, dtype, at):
+    """Refuses a tensor that is not on device `at` (any with None), not of `shape` and `dtype`, or whose last axis is not
+    dense."""
+    on = t.get_device()
+    if on < 0:
         raise _lib.I2PCError(f"{name} must be a device tensor")
-    if like is not None and at != like.get_device():
-        raise _lib.I2PCError(f"{name} is on device {at}, not on {like.get_device()}")
-    if t.dtype not in dtypes:
-        raise TypeError(f"{name}: expected {' or '.join(map(str, dtypes))}, got {t.dtype}")
+    if on != at and at is not None:
+        raise _lib.I2PCError(f"{name} is on device {on}, not on {at}")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name}: expected the shape {tuple(shape)}, got {tuple(t.shape)}")
     if shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name}: the last axis must be dense, its stride is {t.stride(-1)}")
 
 
-def _rows_dim(t, name):
+def _dense(t, name, shape, dtype, at):
+    _operand(t, name, shape, dtype, at)
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _rows_dim(t, name, dtypes):
+    """(rows, dim, row pitch) of a 2-D device tensor of one of `dtypes`; one row has no pitch of its own: its width."""
+    if t.get_device() < 0:
+        raise _lib.I2PCError(f"{name} must be a device tensor")
     if t.dim() != 2:
         raise ValueError(f"{name}: expected [rows, dim], got the shape {tuple(t.shape)}")
-    return t.shape
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: expected {' or '.join(map(str, dtypes))}, got {t.dtype}")
+    rows, dim = t.shape
+    pitch, dense = t.stride()
+    if dim > 1 and dense != 1:
+        raise ValueError(f"{name}: the last axis must be dense, its stride is {dense}")
+    return rows, dim, pitch if rows > 1 else max(pitch, dim)
 
 
 def _pitch(t):
-    """Row pitch of a 2-D tensor (one row has none of its own: its width)."""
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
 
 
-def _on_device_of(t):
-    """The device of `t` made current for a launch, where it is not already."""
-    torch = _torch()
-    at = t.get_device()
-    return contextlib.nullcontext() if at < 0 or at == torch._C._cuda_getDevice() else torch.cuda.device(at)
+def _elsewhere(at):
+    """Whether device `at` is not the current one (the call is then made again with it current)."""
+    return at >= 0 and at != _torch()._C._cuda_getDevice()
 
 
-def _launch(label, nbytes, name, t, *args):
-    """Calls the entry point on the current stream of the device of `t`, timed where a profile is taken.  (The raw
-    stream handle: building a Stream object for it costs more than the launch leaves to the host.)"""
-    stream = _torch()._C._cuda_getCurrentRawStream(t.get_device())
+def _launch(label, nbytes, name, at, *args):
+    """Calls the entry point on the current stream of device `at`, timed where a profile is taken.  (The raw stream handle:
+    building a Stream object for it costs the host as much as a launch.)"""
+    stream = _torch()._C._cuda_getCurrentRawStream(at)
     if profile is None:
         _lib.call(name, *args, stream)
         return
@@ -913,23 +924,27 @@ def layernorm_train(x, gamma, beta, eps, out=None, stats=None):
     training step: (y, stats) with y bf16 [rows, dim] and stats fp32 [rows, 2] = each row's (mean, 1 / std),
     which layernorm_backward reads.  gamma, beta: fp32 [dim].  Rows and statistics are held in fp32."""
     torch = _torch()
-    rows, dim = _rows_dim(x, "x")
-    f32 = (torch.float32,)
-    _operand(x, "x", (rows, dim), (torch.float32, torch.bfloat16))
-    _operand(gamma, "gamma", (dim,), f32, x)
-    _operand(beta, "beta", (dim,), f32, x)
-    with _on_device_of(x):
-        if out is None:
-            out = x.new_empty((rows, dim), dtype=torch.bfloat16)
-        else:
-            _operand(out, "out", (rows, dim), (torch.bfloat16,), x)
-        if stats is None:
-            stats = x.new_empty((rows, 2), dtype=torch.float32)
-        else:
-            _dense(stats, "stats", (rows, 2), x)
-        e = x.element_size()
-        _launch("k_lnt_fwd", rows * dim * (e + 2.0) + 8.0 * rows, "i2pc_layernorm_train", x, _p(x), int(e == 4), _pitch(x),
-                _p(gamma), _p(beta), eps, rows, dim, _p(out), _pitch(out), _p(stats))
+    f32, bf = torch.float32, torch.bfloat16
+    rows, dim, pitch = _rows_dim(x, "x", (f32, bf))
+    at = x.get_device()
+    if _elsewhere(at):
+        with torch.cuda.device(at):
+            return layernorm_train(x, gamma, beta, eps, out, stats)
+    _operand(gamma, "gamma", (dim,), f32, at)
+    _operand(beta, "beta", (dim,), f32, at)
+    if out is None:
+        out = x.new_empty((rows, dim), dtype=bf)
+        out_pitch = dim
+    else:
+        _operand(out, "out", (rows, dim), bf, at)
+        out_pitch = _pitch(out)
+    if stats is None:
+        stats = x.new_empty((rows, 2), dtype=f32)
+    else:
+        _dense(stats, "stats", (rows, 2), f32, at)
+    wide = x.dtype is f32
+    _launch("k_lnt_fwd", rows * dim * (6.0 if wide else 4.0) + 8.0 * rows, "i2pc_layernorm_train", at, _p(x), wide, pitch,
+            _p(gamma), _p(beta), eps, rows, dim, _p(out), out_pitch, _p(stats))
     return out, stats
 
 
@@ -938,60 +953,62 @@ def layernorm_backward(dy, x, stats, gamma, add=None, dx=None, dgamma=None, dbet
     pass and gamma.  dx has x's type; add (x's type): a gradient added to it before its rounding (the residual
     stream's), dx may be add itself.  dgamma, dbeta: fp32 [dim], summed in fp32 in a fixed order."""
     torch = _torch()
-    rows, dim = _rows_dim(x, "x")
-    f32, same = (torch.float32,), (x.dtype,)
-    _operand(x, "x", (rows, dim), (torch.float32, torch.bfloat16))
-    _operand(dy, "dy", (rows, dim), (torch.bfloat16,), x)
-    _dense(stats, "stats", (rows, 2), x)
-    _operand(gamma, "gamma", (dim,), f32, x)
+    f32, bf, same = torch.float32, torch.bfloat16, x.dtype
+    rows, dim, pitch = _rows_dim(x, "x", (f32, bf))
+    at = x.get_device()
+    if _elsewhere(at):
+        with torch.cuda.device(at):
+            return layernorm_backward(dy, x, stats, gamma, add, dx, dgamma, dbeta)
+    _operand(dy, "dy", (rows, dim), bf, at)
+    _dense(stats, "stats", (rows, 2), f32, at)
+    _operand(gamma, "gamma", (dim,), f32, at)
     if add is not None:
-        _operand(add, "add", (rows, dim), same, x)
-    with _on_device_of(x):
-        if dx is None:
-            dx = x.new_empty((rows, dim))
-        else:
-            _operand(dx, "dx", (rows, dim), same, x)
-        if dgamma is None:
-            dgamma = x.new_empty(dim, dtype=torch.float32)
-        else:
-            _operand(dgamma, "dgamma", (dim,), f32, x)
-        if dbeta is None:
-            dbeta = x.new_empty(dim, dtype=torch.float32)
-        else:
-            _operand(dbeta, "dbeta", (dim,), f32, x)
-        nb = _lib.load().i2pc_layernorm_backward_workspace_bytes(rows, dim)
-        ws = x.new_empty(nb, dtype=torch.uint8) if nb else None
-        e = x.element_size()
-        _launch("k_lnt_bwd", rows * dim * (2.0 + 2.0 * e + (e if add is not None else 0)) + 12.0 * dim,
-                "i2pc_layernorm_backward", x, _p(dy), _pitch(dy), _p(x), int(e == 4), _pitch(x), _p(stats), _p(gamma), _p(add),
-                0 if add is None else _pitch(add), rows, dim, _p(dx), _pitch(dx), _p(dgamma), _p(dbeta), _p(ws), nb)
+        _operand(add, "add", (rows, dim), same, at)
+    if dx is None:
+        dx = x.new_empty((rows, dim))
+        dx_pitch = dim
+    else:
+        _operand(dx, "dx", (rows, dim), same, at)
+        dx_pitch = _pitch(dx)
+    if dgamma is None:
+        dgamma = x.new_empty(dim, dtype=f32)
+    else:
+        _operand(dgamma, "dgamma", (dim,), f32, at)
+    if dbeta is None:
+        dbeta = x.new_empty(dim, dtype=f32)
+    else:
+        _operand(dbeta, "dbeta", (dim,), f32, at)
+    nb = _lib.load().i2pc_layernorm_backward_workspace_bytes(rows, dim)
+    ws = x.new_empty(nb, dtype=torch.uint8) if nb else None
+    e = 4.0 if same is f32 else 2.0
+    _launch("k_lnt_bwd", rows * dim * (2.0 + 2.0 * e + (e if add is not None else 0)) + 12.0 * dim, "i2pc_layernorm_backward", at,
+            _p(dy), _pitch(dy), _p(x), same is f32, pitch, _p(stats), _p(gamma), _p(add), 0 if add is None else _pitch(add), rows,
+            dim, _p(dx), dx_pitch, _p(dgamma), _p(dbeta), _p(ws), nb)
     return dx, dgamma, dbeta
-
-
-def _dense(t, name, shape, like):
-    _operand(t, name, shape, (_torch().float32,), like)
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
 
 
 def gelu_fp8(x, out=None, kept=None):
     """GELU (the erf form) of bf16 rows x [rows, dim], dim % 32 == 0: (y, kept) with y bf16 and kept the Fp8 rows
     of x (quant_fp8's block rule) that gelu_fp8_backward works from: 1.03 bytes a value instead of two."""
     torch = _torch()
-    rows, dim = _rows_dim(x, "x")
-    bf = (torch.bfloat16,)
-    _operand(x, "x", (rows, dim), bf)
-    with _on_device_of(x):
-        if out is None:
-            out = x.new_empty((rows, dim))
-        else:
-            _operand(out, "out", (rows, dim), bf, x)
-        if kept is None:
-            kept = Fp8(x.new_empty((rows, dim), dtype=torch.uint8), x.new_empty((rows, dim // 32), dtype=torch.uint8))
-        else:
-            _kept_operand(kept, rows, dim, x)
-        _launch("k_gelu_keep", rows * dim * (5.0 + 1.0 / 32), "i2pc_gelu_fp8", x, _p(x), _pitch(x), rows, dim, _p(out),
-                _pitch(out), _p(kept.data), _p(kept.scale))
+    bf = torch.bfloat16
+    rows, dim, pitch = _rows_dim(x, "x", (bf,))
+    at = x.get_device()
+    if _elsewhere(at):
+        with torch.cuda.device(at):
+            return gelu_fp8(x, out, kept)
+    if out is None:
+        out = x.new_empty((rows, dim))
+        out_pitch = dim
+    else:
+        _operand(out, "out", (rows, dim), bf, at)
+        out_pitch = _pitch(out)
+    if kept is None:
+        kept = Fp8(x.new_empty((rows, dim), dtype=torch.uint8), x.new_empty((rows, dim // 32), dtype=torch.uint8))
+    else:
+        _kept_operand(kept, rows, dim, at)
+    _launch("k_gelu_keep", rows * dim * (5.0 + 1.0 / 32), "i2pc_gelu_fp8", at, _p(x), pitch, rows, dim, _p(out), out_pitch,
+            _p(kept.data), _p(kept.scale))
     return out, kept
 
 
@@ -1000,35 +1017,37 @@ def gelu_fp8_backward(dy, kept, dx=None, again=None, recompute=False):
     (or an `again` to write to): (dx, again), again = GELU(x~) in bf16, for the next linear layer's weight
     gradient."""
     torch = _torch()
-    rows, dim = _rows_dim(dy, "dy")
-    bf = (torch.bfloat16,)
-    _operand(dy, "dy", (rows, dim), bf)
-    _kept_operand(kept, rows, dim, dy)
-    with _on_device_of(dy):
-        if dx is None:
-            dx = dy.new_empty((rows, dim))
-        else:
-            _operand(dx, "dx", (rows, dim), bf, dy)
-        if again is not None:
-            _operand(again, "again", (rows, dim), bf, dy)
-        elif recompute:
-            again = dy.new_empty((rows, dim))
-        _launch("k_gelu_back", rows * dim * (5.0 + 1.0 / 32 + (2.0 if again is not None else 0.0)), "i2pc_gelu_fp8_backward", dy,
-                _p(dy), _pitch(dy), _p(kept.data), _p(kept.scale), rows, dim, _p(dx), _pitch(dx), _p(again),
-                0 if again is None else _pitch(again))
+    bf = torch.bfloat16
+    rows, dim, pitch = _rows_dim(dy, "dy", (bf,))
+    at = dy.get_device()
+    if _elsewhere(at):
+        with torch.cuda.device(at):
+            return gelu_fp8_backward(dy, kept, dx, again, recompute)
+    _kept_operand(kept, rows, dim, at)
+    dx_pitch = again_pitch = dim
+    if dx is None:
+        dx = dy.new_empty((rows, dim))
+    else:
+        _operand(dx, "dx", (rows, dim), bf, at)
+        dx_pitch = _pitch(dx)
+    if again is not None:
+        _operand(again, "again", (rows, dim), bf, at)
+        again_pitch = _pitch(again)
+    elif recompute:
+        again = dy.new_empty((rows, dim))
+    _launch("k_gelu_back", rows * dim * (5.0 + 1.0 / 32 + (2.0 if again is not None else 0.0)), "i2pc_gelu_fp8_backward", at,
+            _p(dy), pitch, _p(kept.data), _p(kept.scale), rows, dim, _p(dx), dx_pitch, _p(again), again_pitch)
     return dx if again is None else (dx, again)
 
 
-def _kept_operand(kept, rows, dim, like):
-    u8 = (_torch().uint8,)
+def _kept_operand(kept, rows, dim, at):
+    u8 = _torch().uint8
     if not isinstance(kept, Fp8):
         raise TypeError(f"kept: expected Fp8 rows, got {type(kept).__name__}")
     if dim % 32:
         raise ValueError(f"dim={dim} must be a multiple of 32")
-    _operand(kept.data, "kept.data", (rows, dim), u8, like)
-    _operand(kept.scale, "kept.scale", (rows, dim // 32), u8, like)
-    if not (kept.data.is_contiguous() and kept.scale.is_contiguous()):
-        raise ValueError("kept must be contiguous")
+    _dense(kept.data, "kept.data", (rows, dim), u8, at)
+    _dense(kept.scale, "kept.scale", (rows, dim // 32), u8, at)
 
 
 # ------------------------------------------------------------------ attention over packed sequences
@@ -1055,34 +1074,37 @@ _lib.register("i2pc_attention_packed_backward", ctypes.c_int, [ctypes.POINTER(At
                                                                c_void_p])
 
 
-def _attn_packed_desc(q, k, v, out, lse, cu_q, cu_k, k_lens, scale, causal, zero_tail):
-    """Checks the operands of a packed attention call and makes its descriptor."""
+def _attn_packed_desc(q, k, v, out, lse, cu_q, cu_k, k_lens, scale, causal, fresh):
+    """Checks the operands of a packed attention call and makes its descriptor.  fresh: out and lse were made for the call
+    where it is the forward one."""
     torch = _torch()
-    bf, i32 = (torch.bfloat16,), (torch.int32,)
+    bf, i32 = torch.bfloat16, torch.int32
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"q, k: expected [tokens, heads, head_dim], got the shapes {tuple(q.shape)}, {tuple(k.shape)}")
     tq, heads, hd = q.shape
     tk, kv, _ = k.shape
-    _operand(q, "q", (tq, heads, hd), bf)
-    _operand(k, "k", (tk, kv, hd), bf, q)
-    _operand(v, "v", (tk, kv, hd), bf, q)
-    _operand(out, "out", (tq, heads, hd), bf, q)
-    _dense(lse, "lse", (tq, heads), q)
+    _operand(q, "q", (tq, heads, hd), bf, None)
+    at = q.get_device()
+    _operand(k, "k", (tk, kv, hd), bf, at)
+    _operand(v, "v", (tk, kv, hd), bf, at)
+    if not fresh:
+        _operand(out, "out", (tq, heads, hd), bf, at)
+        _dense(lse, "lse", (tq, heads), torch.float32, at)
     if cu_q.dim() != 1 or cu_q.shape[0] < 2:
         raise ValueError(f"cu_q: expected int32 [sequences + 1] of one sequence at least, got the shape {tuple(cu_q.shape)}")
     n = cu_q.shape[0]
-    _operand(cu_q, "cu_q", (n,), i32, q)
+    _operand(cu_q, "cu_q", (n,), i32, at)
     if cu_k is None:
         if tk != tq:
             raise ValueError(f"k has {tk} rows and q {tq}: give cu_k")
         cu_k = cu_q
-    else:
-        _operand(cu_k, "cu_k", (n,), i32, q)
+    elif cu_k is not cu_q:
+        _operand(cu_k, "cu_k", (n,), i32, at)
     if k_lens is not None:
-        _operand(k_lens, "k_lens", (n - 1,), i32, q)
+        _operand(k_lens, "k_lens", (n - 1,), i32, at)
     (q_t, q_h, _), (k_t, k_h, _), (v_t, v_h, _), (o_t, o_h, _) = q.stride(), k.stride(), v.stride(), out.stride()
     return AttnPackedDesc(_p(q), _p(k), _p(v), q_t, q_h, k_t, k_h, v_t, v_h, _p(out), o_t, o_h, _p(lse), _p(cu_q), _p(cu_k),
-                          _p(k_lens), n - 1, tq, tk, heads, kv, hd, bool(causal), zero_tail, hd ** -0.5 if scale is None else scale)
+                          _p(k_lens), n - 1, tq, tk, heads, kv, hd, bool(causal), 0, hd ** -0.5 if scale is None else scale)
 
 
 def attention_packed(q, k, v, cu_q, cu_k=None, k_lens=None, scale=None, causal=False, out=None, lse=None):
@@ -1101,18 +1123,21 @@ def attention_packed(q, k, v, cu_q, cu_k=None, k_lens=None, scale=None, causal=F
     torch = _torch()
     if (out is None) != (lse is None):
         raise ValueError("give both out and lse, or neither")
-    with _on_device_of(q):
-        fresh = out is None
-        if fresh:
-            out = q.new_empty(q.shape)
-            lse = q.new_empty(q.shape[:2], dtype=torch.float32)
-        d = _attn_packed_desc(q, k, v, out, lse, cu_q, cu_k, k_lens, scale, causal, fresh)
-        ref = ctypes.byref(d)
-        nb = _lib.load().i2pc_attention_packed_workspace_bytes(ref)
-        ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
-        # the lengths are on the device: the flops of the call are not known here
-        _launch("k_attnp_fwd", 2.0 * (2 * q.numel() + k.numel() + v.numel()) + 4.0 * lse.numel(), "i2pc_attention_packed", q, ref,
-                _p(ws), nb)
+    at = q.get_device()
+    if _elsewhere(at):
+        with torch.cuda.device(at):
+            return attention_packed(q, k, v, cu_q, cu_k, k_lens, scale, causal, out, lse)
+    fresh = out is None
+    if fresh:
+        out = q.new_empty(q.shape)
+        lse = q.new_empty(q.shape[:2], dtype=torch.float32)
+    d = _attn_packed_desc(q, k, v, out, lse, cu_q, cu_k, k_lens, scale, causal, fresh)
+    d.zero_tail = fresh
+    ref = ctypes.byref(d)
+    nb = _lib.load().i2pc_attention_packed_workspace_bytes(ref)
+    ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
+    # the lengths are on the device: the flops of the call are not known here
+    _launch("k_attnp_fwd", 2.0 * (2 * q.numel() + 2 * k.numel()) + 4.0 * lse.numel(), "i2pc_attention_packed", at, ref, _p(ws), nb)
     return out, lse
 
 
@@ -1122,23 +1147,27 @@ def attention_packed_backward(dout, q, k, v, out, lse, cu_q, cu_k=None, scale=No
     head; all sums are fp32 in a fixed order.  Rows behind the last sequence keep what a given dq / dk / dv holds (give all
     three, or none), and are 0 in new ones."""
     torch = _torch()
-    bf = (torch.bfloat16,)
+    bf = torch.bfloat16
     fresh = dq is None
     if (dk is None) != fresh or (dv is None) != fresh:
         raise ValueError("give all of dq, dk, dv, or none")
-    with _on_device_of(q):
-        d = _attn_packed_desc(q, k, v, out, lse, cu_q, cu_k, None, scale, causal, fresh)
-        _operand(dout, "dout", q.shape, bf, q)
-        if fresh:
-            dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape)
-        else:
-            _operand(dq, "dq", q.shape, bf, q)
-            _operand(dk, "dk", k.shape, bf, q)
-            _operand(dv, "dv", v.shape, bf, q)
-        (d_t, d_h, _), (dq_t, dq_h, _), (dk_t, dk_h, _), (dv_t, dv_h, _) = dout.stride(), dq.stride(), dk.stride(), dv.stride()
-        ref = ctypes.byref(AttnPackedGradDesc(d, _p(dout), d_t, d_h, _p(dq), _p(dk), _p(dv), dq_t, dq_h, dk_t, dk_h, dv_t, dv_h))
-        nb = _lib.load().i2pc_attention_packed_backward_workspace_bytes(ref)
-        ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
-        _launch("k_attnp_bwd", 2.0 * (4 * q.numel() + 2 * k.numel() + 2 * v.numel()) + 4.0 * lse.numel(),
-                "i2pc_attention_packed_backward", q, ref, _p(ws), nb)
+    at = q.get_device()
+    if _elsewhere(at):
+        with torch.cuda.device(at):
+            return attention_packed_backward(dout, q, k, v, out, lse, cu_q, cu_k, scale, causal, dq, dk, dv)
+    d = _attn_packed_desc(q, k, v, out, lse, cu_q, cu_k, None, scale, causal, False)
+    d.zero_tail = fresh
+    _operand(dout, "dout", q.shape, bf, at)
+    if fresh:
+        dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape)
+    else:
+        _operand(dq, "dq", q.shape, bf, at)
+        _operand(dk, "dk", k.shape, bf, at)
+        _operand(dv, "dv", v.shape, bf, at)
+    (d_t, d_h, _), (dq_t, dq_h, _), (dk_t, dk_h, _), (dv_t, dv_h, _) = dout.stride(), dq.stride(), dk.stride(), dv.stride()
+    ref = ctypes.byref(AttnPackedGradDesc(d, _p(dout), d_t, d_h, _p(dq), _p(dk), _p(dv), dq_t, dq_h, dk_t, dk_h, dv_t, dv_h))
+    nb = _lib.load().i2pc_attention_packed_backward_workspace_bytes(ref)
+    ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
+    _launch("k_attnp_bwd", 2.0 * (4 * q.numel() + 4 * k.numel()) + 4.0 * lse.numel(), "i2pc_attention_packed_backward", at, ref,
+            _p(ws), nb)
     return dq, dk, dv

@@ -51,23 +51,26 @@ class _Device:
 def test_shapes_types_and_strides():
     bf = torch.bfloat16
     op = ops._operand
-    op(_Device(torch.zeros(3, 4)), "t", (3, 4), (torch.float32,))
+    op(_Device(torch.zeros(3, 4)), "t", (3, 4), torch.float32, None)
     with pytest.raises(_lib.I2PCError):
-        op(torch.zeros(3, 4), "t", (3, 4), (torch.float32,))
+        op(torch.zeros(3, 4), "t", (3, 4), torch.float32, None)
     with pytest.raises(TypeError):
-        op(_Device(torch.zeros(3, 4)), "t", (3, 4), (bf,))
+        op(_Device(torch.zeros(3, 4)), "t", (3, 4), bf, None)
     with pytest.raises(ValueError):
-        op(_Device(torch.zeros(3, 5)), "t", (3, 4), (torch.float32,))
+        op(_Device(torch.zeros(3, 5)), "t", (3, 4), torch.float32, None)
     with pytest.raises(ValueError):
-        op(_Device(torch.zeros(4, 3).t()), "t", (3, 4), (torch.float32,))
-    with pytest.raises(ValueError):
-        ops.layernorm_train(torch.zeros(2, 3, 4), None, None, 1e-6)
-    with pytest.raises(ValueError):
-        ops.gelu_fp8(torch.zeros(2, 3, 4))
+        op(_Device(torch.zeros(4, 3).t()), "t", (3, 4), torch.float32, None)
+    rows = ops._rows_dim
+    assert rows(_Device(torch.zeros(3, 4)), "x", (torch.float32, bf)) == (3, 4, 4)
+    assert rows(_Device(torch.zeros(3, 9)[:, 2:6]), "x", (torch.float32,)) == (3, 4, 9)
+    assert rows(_Device(torch.zeros(1, 4).expand(1, 4)), "x", (torch.float32,)) == (1, 4, 4)
+    for bad, error in ((torch.zeros(2, 3, 4), ValueError), (torch.zeros(4, 3).t(), ValueError), (torch.zeros(3, 4).half(), TypeError)):
+        with pytest.raises(error):
+            rows(_Device(bad), "x", (torch.float32, bf))
     with pytest.raises(TypeError):
-        ops._kept_operand(torch.zeros(2, 32), 2, 32, None)
+        ops._kept_operand(torch.zeros(2, 32), 2, 32, 0)
     with pytest.raises(ValueError):
-        ops._kept_operand(ops.Fp8(None, None), 2, 33, None)
+        ops._kept_operand(ops.Fp8(None, None), 2, 33, 0)
     dev = lambda *shape, dtype=bf: _Device(torch.zeros(*shape, dtype=dtype))              # noqa: E731
     q, lse, cu = dev(4, 2, 64), dev(4, 2, dtype=torch.float32), dev(2, dtype=torch.int32)
     desc = lambda q=q, k=q, v=q, out=q, lse=lse, cu_q=cu, cu_k=None, k_lens=None: ops._attn_packed_desc(               # noqa: E731

@@ -17,7 +17,6 @@
 #include "common.h"
 
 #include <algorithm>
-#include <cmath>
 #include <type_traits>
 
 namespace i2pc {
@@ -389,8 +388,8 @@ __device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const Lan
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[i]);
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
     mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * c;
-    // a row that sees nothing here keeps its reference
-    const float m_new = first ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, w.m);
+    // a row that sees nothing here keeps its reference; one whose first 32 scores are all -inf gets one below any score
+    const float m_new = first ? fmaxf(mx, -1e30f) : fmaxf(mx, w.m);
     if (!first) {
       const float alpha = __builtin_amdgcn_exp2f(w.m - m_new);
       w.l *= alpha;
@@ -421,7 +420,7 @@ __device__ __forceinline__ void attend_again(Rows& w, const bf16x8 (&qf)[4], con
     const float x = dot_row(K + j * k_t, qf, hh) * c;
     if (j < nk) {
       const float m_new = fmaxf(m, x), alpha = m == m_new ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
-      const float p = __builtin_amdgcn_exp2f(x - m_new);
+      const float p = x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - m_new);
       m = m_new;
       l = fmaf(l, alpha, p);
       for (int i = 0; i < 16; ++i) {
@@ -1237,8 +1236,8 @@ inline bool few_rows(const i2pc_attn_packed_desc& d) {
   return (int64_t)d.total_q * (d.heads / d.kv_heads) <= (int64_t)d.batch * kFew;
 }
 
-// Shares of the keys: one where the row tiles fill the chip, else so many that they do, of 256 keys at least (an
-// upper bound: a share may be empty).
+// Shares of the keys: one where the row tiles fill the chip, else so many that they do, of 256 keys at least on average
+// (few rows: 2048, since each share there is a partial row to join; an upper bound, a share may be empty).
 inline int splits(const i2pc_attn_packed_desc& d) {
   if (d.total_k == 0) return 1;
   const bool few = few_rows(d);
@@ -1262,10 +1261,15 @@ inline KeySplit key_split(const i2pc_attn_packed_desc& d) {
   return {wide * heads < 768 ? 2 : 4, heads};
 }
 
-// Rows apart (the range checks of the tiles' loads go by the row stride), heads apart too where they are written.
+// Rows apart (the range checks of the tiles' loads go by the row stride); where they are written heads apart too, and the
+// heads of a row all before the next row or the rows of a head all before the next head.
 inline bool rows_ok(const void* p, int64_t t, int64_t h, int rows, int heads, bool written) {
-  return rows == 0 || (p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && t % 8 == 0 && h % 8 == 0 && (rows == 1 || t >= 64) &&
-                       t >= 0 && t < ((int64_t)1 << 23) && (written && heads > 1 ? h >= 64 : h >= 0) && h < ((int64_t)1 << 40));
+  if (rows == 0) return true;
+  if (!p || reinterpret_cast<uintptr_t>(p) % 16 || t % 8 || h % 8 || t < 0 || t >= (int64_t)1 << 23 || h < 0 || h >= (int64_t)1 << 40 ||
+      (rows > 1 && t < 64))
+    return false;
+  if (!written || heads == 1) return true;
+  return h >= 64 && (rows == 1 || t >= (heads - 1) * h + 64 || h >= (rows - 1) * t + 64);
 }
 
 int check(const char* what, const i2pc_attn_packed_desc* d) {
@@ -1280,7 +1284,8 @@ int check(const char* what, const i2pc_attn_packed_desc* d) {
   if ((int64_t)d->total_q * d->heads >= most * 32 || ((int64_t)d->total_q / kRows + 2 * (int64_t)d->batch + 2) * d->heads >= most ||
       ((int64_t)d->total_k / 64 + (int64_t)d->batch + 1) * d->kv_heads >= most)
     return set_error(I2PC_EUNSUPPORTED, "%s: total_q * heads must stay below 2^29, (total_k / 64 + batch) * kv_heads below 2^24", what);
-  I2PC_REQUIRE(std::isfinite(d->scale) && d->scale > 0.f, "%s: scale=%g must be finite and above zero", what, (double)d->scale);
+  // lse / scale has to stay finite
+  I2PC_REQUIRE(d->scale >= 0x1p-64f && d->scale <= 0x1p64f, "%s: scale=%g must lie within 2^-64 and 2^64", what, (double)d->scale);
   I2PC_REQUIRE(d->batch == 0 || (d->cu_q && d->cu_k), "%s: NULL cu_q or cu_k", what);
   I2PC_REQUIRE(rows_ok(d->q, d->q_t, d->q_h, d->total_q, d->heads, false) &&
                    rows_ok(d->out, d->o_t, d->o_h, d->total_q, d->heads, true) &&
@@ -1288,7 +1293,7 @@ int check(const char* what, const i2pc_attn_packed_desc* d) {
                    rows_ok(d->v, d->v_t, d->v_h, d->total_k, d->kv_heads, false) &&
                    (d->total_q == 0 || d->lse),
                "%s: q, k, v, out must be 16-byte aligned with strides that are multiples of 8 "
-               "(row strides from 64 to 2^23)", what);
+               "(row strides from 64 to 2^23), out without rows that overlap", what);
   return I2PC_OK;
 }
 
@@ -1362,7 +1367,7 @@ static int check_grad(const i2pc_attn_packed_grad_desc* g) {
                    rows_ok(g->dk, g->dk_t, g->dk_h, d.total_k, d.kv_heads, true) &&
                    rows_ok(g->dv, g->dv_t, g->dv_h, d.total_k, d.kv_heads, true),
                "attention_packed_backward: dout, dq, dk, dv must be 16-byte aligned with strides that are multiples of 8 "
-               "(row strides from 64 to 2^23)");
+               "(row strides from 64 to 2^23), dq, dk, dv without rows that overlap");
   return I2PC_OK;
 }
 

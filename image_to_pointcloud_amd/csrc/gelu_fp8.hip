@@ -52,8 +52,7 @@ __device__ __forceinline__ int64_t at(uint32_t c, uint32_t per_row, int64_t ld) 
   return r * ld + (int64_t)(c - r * per_row) * 8;
 }
 
-__global__ __launch_bounds__(256) void k_gelu_keep(const uint16_t* __restrict__ x, int64_t ldx, uint32_t chunks, uint32_t per_row,
-                                                   uint16_t* __restrict__ y, int64_t ldy, uint8_t* __restrict__ kept,
+__global__ __launch_bounds__(256) void k_gelu_keep(const uint16_t* x, int64_t ldx, uint32_t chunks, uint32_t per_row, uint16_t* y, int64_t ldy, uint8_t* __restrict__ kept,
                                                    uint8_t* __restrict__ scale) {
   const uint32_t c = blockIdx.x * 256 + threadIdx.x;
   // chunks is a multiple of four: a block's four lanes are on or off together
@@ -95,9 +94,9 @@ __global__ __launch_bounds__(256) void k_gelu_keep(const uint16_t* __restrict__ 
 }
 
 template <bool AGAIN>
-__global__ __launch_bounds__(256) void k_gelu_back(const uint16_t* __restrict__ dy, int64_t lddy, const uint8_t* __restrict__ kept,
+__global__ __launch_bounds__(256) void k_gelu_back(const uint16_t* dy, int64_t lddy, const uint8_t* __restrict__ kept,
                                                    const uint8_t* __restrict__ scale, uint32_t chunks, uint32_t per_row,
-                                                   uint16_t* __restrict__ dx, int64_t lddx, uint16_t* __restrict__ again,
+                                                   uint16_t* dx, int64_t lddx, uint16_t* __restrict__ again,
                                                    int64_t lda) {
   const uint32_t c = blockIdx.x * 256 + threadIdx.x;
   if (c >= chunks) return;

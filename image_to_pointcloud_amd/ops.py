@@ -862,6 +862,9 @@ _lib.register("i2pc_gelu_fp8_backward", ctypes.c_int, [c_void_p, c_int64, c_void
                                                        c_int64, c_void_p, c_int64, c_void_p])
 
 
+_INT_MAX = 2 ** 31 - 1
+
+
 def _operand(t, name, shape, dtype, at):
     """Refuses a tensor that is not on device `at` (any with None), not of `shape` and `dtype`, or whose last axis is not
     dense."""
@@ -893,6 +896,8 @@ def _rows_dim(t, name, dtypes):
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: expected {' or '.join(map(str, dtypes))}, got {t.dtype}")
     rows, dim = t.shape
+    if max(rows, dim) > _INT_MAX:
+        raise ValueError(f"{name}: the shape {tuple(t.shape)} is above 2^31 - 1")
     pitch, dense = t.stride()
     if dim > 1 and dense != 1:
         raise ValueError(f"{name}: the last axis must be dense, its stride is {dense}")
@@ -922,7 +927,7 @@ def _launch(label, nbytes, name, at, *args):
 def layernorm_train(x, gamma, beta, eps, out=None, stats=None):
     """LayerNorm of the rows of x [rows, dim] (fp32 or bf16, any row pitch and alignment; dim <= 8192) for a
     training step: (y, stats) with y bf16 [rows, dim] and stats fp32 [rows, 2] = each row's (mean, 1 / std),
-    which layernorm_backward reads.  gamma, beta: fp32 [dim].  Rows and statistics are held in fp32."""
+    which layernorm_backward reads.  gamma, beta: fp32 [dim].  Rows and statistics are held in fp32; out may not be x."""
     torch = _torch()
     f32, bf = torch.float32, torch.bfloat16
     rows, dim, pitch = _rows_dim(x, "x", (f32, bf))
@@ -989,7 +994,7 @@ def layernorm_backward(dy, x, stats, gamma, add=None, dx=None, dgamma=None, dbet
 
 def gelu_fp8(x, out=None, kept=None):
     """GELU (the erf form) of bf16 rows x [rows, dim], dim % 32 == 0: (y, kept) with y bf16 and kept the Fp8 rows
-    of x (quant_fp8's block rule) that gelu_fp8_backward works from: 1.03 bytes a value instead of two."""
+    of x (quant_fp8's block rule) that gelu_fp8_backward works from: 1.03 bytes a value instead of two.  out may be x."""
     torch = _torch()
     bf = torch.bfloat16
     rows, dim, pitch = _rows_dim(x, "x", (bf,))
@@ -1015,7 +1020,7 @@ def gelu_fp8(x, out=None, kept=None):
 def gelu_fp8_backward(dy, kept, dx=None, again=None, recompute=False):
     """dx = dy * GELU'(x~) (bf16) from dy bf16 [rows, dim] and the Fp8 rows x~ that gelu_fp8 kept; with recompute
     (or an `again` to write to): (dx, again), again = GELU(x~) in bf16, for the next linear layer's weight
-    gradient."""
+    gradient.  dx may be dy."""
     torch = _torch()
     bf = torch.bfloat16
     rows, dim, pitch = _rows_dim(dy, "dy", (bf,))
@@ -1083,6 +1088,8 @@ def _attn_packed_desc(q, k, v, out, lse, cu_q, cu_k, k_lens, scale, causal, fres
         raise ValueError(f"q, k: expected [tokens, heads, head_dim], got the shapes {tuple(q.shape)}, {tuple(k.shape)}")
     tq, heads, hd = q.shape
     tk, kv, _ = k.shape
+    if max(tq, tk, heads, kv, hd) > _INT_MAX:
+        raise ValueError(f"q, k: the shapes {tuple(q.shape)}, {tuple(k.shape)} are above 2^31 - 1")
     _operand(q, "q", (tq, heads, hd), bf, None)
     at = q.get_device()
     _operand(k, "k", (tk, kv, hd), bf, at)
@@ -1118,7 +1125,7 @@ def attention_packed(q, k, v, cu_q, cu_k=None, k_lens=None, scale=None, causal=F
     runs.  causal: query i of lq sees the keys j <= i + lk - lq of lk.  scale defaults to 1 / 8.
     out bf16 [total_q, heads, 64]; lse fp32 [total_q, heads] = log(sum(exp(scores))).  A query that sees no key has
     out 0, lse -inf.  Rows behind the last sequence keep what a given `out` / `lse` holds (give both, or neither), and
-    are 0 / -inf in new ones.
+    are 0 / -inf in new ones.  No output may overlap an input or itself.
     """
     torch = _torch()
     if (out is None) != (lse is None):

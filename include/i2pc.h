@@ -571,7 +571,8 @@ int i2pc_model_file_info(const char* path, int32_t* ints32, float* floats16, int
  * packed sequences with its gradients.
  * ------------------------------------------------------------------------ */
 /* y = (x - mean) / std * gamma + beta per row, std = sqrt(var + eps); x [rows][ldx] fp32 (x_f32) or bf16,
- * any alignment; y bf16 [rows][ldy]; stats fp32 [rows][2] = (mean, 1 / std).  0 < dim <= 8192; rows may be 0. */
+ * any alignment; y bf16 [rows][ldy], not over x; stats fp32 [rows][2] = (mean, 1 / std).  0 < dim <= 8192; rows may
+ * be 0. */
 int i2pc_layernorm_train(const void* x, int x_f32, int64_t ldx, const float* gamma, const float* beta, float eps,
                          int rows, int dim, void* y, int64_t ldy, float* stats, void* stream);
 /* Its gradients from dy bf16 [rows][lddy]: dx (x's type) [rows][lddx] (+ add, x's type [rows][lda], or NULL; dx may
@@ -582,10 +583,10 @@ int i2pc_layernorm_backward(const void* dy, int64_t lddy, const void* x, int x_f
                             const float* gamma, const void* add, int64_t lda, int rows, int dim, void* dx, int64_t lddx,
                             float* dgamma, float* dbeta, void* workspace, size_t workspace_bytes, void* stream);
 /* y = GELU(x) (erf form) of bf16 rows, and x kept as MX fp8 (i2pc_quant_fp8's block rule): kept e4m3 [rows][dim],
- * kept_scale E8M0 [rows][dim / 32], both dense.  dim % 32 == 0; row pitches multiples of 8, 16-byte aligned. */
+ * kept_scale E8M0 [rows][dim / 32], both dense.  dim % 32 == 0; row pitches multiples of 8, 16-byte aligned; y may be x, nothing else may overlap. */
 int i2pc_gelu_fp8(const void* x, int64_t ldx, int64_t rows, int dim, void* y, int64_t ldy, void* kept, void* kept_scale,
                   void* stream);
-/* dx = dy GELU'(x~) of the kept x~, and with `again` not NULL also again = GELU(x~); bf16 rows. */
+/* dx = dy GELU'(x~) of the kept x~, and with `again` not NULL also again = GELU(x~); bf16 rows.  dx may be dy. */
 int i2pc_gelu_fp8_backward(const void* dy, int64_t lddy, const void* kept, const void* kept_scale, int64_t rows, int dim,
                            void* dx, int64_t lddx, void* again, int64_t ld_again, void* stream);
 
@@ -594,7 +595,8 @@ int i2pc_gelu_fp8_backward(const void* dy, int64_t lddy, const void* kept, const
  * is given -- a cache with a slab of slots for each sequence.  cu_q, cu_k: int32 [batch + 1] on the device, rising,
  * cu_q[0] = 0; the kernels read them when they run, so a captured graph follows their contents, and hold what they
  * say to total_q / total_k rows.  Element (row t, head h) of q starts at q + t * q_t + h * q_h elements (out, k, v
- * alike) and its head_dim = 64 bf16 values are dense; query head h reads key head h / (heads / kv_heads).
+ * alike) and its head_dim = 64 bf16 values are dense; query head h reads key head h / (heads / kv_heads).  No output may
+ * overlap an input or itself.
  *   S = scale Q K^T; causal: query i of a sequence of lq queries and lk keys sees keys j <= i + lk - lq;
  *   out = softmax(S) V, lse [total_q][heads] = log(sum exp(S)) (fp32); a query that sees no key has out = 0,
  *   lse = -inf.
@@ -607,7 +609,7 @@ typedef struct i2pc_attn_packed_desc {
   float* lse;
   const int32_t *cu_q, *cu_k, *k_lens;
   int32_t batch, total_q, total_k, heads, kv_heads, head_dim, causal, zero_tail;
-  float scale;                   /* > 0 */
+  float scale;                   /* 2^-64 .. 2^64 */
 } i2pc_attn_packed_desc;
 /* Scratch memory of the call (0 where its keys are not split); contents do not matter before or after. */
 size_t i2pc_attention_packed_workspace_bytes(const i2pc_attn_packed_desc* desc);

@@ -369,7 +369,41 @@ def test_no_keys_or_no_queries_at_all():
     assert out.shape == q.shape and not dk.any() and not dv.any()
 
 
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("rows", [1, 70])
+def test_scores_of_minus_infinity(rows, causal):
+    """Keys whose visible scores are -inf have probability 0, also where they are a row's first ones and every other score
+    is far below zero; with a NaN behind the mask too, where the row is done again."""
+    ops = _ops()
+    n = 300
+    q, k, v, _ = make([rows], [n], heads=2, seed=4)
+    q, k = q.abs() + 0.5, -k.abs() * 16 - 8                   # scores of some hundreds below zero
+    k[:70, :, 0] = -INF
+    c = (cu([rows]), cu([n]))
+    ref = reference(q[:, :], k[70:], v[70:], [rows], [n - 70], causal, 0.125)
+    out, lse = ops.attention_packed(q, k, v, *c, causal=causal)
+    inside(out, ref["out"], ref["out_b"], "out")
+    inside(lse, ref["lse"], ref["lse_b"], "lse")
+    if causal and rows > 1:
+        k[n - 1], v[n - 1] = float("nan"), float("nan")       # the last query's own
+        out, lse = ops.attention_packed(q, k, v, *c, causal=True)
+        inside(out[:-1], ref["out"][:-1], ref["out_b"][:-1], "out")
+        inside(lse[:-1], ref["lse"][:-1], ref["lse_b"][:-1], "lse")
+
+
 # ------------------------------------------------------------------ how it is called
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("batch", [16, 17, 64, 65, 200])
+def test_numbers_of_sequences(batch, causal):
+    """Either side of the sizes at which the lookup of a tile changes, with rows behind the last sequence."""
+    gen = torch.Generator().manual_seed(batch)
+    ql = torch.randint(0, 40, (batch,), generator=gen).tolist()
+    kl = torch.randint(0, 60, (batch,), generator=gen).tolist()
+    ql[0], kl[1], ql[-1], kl[-1] = 0, 0, 141, 150
+    q, k, v, dout, out, lse = check(ql, kl, heads=2, kv=1, causal=causal, seed=batch, extra=(150, 270))
+    assert not out[sum(ql):].any() and (lse[sum(ql):] == -INF).all()
+
+
 def test_runs_are_alike_and_streams():
     ops = _ops()
     q, k, v, dout, out, lse = check([300, 64, 1, 150], heads=6, kv=2, causal=True, seed=31)

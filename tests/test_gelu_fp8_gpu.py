@@ -141,3 +141,16 @@ def test_gradient_against_differences():
     want = dy.double() * ((k + h) * cdf(k + h) - (k - h) * cdf(k - h)) / (2 * h)
     # the difference is of second order in h (1e-10) and of 1e-16 |x| / h
     inside(dx, want, BF * want.abs() + dy.double().abs() * (3 * PHI + 1e-9 + 1e-11 * k.abs()) + TINY, "dx")
+
+
+def test_in_place():
+    ops = _ops()
+    gen = torch.Generator().manual_seed(6)
+    x, dy = (torch.randn(70, 96, generator=gen).to(torch.bfloat16).cuda() for _ in range(2))
+    y, kept = ops.gelu_fp8(x)
+    dx, again = ops.gelu_fp8_backward(dy, kept, recompute=True)
+    x2, dy2 = x.clone(), dy.clone()
+    got, kept2 = ops.gelu_fp8(x2, out=x2)
+    assert got is x2 and torch.equal(x2, y) and torch.equal(kept2.data, kept.data) and torch.equal(kept2.scale, kept.scale)
+    ops.gelu_fp8_backward(dy2, kept, dx=dy2, recompute=True)
+    assert torch.equal(dy2, dx)

@@ -129,6 +129,19 @@ def test_add_in_place_and_without():
     assert torch.equal(got[1], plain[1]) and torch.equal(got[2], plain[2])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [513, 515, 1025, 1111, 2049, 4097, 8191])
+def test_add_in_place_where_columns_repeat(dim, dtype):
+    """Widths whose last load starts before another wave's columns end."""
+    ops = _ops()
+    x, gamma, beta, dy, add = case(1500, dim, dtype, 22)
+    _, stats = ops.layernorm_train(x, gamma, beta, EPS)
+    want = ops.layernorm_backward(dy, x, stats, gamma, add=add)
+    got = add.clone()
+    ops.layernorm_backward(dy, x, stats, gamma, add=got, dx=got)
+    assert torch.equal(got, want[0])
+
+
 def test_no_rows():
     ops = _ops()
     x = torch.zeros(0, 96, device="cuda")

@@ -144,6 +144,7 @@ def _desc(**kw):
 
 BAD = [({"head_dim": 128}, -4), ({"kv_heads": 3}, -1), ({"heads": 0}, -1), ({"total_q": -1}, -1), ({"batch": -1}, -1),
        ({"scale": 0.0}, -1), ({"scale": -1.0}, -1), ({"scale": float("nan")}, -1), ({"scale": float("inf")}, -1),
+       ({"scale": 1e-30}, -1), ({"o_t": 64, "o_h": 64}, -1), ({"o_t": 128, "o_h": 64 * 100}, -1),
        ({"q": 24}, -1), ({"k_t": 252}, -1), ({"v_h": 60}, -1), ({"k_t": 0}, -1), ({"o_h": 0}, -1), ({"q_t": 1 << 23}, -1),
        ({"cu_q": None}, -1), ({"cu_k": None}, -1), ({"lse": None}, -1), ({"q": None}, -1), ({"total_q": 1 << 30}, -4),
        ({"total_k": (1 << 31) - 1, "kv_heads": 4}, -4)]
@@ -192,3 +193,41 @@ def test_attention_workspaces_and_the_backward_pass_own_refusals():
     g.dk_h = 0
     assert _rc("i2pc_attention_packed_backward", ctypes.byref(g), 16, need, None)[0] == -1
     assert _rc("i2pc_attention_packed", ctypes.byref(_desc(total_q=0)), None, 0, None) == (0, "")
+
+
+def test_outputs_that_overlap_themselves_are_refused():
+    _built()
+    lib = _lib.load()
+    # [heads, rows, 64] underneath, heads next to each other, one row, one head
+    for kw in ({"o_t": 64, "o_h": 6400}, {"o_t": 256, "o_h": 64}, {"total_q": 1, "o_t": 0, "o_h": 64},
+               {"heads": 1, "kv_heads": 1, "o_t": 64, "o_h": 0}):
+        g = _grad(**kw)
+        assert lib.i2pc_attention_packed_backward_workspace_bytes(ctypes.byref(g)) > 0, kw
+    for n in ("dq", "dk", "dv"):
+        g = _grad()
+        setattr(g, n + "_t", 128)
+        assert lib.i2pc_attention_packed_backward_workspace_bytes(ctypes.byref(g)) == 0, n
+
+
+def _grad(**kw):
+    g = ops.AttnPackedGradDesc()
+    g.f = _desc(**kw)
+    for n in ("dout", "dq", "dk", "dv"):
+        setattr(g, n, 16)
+    for n in ("d", "dq", "dk", "dv"):
+        setattr(g, n + "_t", 256)
+        setattr(g, n + "_h", 64)
+    return g
+
+
+def test_sizes_above_31_bits_are_refused():
+    """Not cut to their low 32 bits on the way to the library."""
+    bf = torch.bfloat16
+    many = _Device(torch.zeros(1, 64, dtype=bf).expand((1 << 32) + 4, 64))
+    with pytest.raises(ValueError):
+        ops._rows_dim(many, "x", (bf,))
+    q = _Device(torch.zeros(4, 1, 64, dtype=bf))
+    k = _Device(torch.zeros(1, 1, 64, dtype=bf).expand((1 << 32) + 4, 1, 64))
+    cu = _Device(torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        ops._attn_packed_desc(q, k, k, q, None, cu, cu, None, None, False, True)

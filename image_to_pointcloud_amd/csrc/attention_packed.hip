@@ -439,6 +439,9 @@ __device__ __forceinline__ void attend_again(Rows& w, const bf16x8 (&qf)[4], con
 // registers, which then are the B operand of O^T += V^T P^T.  K and V tiles of 64 keys go through LDS by
 // LDS-DMA, double-buffered.  KW 2: waves 2, 3 hold the rows of waves 0, 1 again and take the second 32 keys of each tile,
 // and the two states are joined at the end: twice the workgroups, of half the length.
+// Bound by the exponentials and the products together: 8 x 4096 tokens of 16 heads take 546 us (1006 TF), the vector unit 76 %
+// busy and the matrix unit 55 %, at the 1.6 GHz that the power limit leaves.  Four waves a SIMD: eight-wave workgroups of
+// 256 rows were slower (causal prompts 118 against 107 us), as were raised wave priorities.
 template <bool CAUSAL, bool SPLIT, int KW>
 __global__ __launch_bounds__(256, 4) void k_attnp_fwd(const Args a) {
   constexpr int kWgRows = kRows / KW;
@@ -573,6 +576,8 @@ __global__ __launch_bounds__(256, 4) void k_attnp_fwd(const Args a) {
 // Few rows (new tokens over a cache): 32 packed rows of one key head a workgroup, whose four waves take every fourth
 // block of 32 keys of a share, each with its own two LDS buffers and no barrier until the end -- what counts is how many
 // bytes of K and V are on their way, 8 KiB a wave.  A share is lk / nsplit keys, 256 at least.
+// Bound by HBM: one token of 64 sequences over 97 to 8096 keys, 16 heads over 4: 56 us and 5 us for the join (4.5 TB/s; a copy
+// reaches 4.9); one token over 131071 keys, 16 heads over 2: 14 and 4 us.
 constexpr int kFew = 32;
 constexpr int kFewBlock = 32 * 128;                  // bytes of 32 keys' K (or V)
 template <bool CAUSAL>
@@ -704,7 +709,8 @@ __global__ __launch_bounds__(256, 2) void k_attnp_few(const Args a) {
 }
 
 // The shares of a split call joined, W waves to a row: out = sum_s 2^(l_s - m) O_s / sum_s 2^(l_s - m).  Wave v takes the
-// shares 8 v .. 8 v + 7, then 8 W further, eight loads in flight; a lane is a d.
+// shares 8 v .. 8 v + 7, then 8 W further, eight loads in flight; a lane is a d.  Bound by the latency of two dependent
+// reads: 4 to 5 us.
 template <int W>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_attnp_join(const Args a) {
   __shared__ float red[W == 1 ? 1 : W][W == 1 ? 1 : 64];
@@ -759,7 +765,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_attnp_join(const Args
 // dQ: the forward's rows and tiles; per 32 keys S^T = K Q^T and dP^T = V dO^T (which starts at -D), then
 // dQ^T += K^T dS^T.  KW 2 as in the forward pass.  D = rowsum(dO O) is taken on the way from the rows that the kernel holds
 // anyway, and left for the dK / dV kernel: ndelta = -D, nlse = -lse / scale (-inf for a row that saw nothing, so that its
-// probabilities are 0), both [H][Tq].
+// probabilities are 0), both [H][Tq].  The rounding of O to bf16 is off in D by |dO| |O| 2^-9, which counts where a row has
+// few keys (the share falls with the root of their number): there D = sum P dP is taken from the tile itself.
+// Bound as the forward pass: 8 x 4096 tokens of 16 heads 805 us, 1024 TF over the three products.  Three waves a SIMD; two
+// with the blocks interleaved as in the dK / dV kernel were slower (six images' step 91 against 84 us).
 template <bool CAUSAL, int KW>
 __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
   constexpr int kWgRows = kRows / KW;
@@ -806,28 +815,41 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
     df[t] = *reinterpret_cast<const bf16x8*>(dr + 16 * t + 8 * hh);
   }
   const float c = a.c;
-  float nl;
-  f32x16 nd, dq[2];
-  {
-    const float d = dot_row(a.out + (s.q0 + qi) * a.o_t + h * a.o_h, df, hh), lse = a.lse[(int64_t)(s.q0 + qi) * a.H + h];
-    const bool none = lse == -INFINITY;
-    const float neg = none ? -INFINITY : -lse / a.scale;
-    nl = neg * c;
-    for (int i = 0; i < 16; ++i) {
-      nd[i] = none ? 0.f : -d;
-      dq[0][i] = dq[1][i] = 0.f;
-    }
-    if (r < R && kw == 0 && hh == 0) {
-      const int64_t at = (int64_t)h * a.Tq + s.q0 + qi;
-      a.nlse[at] = neg;
-      a.ndelta[at] = nd[0];
-    }
-  }
+  const float lse = a.lse[(int64_t)(s.q0 + qi) * a.H + h], neg = lse == -INFINITY ? -INFINITY : -lse / a.scale, nl = neg * c;
+  float d = dot_row(a.out + (s.q0 + qi) * a.o_t + h * a.o_h, df, hh);
   __builtin_amdgcn_s_waitcnt(0xF70);
   __syncthreads();
 
-  int bad = 0;
   const Lanes ad(lds_addr(smem) + kw * 4096, lane);
+  if (wave_on && nk_last <= kKV) {                   // D of rows with one tile of keys: sum P dP
+    d = 0.f;
+#pragma clang loop unroll(disable)
+    for (int k2 = 0; 32 * k2 < nk_last; ++k2) {
+      const Lanes at = ad.behind((uint32_t)(k2 - kw) * 4096);
+      const int lim = whole(nk - 32 * k2 - 4 * hh);
+      f32x16 st, dp;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        st = mfma(at.rows(t, 0), qf[t], t == 0 ? f32x16{} : st);
+        dp = mfma(at.rows(t, kTileBytes), df[t], t == 0 ? f32x16{} : dp);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) d += (i & 3) + 8 * (i >> 2) < lim ? __builtin_amdgcn_exp2f(fmaf(st[i], c, nl)) * dp[i] : 0.f;
+    }
+    d += __shfl_xor(d, 32);
+  }
+  f32x16 nd, dq[2];
+  for (int i = 0; i < 16; ++i) {
+    nd[i] = lse == -INFINITY ? 0.f : -d;
+    dq[0][i] = dq[1][i] = 0.f;
+  }
+  if (r < R && kw == 0 && hh == 0) {
+    const int64_t at = (int64_t)h * a.Tq + s.q0 + qi;
+    a.nlse[at] = neg;
+    a.ndelta[at] = nd[0];
+  }
+
+  int bad = 0;
   auto step = [&](int key0, auto buffer) {
     constexpr int cur = decltype(buffer)::value;
     if (key0 + kKV < ke) stage(cur ^ 1, key0 + kKV);
@@ -901,7 +923,9 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
 // dK^T += Q^T dS.  Tiles are of RT = 256 / KW rows: with KW 4 every wave has 32 keys and takes both 32-row blocks of a tile;
 // with KW 2 waves 2, 3 hold the keys of waves 0, 1 again, a wave takes two of the four blocks and the sums are added at the
 // end.  A wave's two blocks are independent: while one's exponentials are on the vector unit the other's products are on
-// the matrix unit.
+// the matrix unit.  8 x 4096 tokens of 16 heads: 1060 us, 1037 TF over the four products (851 cycles a block, 512 of them
+// on the matrix unit; the blocks interleaved and the addresses out of the loops took the whole backward pass from 1777 to
+// 1693 us).
 template <bool CAUSAL, int KW>
 __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
   constexpr int RT = 256 / KW, kRowBytes = RT * 128;
@@ -1200,7 +1224,8 @@ __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
     }
 }
 
-// The query heads' partial sums of dK and dV added, in their order: 32 lanes a key row, four values each.
+// The query heads' partial sums of dK and dV added, in their order: 32 lanes a key row, four values each.  Bound by reading
+// them: 60 MB (7300 tokens, 16 heads) 12 us.
 __global__ __launch_bounds__(256) void k_attnp_sum(const Args a) {
   const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = (int64_t)a.Tk * a.Hk;
   if (n >= rows) return;

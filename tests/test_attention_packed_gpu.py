@@ -43,8 +43,9 @@ def make(ql, kl=None, heads=2, kv=None, seed=0, layout="rows", extra=(0, 0), siz
     return one(tq, heads), one(tk, kv), one(tk, kv), one(tq, heads)
 
 
-def reference(q, k, v, ql, kl, causal, scale, dout=None, starts=None):
-    """Values and, for each output, the bound on its error; rows behind the sequences are zero."""
+def reference(q, k, v, ql, kl, causal, scale, dout=None, starts=None, short=0):
+    """Values and, for each output, the bound on its error; rows behind the sequences are zero.  short: sequences of up to
+    that many keys have D from fp32 sums instead of the rounded output."""
     q, k, v = (t.double().cpu() for t in (q, k, v))
     H, Hk = q.shape[1], k.shape[1]
     r = {"out": torch.zeros_like(q), "out_b": torch.zeros_like(q), "lse": torch.full(q.shape[:2], -INF, dtype=torch.float64),
@@ -81,6 +82,8 @@ def reference(q, k, v, ql, kl, causal, scale, dout=None, starts=None):
                 r["dv_b"][keys, g] += P.T @ ((BF * 1.02 + 2 * es) * G.abs())
                 D = (G * O).sum(1, keepdim=True)
                 eD = (G.abs() * r["out_b"][rows, h]).sum(1, keepdim=True) * 1.02
+                if n <= short:
+                    eD = 3 * es * (P * (G.abs() @ V.abs().T)).sum(1, keepdim=True)
                 dP = G @ V.T
                 Z = P * (dP - D)
                 eZ = 1.02 * (BF * Z.abs() + P * eD + 3 * es * P * (G.abs() @ V.abs().T + D.abs()))
@@ -194,6 +197,20 @@ def test_scores_that_rise_along_the_keys():
         ref = reference(q, k, v, [200], [200], causal, 0.125)
         inside(out, ref["out"], ref["out_b"], "out")
         inside(lse, ref["lse"], ref["lse_b"], "lse")
+
+
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("batch", [6, 160])
+def test_gradients_of_rows_with_few_keys(batch, causal):
+    """Their D is not that of the rounded output: nearly all of dP may cancel against it.  (Few and many row tiles.)"""
+    ops = _ops()
+    ql, kl = [64, 2, 33, 5, 150, 17][:batch] + [60] * (batch - 6), [64, 2, 33, 7, 40, 64][:batch] + [60] * (batch - 6)
+    q, k, v, dout = make(ql, kl, heads=8, kv=2, seed=13)
+    out, lse = ops.attention_packed(q, k, v, cu(ql), cu(kl), causal=causal)
+    got = ops.attention_packed_backward(dout, q, k, v, out, lse, cu(ql), cu(kl), causal=causal)
+    ref = reference(q, k, v, ql, kl, causal, 0.125, dout, short=64)
+    for n, t in zip(("dq", "dk", "dv"), got):
+        inside(t, ref[n], ref[n + "_b"], n)
 
 
 # ------------------------------------------------------------------ one token over a cache

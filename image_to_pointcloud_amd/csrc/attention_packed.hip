@@ -767,7 +767,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_attnp_join(const Args
 // anyway, and left for the dK / dV kernel: ndelta = -D, nlse = -lse / scale (-inf for a row that saw nothing, so that its
 // probabilities are 0), both [H][Tq].  The rounding of O to bf16 is off in D by |dO| |O| 2^-9, which counts where a row has
 // few keys (the share falls with the root of their number): there D = sum P dP is taken from the tile itself.
-// Bound as the forward pass: 8 x 4096 tokens of 16 heads 805 us, 1024 TF over the three products.  Three waves a SIMD; two
+// Bound as the forward pass: 8 x 4096 tokens of 16 heads 762 us, 1082 TF over the three products.  Three waves a SIMD; two
 // with the blocks interleaved as in the dK / dV kernel were slower (six images' step 91 against 84 us).
 template <bool CAUSAL, int KW>
 __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
@@ -923,7 +923,7 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
 // dK^T += Q^T dS.  Tiles are of RT = 256 / KW rows: with KW 4 every wave has 32 keys and takes both 32-row blocks of a tile;
 // with KW 2 waves 2, 3 hold the keys of waves 0, 1 again, a wave takes two of the four blocks and the sums are added at the
 // end.  A wave's two blocks are independent: while one's exponentials are on the vector unit the other's products are on
-// the matrix unit.  8 x 4096 tokens of 16 heads: 1060 us, 1037 TF over the four products (851 cycles a block, 512 of them
+// the matrix unit.  8 x 4096 tokens of 16 heads: 1035 us, 1062 TF over the four products (851 cycles a block, 512 of them
 // on the matrix unit; the blocks interleaved and the addresses out of the loops took the whole backward pass from 1777 to
 // 1693 us).
 template <bool CAUSAL, int KW>

@@ -552,3 +552,22 @@ def test_a_block_of_an_encoder_trains():
         assert rel <= tol, f"{name}: {rel:.3e}"
     # the recomputed activation is that of the kept values
     assert float((again.float() - a.float()).norm() / a.float().norm()) <= 2.0 ** -4
+
+
+def test_profiled_calls_are_listed(monkeypatch):
+    """With a profile list every call leaves its label, bytes and two events, and computes the same."""
+    ops = _ops()
+    q, k, v, dout = make([40, 30], heads=2, seed=1)
+    c, x, g = cu([40, 30]), torch.randn(9, 96, device="cuda"), torch.ones(96, device="cuda")
+    want = ops.attention_packed(q, k, v, c)
+    seen = []
+    monkeypatch.setattr(ops, "profile", seen)
+    out, lse = ops.attention_packed(q, k, v, c)
+    ops.attention_packed_backward(dout, q, k, v, out, lse, c)
+    y, stats = ops.layernorm_train(x, g, g, 1e-6)
+    ops.layernorm_backward(y, x, stats, g)
+    ops.gelu_fp8_backward(y, ops.gelu_fp8(y)[1])
+    torch.cuda.synchronize()
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    assert [s[0] for s in seen] == ["k_attnp_fwd", "k_attnp_bwd", "k_lnt_fwd", "k_lnt_bwd", "k_gelu_keep", "k_gelu_back"]
+    assert all(s[2] > 0 and s[3].elapsed_time(s[4]) >= 0 for s in seen)

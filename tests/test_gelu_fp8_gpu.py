@@ -154,3 +154,18 @@ def test_in_place():
     assert got is x2 and torch.equal(x2, y) and torch.equal(kept2.data, kept.data) and torch.equal(kept2.scale, kept.scale)
     ops.gelu_fp8_backward(dy2, kept, dx=dy2, recompute=True)
     assert torch.equal(dy2, dx)
+
+
+def test_offsets_beyond_32_bits():
+    ops = _ops()
+    rows, dim, pitch = 600, 96, 1 << 22
+    x, dy = (torch.randn(rows, dim, generator=torch.Generator().manual_seed(i)).to(torch.bfloat16).cuda() for i in (1, 2))
+    buf = torch.empty(rows * pitch, dtype=torch.bfloat16, device="cuda")              # only the rows are written
+    far = [buf.as_strided((rows, dim), (pitch, 1), at * 128) for at in range(5)]
+    far[0].copy_(x), far[1].copy_(dy)
+    y, kept = ops.gelu_fp8(far[0], out=far[2])
+    y2, kept2 = ops.gelu_fp8(x)
+    assert torch.equal(y, y2) and torch.equal(kept.data, kept2.data) and torch.equal(kept.scale, kept2.scale)
+    dx, again = ops.gelu_fp8_backward(far[1], kept, dx=far[3], again=far[4])
+    dx2, again2 = ops.gelu_fp8_backward(dy, kept, recompute=True)
+    assert torch.equal(dx, dx2) and torch.equal(again, again2)

@@ -226,3 +226,20 @@ def test_gradient_against_differences():
         # the difference's own error is of order step^2 and 1e-16 / step: 1e-9 of the sum of magnitudes
         size = (grad.double().abs() * v.abs()).sum() + dy.double().abs().sum()
         assert abs(float((grad.double() * v).sum() - slope)) <= 1e-5 * float(size)
+
+
+def test_offsets_beyond_32_bits():
+    """Rows that lie 2^22 values apart in one buffer of more than 4 GiB, and the same rows packed."""
+    ops = _ops()
+    rows, dim, pitch = 600, 384, 1 << 22
+    x, gamma, beta, dy, add = case(rows, dim, torch.bfloat16, 61)
+    buf = torch.empty(rows * pitch, dtype=torch.bfloat16, device="cuda")              # only the rows are written
+    far = [buf.as_strided((rows, dim), (pitch, 1), at * 1024) for at in range(5)]
+    for to, t in zip(far, (x, dy, add)):
+        to.copy_(t)
+    y, stats = ops.layernorm_train(far[0], gamma, beta, EPS, out=far[3])
+    y2, stats2 = ops.layernorm_train(x, gamma, beta, EPS)
+    assert torch.equal(y, y2) and torch.equal(stats, stats2)
+    got = ops.layernorm_backward(far[1], far[0], stats, gamma, add=far[2], dx=far[4])
+    for a, b in zip(got, ops.layernorm_backward(dy, x, stats, gamma, add=add)):
+        assert torch.equal(a, b)

@@ -134,6 +134,61 @@ def test_packs_and_grouped_heads(heads, kv, causal):
     check([1, 70, 0, 33, 129, 64, 0, 2], heads=heads, kv=kv, causal=causal, seed=heads * 7 + kv)
 
 
+@pytest.mark.parametrize("heads,kv,causal", [(16, 16, False), (26, 26, True), (24, 6, False), (24, 6, True), (24, 12, True)])
+def test_many_workgroups(heads, kv, causal):
+    """Packs that fill the chip take other tiles than small ones: 128 rows or keys a workgroup, heads of a group apart or
+    together."""
+    check([577, 577, 130, 577, 1, 577, 33, 577, 0, 577, 577, 577], heads=heads, kv=kv, causal=causal, seed=heads + kv, extra=(40, 40))
+
+
+def test_chunks_over_slabs():
+    """Long chunks at the end of caches, NaN behind the filled slots."""
+    ops = _ops()
+    ql, lens, slab = [300, 1, 900, 77], [1500, 640, 901, 77], 1600
+    q, k, v, _ = make(ql, [slab] * 4, 8, 2, seed=14)
+    for b, n in enumerate(lens):
+        k[b * slab + n:(b + 1) * slab] = float("nan")
+        v[b * slab + n:(b + 1) * slab] = float("nan")
+    for causal in (True, False):
+        out, lse = ops.attention_packed(q, k, v, cu(ql), cu([slab] * 4), k_lens=torch.tensor(lens, dtype=torch.int32).cuda(),
+                                        causal=causal)
+        ref = reference(q, k, v, ql, lens, causal, 0.125, starts=[b * slab for b in range(4)])
+        inside(out, ref["out"], ref["out_b"], "out")
+        inside(lse, ref["lse"], ref["lse_b"], "lse")
+
+
+def test_more_query_heads_than_a_row_block():
+    """40 query heads over one key head: a position's rows lie in two blocks of 32."""
+    check([1, 20, 0, 37], heads=40, kv=1, causal=True, seed=3)
+    check([90], heads=72, kv=2, seed=4)
+
+
+def test_heads_that_share_memory():
+    """Keys and values broadcast over the heads (head stride 0) are those of one grouped key head, and their gradients are
+    the query heads' own."""
+    ops = _ops()
+    q, k, v, dout = make([70, 9], heads=4, kv=1, seed=8)
+    c = cu([70, 9])
+    ke, ve = k.expand(79, 4, 64), v.expand(79, 4, 64)
+    out, lse = ops.attention_packed(q, ke, ve, c, causal=True)
+    ref = reference(q, ke, ve, [70, 9], [70, 9], True, 0.125, dout)
+    inside(out, ref["out"], ref["out_b"], "out")
+    for n, t in zip(("dq", "dk", "dv"), ops.attention_packed_backward(dout, q, ke, ve, out, lse, c, causal=True)):
+        inside(t, ref[n], ref[n + "_b"], n)
+
+
+def test_one_tensor_as_all_three():
+    ops = _ops()
+    x, _, _, dout = make([100, 31], heads=2, seed=9)
+    c = cu([100, 31])
+    a, la = ops.attention_packed(x, x, x, c)
+    b, lb = ops.attention_packed(x, x.clone(), x.clone(), c)
+    assert torch.equal(a, b) and torch.equal(la, lb)
+    for s, t in zip(ops.attention_packed_backward(dout, x, x, x, a, la, c),
+                    ops.attention_packed_backward(dout, x, x.clone(), x.clone(), b, lb, c)):
+        assert torch.equal(s, t)
+
+
 @pytest.mark.parametrize("layout", ["heads", "wide"])
 def test_strides(layout):
     check([40, 100, 3], heads=4, kv=2, causal=True, layout=layout, seed=5)
@@ -316,6 +371,33 @@ def test_nonfinite_masked_rows_in_the_gradients(bad):
     dq, _, _ = ops.attention_packed_backward(dout, q, k2, v2, out, lse, c, causal=True)
     keep = [i for i in range(240) if not 120 <= i < 150]
     inside(dq[keep], ref["dq"][keep], ref["dq_b"][keep], "dq")
+
+
+@pytest.mark.parametrize("heads,kv", [(26, 26), (24, 6)])
+def test_nonfinite_masked_rows_in_many_workgroups(heads, kv):
+    """The same where a pack fills the chip: NaN keys reach only the queries behind them, NaN queries only the keys before."""
+    ops = _ops()
+    ql = [577, 577, 130, 577, 1, 577, 33, 577, 577, 577, 577]
+    q, k, v, dout = make(ql, heads=heads, kv=kv, seed=5)
+    c = cu(ql)
+    ref = reference(q, k, v, ql, ql, True, 0.125, dout)
+    out, lse = ops.attention_packed(q, k, v, c, causal=True)
+    T, first, last = sum(ql), 577 + 300, 2 * 577              # the second sequence from its position 300 on
+    k2, v2 = k.clone(), v.clone()
+    k2[first], v2[first] = float("nan"), float("nan")
+    o2, l2 = ops.attention_packed(q, k2, v2, c, causal=True)
+    dq, _, _ = ops.attention_packed_backward(dout, q, k2, v2, out, lse, c, causal=True)
+    keep = [i for i in range(T) if not first <= i < last]
+    for n, t in (("out", o2), ("lse", l2), ("dq", dq)):
+        inside(t[keep], ref[n][keep], ref[n + "_b"][keep], n)
+        assert t[first:last].isnan().all()
+    q2, d2 = q.clone(), dout.clone()
+    q2[first], d2[first] = float("nan"), float("nan")
+    _, dk, dv = ops.attention_packed_backward(d2, q2, k, v, out, lse, c, causal=True)
+    keep = [i for i in range(T) if not 577 <= i <= first]
+    for n, t in (("dk", dk), ("dv", dv)):
+        inside(t[keep], ref[n][keep], ref[n + "_b"][keep], n)
+        assert t[577:first + 1].isnan().all()
 
 
 def test_nonfinite_neighbours_in_the_pack():

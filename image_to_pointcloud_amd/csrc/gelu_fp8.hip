@@ -7,23 +7,27 @@
 //
 // Phi is the normal distribution's cdf (the erf form of GELU), phi its density.  Both directions read and
 // write each value once and are bound by HBM: 16 B of bf16 a lane and load, four lanes share a block.
-// 18464 x 4096: 71 us forward (5.4 TB/s, part of it from the last-level cache; a copy of 2 GiB reaches 4.9), 91 us backward
-// with `again` (5.8 TB/s).  What it took: no infinity tests on the usual path (167 -> 159 us for both).
+// 18464 x 4096, calls one after the other: 68.5 us forward (5.6 TB/s, part of it from the last-level cache; a copy of 2 GiB
+// reaches 4.9), 92 us backward with `again` (5.8 TB/s), 72 us without (5.3 TB/s; the vector unit counts too: two more operations
+// a value are 3 %).  What it took: no infinity tests on the usual path (167 -> 159 us for both).
 #include "common.h"
 #include "mx.h"
 
 namespace i2pc {
 namespace gelu8 {
 
-// Phi(-|x|) and exp(-x^2 / 2): erfc by Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7, halved here), which needs that
-// exponential anyway.  Its constants are scaled by sqrt(1/2) and 1/2.
+// Phi(-|x|) = t P(t) ex with ex = exp(-x^2 / 2) and t = 1 / (1 + 0.29 |x|): Phi(-|x|) / ex is a smooth function of t down to
+// t = 0, where it goes as 1 / |x|.  P is a minimax fit of degree 5 over |x| <= 14, made for this kernel, of the error over the
+// smaller of 5e-8 and 2^-13 Phi(-|x|): the tail is within 5.8e-8 and within 2^-13 of its own size, so that GELU and its slope
+// hold bf16's rounding far below zero too (down to x = -13, where ex leaves fp32's normal range).
 __device__ __forceinline__ float normal_tail(float x, float& ex) {
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.23164188f, fabsf(x), 1.0f));
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.29f, fabsf(x), 1.0f));
   ex = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);
-  float p = fmaf(t, 0.5307027145f, -0.7265760135f);
-  p = fmaf(t, p, 0.7107068705f);
-  p = fmaf(t, p, -0.142248368f);
-  p = fmaf(t, p, 0.127414796f);
+  float p = fmaf(t, -0.08956327289f, 0.2875475585f);
+  p = fmaf(t, p, -0.09686156362f);
+  p = fmaf(t, p, 0.1819336414f);
+  p = fmaf(t, p, 0.09999677539f);
+  p = fmaf(t, p, 0.1169468239f);
   return p * t * ex;
 }
 // GELU(x) = max(x, 0) - |x| Phi(-|x|).  ENDS: +-inf may come in (inf * 0 otherwise).  NaN stays NaN in both forms.
@@ -32,10 +36,10 @@ __device__ __forceinline__ float gelu(float x, float tail) {
   const float y = fmaf(-fabsf(x), tail, fmaxf(x, 0.f));
   return ENDS && fabsf(x) == INFINITY ? fmaxf(x, 0.f) : y;
 }
-// Phi(x) + x phi(x)
+// Phi(x) + x phi(x).  Below zero Phi is the tail itself: by way of 1 or 1 / 2 the error of those would stay.
 template <bool ENDS>
 __device__ __forceinline__ float gelu_slope(float x, float tail, float ex) {
-  const float c = 0.5f + __builtin_copysignf(0.5f - tail, x);
+  const float c = x < 0.f ? tail : 1.0f - tail;
   return ENDS && fabsf(x) == INFINITY ? c : fmaf(x * 0.39894228040143268f, ex, c);
 }
 

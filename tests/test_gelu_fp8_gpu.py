@@ -169,3 +169,26 @@ def test_offsets_beyond_32_bits():
     dx, again = ops.gelu_fp8_backward(far[1], kept, dx=far[3], again=far[4])
     dx2, again2 = ops.gelu_fp8_backward(dy, kept, recompute=True)
     assert torch.equal(dx, dx2) and torch.equal(again, again2)
+
+
+def test_the_negative_tail():
+    """Far below zero the value and the slope keep their own rounding, not the error of a number next to 1: every bf16 x in
+    [-12.9, -4], a block to each.  Phi(-|x|) is within 2^-13.07 of its value by its polynomial and 2^-16.5 by the exponent of
+    up to 122, which two fp32 roundings leave 122 * 2^-23 * ln 2 off; with ten roundings more, 2^-12.9 in all."""
+    ops = _ops()
+    rel = 2.0 ** -12.9
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    x = bits[(bits >= -12.9) & (bits <= -4)]
+    x = x[:, None].expand(-1, 32).contiguous().cuda()
+    dy = torch.ones_like(x)
+    y, kept = ops.gelu_fp8(x)
+    want = x.double() * cdf(x.double())
+    inside(y, want, (BF + rel) * want.abs(), "y")
+    dx, again = ops.gelu_fp8_backward(dy, kept, recompute=True)
+    k = kept_values(kept)
+    assert (k < -3.7).all()
+    want = k * cdf(k)
+    inside(again, want, (BF + rel) * want.abs(), "again")
+    want = slope(k)
+    terms = cdf(k) + k.abs() * torch.exp(-k.square() / 2) / math.sqrt(2 * math.pi)
+    inside(dx, want, BF * want.abs() + rel * 1.02 * terms, "dx")

@@ -901,11 +901,11 @@ def _rows_dim(t, name, dtypes):
     pitch, dense = t.stride()
     if dim > 1 and dense != 1:
         raise ValueError(f"{name}: the last axis must be dense, its stride is {dense}")
-    return rows, dim, pitch if rows > 1 else max(pitch, dim)
+    return rows, dim, pitch if rows > 1 else dim
 
 
 def _pitch(t):
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _elsewhere(at):

@@ -192,3 +192,18 @@ def test_the_negative_tail():
     want = slope(k)
     terms = cdf(k) + k.abs() * torch.exp(-k.square() / 2) / math.sqrt(2 * math.pi)
     inside(dx, want, BF * want.abs() + rel * 1.02 * terms, "dx")
+
+
+@pytest.mark.parametrize("pitch", [100, 3, 0])
+def test_one_row_has_no_pitch(pitch):
+    ops = _ops()
+    x, dy = inputs(1, 96, 2)
+    want = ops.gelu_fp8(x)
+    wdx, wagain = ops.gelu_fp8_backward(dy, want[1], recompute=True)
+
+    def odd(t):
+        return t.reshape(-1).as_strided((1, 96), (pitch, 1))
+    y, kept = ops.gelu_fp8(odd(x.clone()), out=odd(torch.zeros_like(x)))
+    dx, again = ops.gelu_fp8_backward(odd(dy.clone()), kept, dx=odd(torch.zeros_like(x)), again=odd(torch.zeros_like(x)))
+    for a, b in ((y, want[0]), (kept.data, want[1].data), (kept.scale, want[1].scale), (dx, wdx), (again, wagain)):
+        assert torch.equal(a, b)

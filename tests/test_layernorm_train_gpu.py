@@ -243,3 +243,19 @@ def test_offsets_beyond_32_bits():
     got = ops.layernorm_backward(far[1], far[0], stats, gamma, add=far[2], dx=far[4])
     for a, b in zip(got, ops.layernorm_backward(dy, x, stats, gamma, add=add)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("pitch", [400, 3, 0])
+def test_one_row_has_no_pitch(pitch):
+    ops = _ops()
+    x, gamma, beta, dy, add = case(1, 384, torch.float32, 71)
+    y, stats = ops.layernorm_train(x, gamma, beta, EPS)
+    want = ops.layernorm_backward(dy, x, stats, gamma, add=add)
+
+    def odd(t):
+        return t.reshape(-1).as_strided((1, 384), (pitch, 1))
+    y2, s2 = ops.layernorm_train(odd(x.clone()), gamma, beta, EPS, out=odd(torch.zeros_like(y)))
+    assert torch.equal(y, y2) and torch.equal(stats, s2)
+    got = ops.layernorm_backward(odd(dy.clone()), odd(x.clone()), s2, gamma, add=odd(add.clone()), dx=odd(torch.zeros_like(x)))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

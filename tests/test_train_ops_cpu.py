@@ -231,3 +231,12 @@ def test_sizes_above_31_bits_are_refused():
     cu = _Device(torch.zeros(2, dtype=torch.int32))
     with pytest.raises(ValueError):
         ops._attn_packed_desc(q, k, k, q, None, cu, cu, None, None, False, True)
+
+
+def test_one_row_has_no_pitch():
+    """Its stride is never taken: not that of the buffer that it is a slice of, whatever that is."""
+    bf = torch.bfloat16
+    buf = torch.zeros(5, 100, dtype=bf)
+    for t in (buf[:1, :96], buf.as_strided((1, 96), (3, 1)), buf.as_strided((1, 96), (0, 1)), buf.as_strided((0, 96), (5, 1))):
+        assert ops._rows_dim(_Device(t), "x", (bf,))[1:] == (96, 96) and ops._pitch(t) == 96
+    assert ops._rows_dim(_Device(buf[:2, :96]), "x", (bf,)) == (2, 96, 100) and ops._pitch(buf[:2, :96]) == 100

@@ -1325,11 +1325,16 @@ int check(const char* what, const i2pc_attn_packed_desc* d) {
   return I2PC_OK;
 }
 
+// The row stride of an operand of one row is never taken, but the kernels take the end of a tile's rows from it: rows behind the
+// first have to lie behind its 64 values.
+inline int64_t pitch(int64_t t, int rows) { return rows > 1 ? t : 64; }
+
 Args args_of(const i2pc_attn_packed_desc& d) {
   Args a = {};
   a.q = static_cast<const bf16_t*>(d.q), a.k = static_cast<const bf16_t*>(d.k), a.v = static_cast<const bf16_t*>(d.v);
-  a.q_t = d.q_t, a.q_h = d.q_h, a.k_t = d.k_t, a.k_h = d.k_h, a.v_t = d.v_t, a.v_h = d.v_h;
-  a.out = static_cast<bf16_t*>(d.out), a.o_t = d.o_t, a.o_h = d.o_h, a.lse = d.lse;
+  a.q_t = pitch(d.q_t, d.total_q), a.q_h = d.q_h, a.k_t = pitch(d.k_t, d.total_k), a.k_h = d.k_h;
+  a.v_t = pitch(d.v_t, d.total_k), a.v_h = d.v_h;
+  a.out = static_cast<bf16_t*>(d.out), a.o_t = pitch(d.o_t, d.total_q), a.o_h = d.o_h, a.lse = d.lse;
   a.cu_q = d.cu_q, a.cu_k = d.cu_k, a.k_lens = d.k_lens;
   a.B = d.batch, a.Tq = d.total_q, a.Tk = d.total_k, a.H = d.heads, a.Hk = d.kv_heads, a.G = d.heads / d.kv_heads;
   a.zero_tail = d.zero_tail != 0;
@@ -1421,9 +1426,11 @@ extern "C" int i2pc_attention_packed_backward(const i2pc_attn_packed_grad_desc* 
     return set_error(I2PC_EWORKSPACE, "attention_packed_backward: workspace of %zu bytes, needs %zu (16-byte aligned)",
                      workspace_bytes, need);
   attnp::Args a = attnp::args_of(d);
-  a.dout = static_cast<const attn::bf16_t*>(g->dout), a.d_t = g->d_t, a.d_h = g->d_h;
+  a.dout = static_cast<const attn::bf16_t*>(g->dout), a.d_t = attnp::pitch(g->d_t, d.total_q), a.d_h = g->d_h;
   a.dq = static_cast<attn::bf16_t*>(g->dq), a.dk = static_cast<attn::bf16_t*>(g->dk), a.dv = static_cast<attn::bf16_t*>(g->dv);
-  a.dq_t = g->dq_t, a.dq_h = g->dq_h, a.dk_t = g->dk_t, a.dk_h = g->dk_h, a.dv_t = g->dv_t, a.dv_h = g->dv_h;
+  a.dq_t = attnp::pitch(g->dq_t, d.total_q), a.dq_h = g->dq_h;
+  a.dk_t = attnp::pitch(g->dk_t, d.total_k), a.dk_h = g->dk_h;
+  a.dv_t = attnp::pitch(g->dv_t, d.total_k), a.dv_h = g->dv_h;
   a.nlse = static_cast<float*>(workspace);
   a.ndelta = a.nlse + (size_t)a.Tq * a.H;
   hipStream_t s = as_stream(stream);

@@ -653,3 +653,28 @@ def test_profiled_calls_are_listed(monkeypatch):
     assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
     assert [s[0] for s in seen] == ["k_attnp_fwd", "k_attnp_bwd", "k_lnt_fwd", "k_lnt_bwd", "k_gelu_keep", "k_gelu_back"]
     assert all(s[2] > 0 and s[3].elapsed_time(s[4]) >= 0 for s in seen)
+
+
+@pytest.mark.parametrize("pitch", [0, 8])
+def test_one_row_has_no_pitch(pitch):
+    """The stride from row to row of an operand of one row is never taken."""
+    ops = _ops()
+    H = 4
+    q, k, v, dout = make([1], heads=H, seed=6)
+    q70, k70, v70, d70 = make([70], heads=H, seed=7)
+
+    def one(t):
+        return t.reshape(H, 64).as_strided((1, H, 64), (pitch, 64, 1))
+    c1, c70 = cu([1]), cu([70])
+    for qs, ks, c, ck in (((q, dout), (k70, v70), c1, c70), ((q70, d70), (k, v), c70, c1), ((q, dout), (k, v), c1, c1)):
+        a, b = [t.clone() for t in qs + ks], [one(t.clone()) if t.shape[0] == 1 else t for t in qs + ks]
+        out, lse = ops.attention_packed(a[0], a[2], a[3], c, ck)
+        o2 = torch.empty_like(out) if out.shape[0] > 1 else one(torch.empty_like(out))
+        l2 = torch.empty_like(lse)
+        ops.attention_packed(b[0], b[2], b[3], c, ck, out=o2, lse=l2)
+        assert torch.equal(out, o2) and torch.equal(lse, l2)
+        want = ops.attention_packed_backward(a[1], a[0], a[2], a[3], out, lse, c, ck)
+        got = [one(torch.empty_like(t)) if t.shape[0] == 1 else torch.empty_like(t) for t in want]
+        ops.attention_packed_backward(b[1], b[0], b[2], b[3], o2, l2, c, ck, dq=got[0], dk=got[1], dv=got[2])
+        for x, y in zip(want, got):
+            assert torch.equal(x, y)

@@ -1290,12 +1290,13 @@ inline KeySplit key_split(const i2pc_attn_packed_desc& d) {
 }
 
 // Rows apart (the range checks of the tiles' loads go by the row stride); where they are written heads apart too, and the
-// heads of a row all before the next row or the rows of a head all before the next head.
+// heads of a row all before the next row or the rows of a head all before the next head.  The stride of a single row or head is
+// not looked at.
 inline bool rows_ok(const void* p, int64_t t, int64_t h, int rows, int heads, bool written) {
   if (rows == 0) return true;
-  if (!p || reinterpret_cast<uintptr_t>(p) % 16 || t % 8 || h % 8 || t < 0 || t >= (int64_t)1 << 23 || h < 0 || h >= (int64_t)1 << 40 ||
-      (rows > 1 && t < 64))
-    return false;
+  if (!p || reinterpret_cast<uintptr_t>(p) % 16) return false;
+  if (rows > 1 && (t % 8 || t < 64 || t >= (int64_t)1 << 23)) return false;
+  if (heads > 1 && (h % 8 || h < 0 || h >= (int64_t)1 << 40)) return false;
   if (!written || heads == 1) return true;
   return h >= 64 && (rows == 1 || t >= (heads - 1) * h + 64 || h >= (rows - 1) * t + 64);
 }

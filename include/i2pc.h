@@ -595,8 +595,9 @@ int i2pc_gelu_fp8_backward(const void* dy, int64_t lddy, const void* kept, const
  * is given -- a cache with a slab of slots for each sequence.  cu_q, cu_k: int32 [batch + 1] on the device, rising,
  * cu_q[0] = 0; the kernels read them when they run, so a captured graph follows their contents, and hold what they
  * say to total_q / total_k rows.  Element (row t, head h) of q starts at q + t * q_t + h * q_h elements (out, k, v
- * alike) and its head_dim = 64 bf16 values are dense; query head h reads key head h / (heads / kv_heads).  No output may
- * overlap an input or itself.
+ * alike) and its head_dim = 64 bf16 values are dense, 16-byte aligned; query head h reads key head h / (heads / kv_heads).
+ * The row stride of a single row and the head stride of a single head do not matter.  No output may overlap an input or
+ * itself.
  *   S = scale Q K^T; causal: query i of a sequence of lq queries and lk keys sees keys j <= i + lk - lq;
  *   out = softmax(S) V, lse [total_q][heads] = log(sum exp(S)) (fp32); a query that sees no key has out = 0,
  *   lse = -inf.

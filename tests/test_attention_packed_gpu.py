@@ -655,7 +655,7 @@ def test_profiled_calls_are_listed(monkeypatch):
     assert all(s[2] > 0 and s[3].elapsed_time(s[4]) >= 0 for s in seen)
 
 
-@pytest.mark.parametrize("pitch", [0, 8])
+@pytest.mark.parametrize("pitch", [0, 8, 3, 1 << 24])
 def test_one_row_has_no_pitch(pitch):
     """The stride from row to row of an operand of one row is never taken."""
     ops = _ops()
@@ -678,3 +678,15 @@ def test_one_row_has_no_pitch(pitch):
         ops.attention_packed_backward(b[1], b[0], b[2], b[3], o2, l2, c, ck, dq=got[0], dk=got[1], dv=got[2])
         for x, y in zip(want, got):
             assert torch.equal(x, y)
+
+
+def test_one_head_has_no_pitch():
+    ops = _ops()
+    q, k, v, dout = make([70], heads=1, seed=6)
+    out, lse = ops.attention_packed(q, k, v, cu([70]))
+    odd = [t.as_strided((70, 1, 64), (64, 3, 1)) for t in (q, k, v, out, dout)]
+    o2, l2 = ops.attention_packed(*odd[:3], cu([70]))
+    assert torch.equal(out, o2) and torch.equal(lse, l2)
+    for a, b in zip(ops.attention_packed_backward(dout, q, k, v, out, lse, cu([70])),
+                    ops.attention_packed_backward(odd[4], *odd[:3], odd[3], lse, cu([70]))):
+        assert torch.equal(a, b)

@@ -240,3 +240,13 @@ def test_one_row_has_no_pitch():
     for t in (buf[:1, :96], buf.as_strided((1, 96), (3, 1)), buf.as_strided((1, 96), (0, 1)), buf.as_strided((0, 96), (5, 1))):
         assert ops._rows_dim(_Device(t), "x", (bf,))[1:] == (96, 96) and ops._pitch(t) == 96
     assert ops._rows_dim(_Device(buf[:2, :96]), "x", (bf,)) == (2, 96, 100) and ops._pitch(buf[:2, :96]) == 100
+
+
+def test_strides_of_one_row_or_head_do_not_matter():
+    _built()
+    lib = _lib.load()
+    for kw in ({"total_q": 1, "q_t": 3, "o_t": 1 << 40}, {"total_k": 1, "k_t": -5, "v_t": 0},
+               {"heads": 1, "kv_heads": 1, "q_h": 3, "k_h": -1, "v_h": 1 << 50, "o_h": 1}):
+        assert lib.i2pc_attention_packed_backward_workspace_bytes(ctypes.byref(_grad(**kw))) > 0, kw
+    for kw in ({"total_q": 2, "q_t": 3}, {"heads": 2, "kv_heads": 2, "q_h": 3}, {"total_k": 1, "k": 24}):
+        assert lib.i2pc_attention_packed_backward_workspace_bytes(ctypes.byref(_grad(**kw))) == 0, kw

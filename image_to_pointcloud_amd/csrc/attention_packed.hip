@@ -542,9 +542,12 @@ __global__ __launch_bounds__(256, 4) void k_attnp_fwd(const Args a) {
     if (kw == 1) return;
     const float m1 = ml[0][rw][lane], l1 = ml[1][rw][lane];
     if (l1 != 0.f) {                                 // (NaN: joined too)
-      const float mm = l == 0.f ? m1 : fmaxf(m, m1);
-      const float f0 = m == mm ? 1.f : __builtin_amdgcn_exp2f(m - mm), f1 = m1 == mm ? 1.f : __builtin_amdgcn_exp2f(m1 - mm);
-      l = l == 0.f ? l1 * f1 : fmaf(l, f0, l1 * f1);
+      // a half without a probability has no say: its reference may lie anywhere
+      const bool empty = l == 0.f;
+      const float mm = empty ? m1 : fmaxf(m, m1);
+      const float f0 = empty ? 0.f : m == mm ? 1.f : __builtin_amdgcn_exp2f(m - mm);
+      const float f1 = m1 == mm ? 1.f : __builtin_amdgcn_exp2f(m1 - mm);
+      l = fmaf(l, f0, l1 * f1);
       m = mm;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {

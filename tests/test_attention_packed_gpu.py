@@ -690,3 +690,20 @@ def test_one_head_has_no_pitch():
     for a, b in zip(ops.attention_packed_backward(dout, q, k, v, out, lse, cu([70])),
                     ops.attention_packed_backward(odd[4], *odd[:3], odd[3], lse, cu([70]))):
         assert torch.equal(a, b)
+
+
+def test_a_half_without_a_probability_beside_a_masked_nan():
+    """Two waves share a row's keys.  The rows from 32 on see 49 to 80 keys; the first 32 have scores of -inf, so that one wave
+    has no probability for the rows up to 64 keys, and a NaN that the mask hides has it done again."""
+    ops = _ops()
+    q, k, v, _ = make([100], [116], heads=2, seed=4)
+    q, k = q.abs() + 0.5, -k.abs() * 16 - 8                   # scores of some hundreds below zero
+    k[:32, :, 0] = -INF
+    v[90] = float("nan")
+    out, lse = ops.attention_packed(q, k, v, cu([100]), cu([116]), causal=True)
+    v2 = v.clone()
+    v2[90] = 0
+    ref = reference(q[16:], k[32:], v2[32:], [84], [84], True, 0.125)
+    inside(out[16:74], ref["out"][:58], ref["out_b"][:58], "out")
+    inside(lse[16:], ref["lse"], ref["lse_b"], "lse")
+    assert out[74:].isnan().all()

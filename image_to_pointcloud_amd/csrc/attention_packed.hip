@@ -17,6 +17,7 @@
 #include "common.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 namespace i2pc {
@@ -44,7 +45,7 @@ struct Args {
   int B, Tq, Tk, H, Hk, G, zero_tail, nsplit;
   float c;                       // scale * log2(e)
   float* part_o;                 // [nsplit][Hk][Tq * G][64], rows normalised
-  float* part_l;                 // [nsplit][Hk][Tq * G], log2(sum exp) or -inf
+  float2* part_l;                // [nsplit][Hk][Tq * G], a row's reference and its sum
   // backward
   const bf16_t* dout;
   int64_t d_t, d_h;
@@ -331,24 +332,29 @@ __device__ __forceinline__ void zero_rows(bf16_t* out, int64_t o_t, int64_t o_h,
 // A row's running state, a row to a lane (its two lane halves hold different keys' probabilities and different d of O).
 struct Rows {
   f32x16 o[2];                   // O^T, not normalised
-  float m;                       // the reference, c times a raw score
-  float l;                       // this half's sum of 2^(c s - m)
+  float m;                       // the reference, a raw score
+  float l;                       // this half's sum of 2^(c (s - m))
   int bad;                       // met an infinity or NaN in a partly masked block
+  bool far;                      // (uniform) c m of some row is too large for a product that is not rounded beside one that is
   __device__ __forceinline__ void clear() {
     for (int i = 0; i < 16; ++i) o[0][i] = o[1][i] = 0.f;
     m = l = 0.f;
     bad = 0;
+    far = false;
   }
 };
 
-// 32 keys (at bytes atK, atV behind the addresses' tile) for 32 rows: p = 2^(c s - m), one FMA and one exponential a
+// 32 keys (at bytes atK, atV behind the addresses' tile) for 32 rows: p = 2^(c s - c m), one FMA and one exponential a
 // score.  m moves only when a probability could pass 2^8 (harmless for the bf16 operand and the fp32 sums), so the usual
 // block has no maximum and no rescale.  `first`: the rows' first block, which sets m.  left: how many of the block's keys
 // the lane's row sees; partial (uniform): not all of them for some row of the wave.
+// c m is rounded and c s within the FMA is not: the exponent of s = m is off by up to 2^-25 |c m|, the same for a row's every
+// score, which the sum takes out again -- until it leaves the exponential's range.  Rows whose |c m| is above 2^12 (`far`) take
+// 2^(c (s - m)) instead, with their maximum anew in each block.
 template <bool CAUSAL>
 __device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const Lanes& ad, uint32_t atK, uint32_t atV, bool first,
                                        bool partial, int left, float c, int hh) {
-  constexpr float kThresh = 256.f;
+  constexpr float kThresh = 256.f, kFar = 4096.f;
   bf16x8 kf[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) kf[t] = ad.rows(t, atK);
@@ -368,18 +374,18 @@ __device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const Lan
   }
   float ls = 0.f;
   uint32_t pk[8];
-  auto probs = [&]() {
+  auto probs = [&](float mc) {
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
-      const float p0 = __builtin_amdgcn_exp2f(fmaf(st[i], c, -w.m));
-      const float p1 = __builtin_amdgcn_exp2f(fmaf(st[i + 1], c, -w.m));
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(st[i], c, -mc));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(st[i + 1], c, -mc));
       ls = i ? ls + (p0 + p1) : p0 + p1;
       pk[i >> 1] = pack_bf16(p0, p1);
     }
   };
-  bool full = first;
+  bool full = first || w.far;
   if (!full) {
-    probs();
+    probs(w.m * c);
     full = __ballot(ls >= kThresh) != 0;
   }
   if (full) {
@@ -387,11 +393,13 @@ __device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const Lan
 #pragma unroll
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[i]);
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-    mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * c;
-    // a row that sees nothing here keeps its reference; one whose first 32 scores are all -inf gets one below any score
-    const float m_new = first ? fmaxf(mx, -1e30f) : fmaxf(mx, w.m);
+    mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+    // a row that sees nothing here keeps its reference; one whose first 32 scores are all -inf gets one below the others that is
+    // finite, and times c too
+    const float low = -0x1p126f * __builtin_amdgcn_rcpf(fmaxf(c, 1.f));
+    const float m_new = first ? (mx == -INFINITY ? low : mx) : fmaxf(mx, w.m);
     if (!first) {
-      const float alpha = __builtin_amdgcn_exp2f(w.m - m_new);
+      const float alpha = __builtin_amdgcn_exp2f((w.m - m_new) * c);
       w.l *= alpha;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -400,7 +408,14 @@ __device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const Lan
       }
     }
     w.m = m_new;
-    probs();
+    float mc = m_new * c;
+    w.far = __ballot(fabsf(mc) > kFar && m_new != low) != 0;
+    if (__builtin_expect(w.far, 0)) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st[i] -= m_new;
+      mc = 0.f;
+    }
+    probs(mc);
   }
   w.l += ls;
   if (CAUSAL && partial) w.bad |= has_nonfinite(ad, atV);
@@ -410,6 +425,13 @@ __device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const Lan
     for (int dt = 0; dt < 2; ++dt) w.o[dt] = mfma(vf[t][dt], p_frag(pk, t), w.o[dt]);
 }
 
+// log(sum exp(scale s)) of a row from its reference and sum: -inf for a row that saw no key (or only scores of -inf), and for
+// no other
+__device__ __forceinline__ float lse_of(float m, float l, float scale) {
+  const float x = fmaf(m, scale, log2f(l) * 0.69314718055994531f);
+  return l != 0.f && x == -INFINITY ? -FLT_MAX : x;
+}
+
 // The state of the keys [from, to) again, key by key: rows that `bad` says need it.
 __device__ __forceinline__ void attend_again(Rows& w, const bf16x8 (&qf)[4], const bf16_t* K, int64_t k_t, const bf16_t* V,
                                              int64_t v_t, int from, int to, int step, int nk, float c, int hh) {
@@ -417,10 +439,10 @@ __device__ __forceinline__ void attend_again(Rows& w, const bf16x8 (&qf)[4], con
   w.clear();
 #pragma clang loop unroll(disable)
   for (int j = from; j < to; j += (j & 31) == 31 ? step : 1) {
-    const float x = dot_row(K + j * k_t, qf, hh) * c;
+    const float x = dot_row(K + j * k_t, qf, hh);
     if (j < nk) {
-      const float m_new = fmaxf(m, x), alpha = m == m_new ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
-      const float p = x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - m_new);
+      const float m_new = fmaxf(m, x), alpha = m == m_new ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
+      const float p = x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x - m_new) * c);
       m = m_new;
       l = fmaf(l, alpha, p);
       for (int i = 0; i < 16; ++i) {
@@ -545,8 +567,8 @@ __global__ __launch_bounds__(256, 4) void k_attnp_fwd(const Args a) {
       // a half without a probability has no say: its reference may lie anywhere
       const bool empty = l == 0.f;
       const float mm = empty ? m1 : fmaxf(m, m1);
-      const float f0 = empty ? 0.f : m == mm ? 1.f : __builtin_amdgcn_exp2f(m - mm);
-      const float f1 = m1 == mm ? 1.f : __builtin_amdgcn_exp2f(m1 - mm);
+      const float f0 = empty ? 0.f : m == mm ? 1.f : __builtin_amdgcn_exp2f((m - mm) * c);
+      const float f1 = m1 == mm ? 1.f : __builtin_amdgcn_exp2f((m1 - mm) * c);
       l = fmaf(l, f0, l1 * f1);
       m = mm;
 #pragma unroll
@@ -558,11 +580,10 @@ __global__ __launch_bounds__(256, 4) void k_attnp_fwd(const Args a) {
   }
   if (r >= R) return;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  const float l2 = l == 0.f ? -INFINITY : m + log2f(l);
   if (SPLIT) {
     const int64_t row = ((int64_t)split * a.Hk + hk) * a.Tq * a.G + (int64_t)s.q0 * a.G + r;
-    if (hh == 0) a.part_l[row] = l2;
-    if (l2 != -INFINITY) {
+    if (hh == 0) a.part_l[row] = make_float2(m, l);
+    if (l != 0.f) {
 #pragma unroll
       for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
@@ -572,7 +593,7 @@ __global__ __launch_bounds__(256, 4) void k_attnp_fwd(const Args a) {
     }
   } else {
     store_acc(a.out + (s.q0 + qi) * a.o_t + h * a.o_h, w.o, inv, hh);
-    if (hh == 0) a.lse[(int64_t)(s.q0 + qi) * a.H + h] = l2 * 0.69314718055994531f;
+    if (hh == 0) a.lse[(int64_t)(s.q0 + qi) * a.H + h] = lse_of(m, l, a.scale);
   }
 }
 
@@ -663,7 +684,7 @@ __global__ __launch_bounds__(256, 2) void k_attnp_few(const Args a) {
   if (CAUSAL && __ballot(w.bad) != 0) attend_again(w, qf, Kg, a.k_t, Vg, a.v_t, first, ke, 97, nk, c, hh);
   const float l = w.l + __shfl_xor(w.l, 32);
 
-  // the four waves' sums: sum_w f_w O_w, f_w = 2^(m_w - m)
+  // the four waves' sums: sum_w f_w O_w, f_w = 2^(c (m_w - m))
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   float* ow = reinterpret_cast<float*>(mine);
 #pragma unroll
@@ -686,32 +707,31 @@ __global__ __launch_bounds__(256, 2) void k_attnp_few(const Args a) {
   for (int v = 0; v < 4; ++v) {
     const float lv = ml[1][v][row];
     if (lv == 0.f) continue;                         // saw nothing (a NaN sum is not skipped)
-    const float mv = ml[0][v][row], f = mv == m ? 1.f : __builtin_amdgcn_exp2f(mv - m);
+    const float mv = ml[0][v][row], f = mv == m ? 1.f : __builtin_amdgcn_exp2f((mv - m) * c);
     total = fmaf(f, lv, total);
     const float* x = reinterpret_cast<const float*>(smem + v * 4 * kFewBlock) + row * 68 + d;
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = fmaf(f, x[i], acc[i]);
   }
   const float inv = total == 0.f ? 0.f : 1.0f / total;
-  const float l2 = total == 0.f ? -INFINITY : m + log2f(total);
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] *= inv;
   const int i = r / a.G, hq = hk * a.G + r - i * a.G;
   if (a.nsplit == 1) {
     *reinterpret_cast<uint4*>(a.out + (s.q0 + i) * a.o_t + hq * a.o_h + d) =
         make_uint4(pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3]), pack_bf16(acc[4], acc[5]), pack_bf16(acc[6], acc[7]));
-    if (d == 0) a.lse[(int64_t)(s.q0 + i) * a.H + hq] = l2 * 0.69314718055994531f;
+    if (d == 0) a.lse[(int64_t)(s.q0 + i) * a.H + hq] = lse_of(m, total, a.scale);
   } else {
     const int64_t at = ((int64_t)split * a.Hk + hk) * a.Tq * a.G + (int64_t)s.q0 * a.G + r;
-    if (d == 0) a.part_l[at] = l2;
-    if (l2 != -INFINITY) {
+    if (d == 0) a.part_l[at] = make_float2(m, total);
+    if (total != 0.f) {
       *reinterpret_cast<float4*>(a.part_o + at * 64 + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
       *reinterpret_cast<float4*>(a.part_o + at * 64 + d + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
     }
   }
 }
 
-// The shares of a split call joined, W waves to a row: out = sum_s 2^(l_s - m) O_s / sum_s 2^(l_s - m).  Wave v takes the
+// The shares of a split call joined, W waves to a row: out = sum_s w_s O_s / sum_s w_s, w_s = l_s 2^(c (m_s - m)).  Wave v takes the
 // shares 8 v .. 8 v + 7, then 8 W further, eight loads in flight; a lane is a d.  Bound by the latency of two dependent
 // reads: 4 to 5 us.
 template <int W>
@@ -724,14 +744,18 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_attnp_join(const Args
   const bool tail = t >= cu_at(a.cu_q, a.B, a.Tq);
   if (tail && !a.zero_tail) return;
   const int64_t step = rows * a.Hk;                  // from share to share
-  const float* pl = a.part_l + hk * rows + row;
+  const float2* pl = a.part_l + hk * rows + row;
   const float* po = a.part_o + (hk * rows + row) * 64 + lane;
   float acc = 0.f, m = -INFINITY, total = 0.f;
   if (!tail) {
-    for (int s = lane; s < a.nsplit; s += 64) m = fmaxf(m, pl[s * step]);
+    for (int s = lane; s < a.nsplit; s += 64) {
+      const float2 x = pl[s * step];
+      m = fmaxf(m, x.y == 0.f ? -INFINITY : x.x);
+    }
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
     for (int s0 = 8 * v; s0 < a.nsplit; s0 += 8 * W) {
-      float l[8], o[8];
+      float2 l[8];
+      float o[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) l[j] = pl[min(s0 + j, a.nsplit - 1) * step];
 #pragma unroll
@@ -739,8 +763,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_attnp_join(const Args
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         // an empty share wrote no O; NaN shares (a NaN or infinite score) stay NaN
-        const bool on = s0 + j < a.nsplit && l[j] != -INFINITY;
-        const float w = on ? __builtin_amdgcn_exp2f(l[j] - m) : 0.f;
+        const bool on = s0 + j < a.nsplit && l[j].y != 0.f;
+        const float w = on ? l[j].y * __builtin_amdgcn_exp2f((l[j].x - m) * a.c) : 0.f;
         total += w;
         acc = on ? fmaf(w, o[j], acc) : acc;
       }
@@ -761,7 +785,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_attnp_join(const Args
   }
   const __bf16 o = (__bf16)(total == 0.f ? 0.f : acc / total);
   a.out[t * a.o_t + h * a.o_h + lane] = __builtin_bit_cast(bf16_t, o);
-  if (lane == 0) a.lse[(int64_t)t * a.H + h] = total == 0.f ? -INFINITY : (m + log2f(total)) * 0.69314718055994531f;
+  if (lane == 0) a.lse[(int64_t)t * a.H + h] = lse_of(m, total, a.scale);
 }
 
 // ------------------------------------------------------------------ backward
@@ -1356,7 +1380,7 @@ using namespace i2pc;
 extern "C" size_t i2pc_attention_packed_workspace_bytes(const i2pc_attn_packed_desc* d) {
   if (attnp::check("attention_packed", d) != I2PC_OK) return 0;
   const int n = attnp::splits(*d);
-  return n == 1 ? 0 : (size_t)n * d->heads * d->total_q * 65 * sizeof(float);
+  return n == 1 ? 0 : (size_t)n * d->heads * d->total_q * 66 * sizeof(float);
 }
 
 extern "C" int i2pc_attention_packed(const i2pc_attn_packed_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
@@ -1375,7 +1399,7 @@ extern "C" int i2pc_attention_packed(const i2pc_attn_packed_desc* d, void* works
   const dim3 block(256), grid((uint32_t)(attnp::row_tiles(*d, few ? attnp::kFew : attnp::kRows / kw) * a.Hk * a.nsplit));
   if (a.nsplit > 1) {
     a.part_o = static_cast<float*>(workspace);
-    a.part_l = a.part_o + (size_t)a.nsplit * a.H * a.Tq * 64;
+    a.part_l = reinterpret_cast<float2*>(a.part_o + (size_t)a.nsplit * a.H * a.Tq * 64);
   }
   if (few && d->causal) hipLaunchKernelGGL(attnp::k_attnp_few<true>, grid, block, 0, s, a);
   else if (few) hipLaunchKernelGGL(attnp::k_attnp_few<false>, grid, block, 0, s, a);

@@ -599,8 +599,8 @@ int i2pc_gelu_fp8_backward(const void* dy, int64_t lddy, const void* kept, const
  * The row stride of a single row and the head stride of a single head do not matter.  No output may overlap an input or
  * itself.
  *   S = scale Q K^T; causal: query i of a sequence of lq queries and lk keys sees keys j <= i + lk - lq;
- *   out = softmax(S) V, lse [total_q][heads] = log(sum exp(S)) (fp32); a query that sees no key has out = 0,
- *   lse = -inf.
+ *   out = softmax(S) V, lse [total_q][heads] = log(sum exp(S)) (fp32; beyond its range inf or the lowest finite value);
+ *   a query that sees no key has out = 0, lse = -inf.  Scores may have any size that fp32 holds before the scale.
  * Rows behind the last sequence are left as they were, or zero (lse -inf) with zero_tail. */
 typedef struct i2pc_attn_packed_desc {
   const void *q, *k, *v;

@@ -1,0 +1,164 @@
+"""Packed attention where scores are large, against the formulas in 64 bits.
+
+Most cases have whole numbers times powers of two as q and k, so that every score is exact in fp32 whatever the order of its sum:
+what is left of a probability's error is its exponent, 2^-24 of at most 150 in a few roundings, and the exponential's, below
+`ES` = 2^-15 together.  The roundings to bf16 are counted as everywhere: P and dS before their products, the output that
+D = rowsum(dO out) is taken from, the results."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+BF, ES = 2.0 ** -8, 2.0 ** -15
+INF = math.inf
+
+
+def _ops():
+    from image_to_pointcloud_amd import ops
+    return ops
+
+
+def cu(lens):
+    return torch.tensor([0] + list(lens), dtype=torch.int32).cumsum(0).to(torch.int32).cuda()
+
+
+def inputs(kind, e, tq, tk, heads, kv, seed):
+    """q, k, v, dout (bf16, on the device).  ties: scores 2^(2e) times whole numbers around zero; low: the same below zero;
+    offset, -offset: whole numbers behind +-2^(2e)."""
+    gen = torch.Generator().manual_seed(seed)
+    q, k = (torch.randint(-1, 2, (t, h, 64), generator=gen).float() for t, h in ((tq, heads), (tk, kv)))
+    if kind == "ties":
+        q, k = q * 2.0 ** e, k * 2.0 ** e
+    elif kind == "low":
+        q, k = q.abs(), -k.abs()
+        q[..., 0], k[..., 0] = 1, -1
+        q, k = q * 2.0 ** e, k * 2.0 ** e
+    else:
+        q[..., 0], k[..., 0] = 2.0 ** e, 2.0 ** e * (-1 if kind[0] == "-" else 1)
+    v, dout = (torch.randn(t, h, 64, generator=gen) for t, h in ((tk, kv), (tq, heads)))
+    return tuple(t.to(torch.bfloat16).cuda() for t in (q, k, v, dout))
+
+
+def reference(q, k, v, ql, kl, causal, scale, dout=None, starts=None, rounded=0.0, es=None):
+    """Values and bounds.  rounded: the share of |lse| by which a probability of the backward pass may be off; es: a function of
+    the summed magnitudes of a score's terms instead of ES."""
+    q, k, v = (t.double().cpu() for t in (q, k, v))
+    H, Hk = q.shape[1], k.shape[1]
+    names = [("out", q)]
+    r = {"lse": torch.full(q.shape[:2], -INF, dtype=torch.float64)}
+    if dout is not None:
+        dout = dout.double().cpu()
+        names += [("dq", q), ("dk", k), ("dv", v)]
+    for n, t in names:
+        r[n], r[n + "_b"] = torch.zeros_like(t), torch.zeros_like(t)
+    r["lse_b"] = torch.zeros_like(r["lse"])
+    q0 = k0 = 0
+    for b, (a, n) in enumerate(zip(ql, kl)):
+        if starts is not None:
+            k0 = starts[b]
+        for h in range(H if a and n else 0):
+            g = h // (H // Hk)
+            rows, keys = slice(q0, q0 + a), slice(k0, k0 + n)
+            Q, K, V = q[rows, h], k[keys, g], v[keys, g]
+            S = scale * (Q @ K.T)
+            on = torch.ones(a, n, dtype=torch.bool)
+            if causal:
+                on = torch.arange(n)[None, :] <= torch.arange(a)[:, None] + n - a
+            S = S.masked_fill(~on, -INF)
+            top = S.amax(1, keepdim=True)
+            top = torch.where(top == -INF, torch.zeros_like(top), top)
+            W = torch.exp(S - top)
+            total = W.sum(1, keepdim=True)
+            P = W / torch.where(total == 0, torch.ones_like(total), total)
+            lse = (top + torch.log(total))[:, 0]
+            A, O = P @ V.abs(), P @ V
+            e = torch.full_like(total, ES) if es is None else es((P * (scale * (Q.abs() @ K.abs().T))).sum(1, keepdim=True))
+            r["out"][rows, h], r["lse"][rows, h] = O, lse
+            r["out_b"][rows, h] = BF * O.abs() + (BF * 1.02 + 2 * e) * A
+            # scale log2(e), its product with the reference, the sum with log2 of the sum, ln 2: a half step each
+            r["lse_b"][rows, h] = 2.0 ** -22 * lse.abs().nan_to_num(posinf=0.0, neginf=0.0) + 2.0 ** -18 + e[:, 0]
+            if dout is not None:
+                e = e + rounded * lse.abs().nan_to_num(posinf=0.0)[:, None]
+                G = dout[rows, h]
+                r["dv"][keys, g] += P.T @ G
+                r["dv_b"][keys, g] += P.T @ ((BF * 1.02 + 2 * e) * G.abs())
+                D, dP = (G * O).sum(1, keepdim=True), G @ V.T
+                eD = (G.abs() * r["out_b"][rows, h]).sum(1, keepdim=True) * 1.02
+                Z = P * (dP - D)
+                eZ = 1.02 * (BF * Z.abs() + P * eD + 3 * e * P * (G.abs() @ V.abs().T + D.abs()))
+                r["dq"][rows, h] = scale * Z @ K
+                r["dq_b"][rows, h] = scale * 1.02 * (eZ @ K.abs() + ES * (Z.abs() @ K.abs()))
+                r["dk"][keys, g] += scale * Z.T @ Q
+                r["dk_b"][keys, g] += scale * 1.02 * (eZ.T @ Q.abs() + ES * (Z.abs().T @ Q.abs()))
+        q0, k0 = q0 + a, k0 + n
+    if dout is not None:
+        for n in ("dq", "dk", "dv"):
+            r[n + "_b"] += BF * r[n].abs()
+    return r
+
+
+def inside(got, r, name, rows=slice(None)):
+    got, want, bound = got.detach().double().cpu()[rows], r[name][rows], r[name + "_b"][rows]
+    off = (got - want).abs()
+    ok = (got == want) | (off <= bound + 1e-30)
+    assert ok.all(), (f"{name}: {int((~ok).sum())} of {ok.numel()} values off, worst by {((off - bound)[~ok]).max():.3e} "
+                      f"(NaN: {int(got.isnan().sum())})")
+
+
+# scores of 2^35, 2^28, 2^40 and 2^64 by the operands or the scale; of -2^36 and below; around +-2^19 a few steps apart
+KINDS = [("ties", 16, 0.125), ("ties", 0, 2.0 ** 28), ("ties", 0, 2.0 ** 40), ("ties", 0, 2.0 ** 64), ("low", 16, 0.125),
+         ("low", 20, 2.0 ** 64), ("offset", 11, 0.125), ("-offset", 11, 0.125)]
+IDS = [f"{n}-{e}-{math.log2(s):g}" for n, e, s in KINDS]
+
+
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("kind,e,scale", KINDS, ids=IDS)
+def test_large_scores(kind, e, scale, causal):
+    """One tile, a pack that fills the chip, keys in shares."""
+    ops = _ops()
+    for ql, kl, heads, kv in (([200, 31], [200, 31], 2, 2), ([100], [3000], 2, 2), ([3, 17], [400, 30], 4, 2),
+                              ([577, 130, 577, 1, 577, 577, 577, 0, 577, 577], None, 26, 26)):
+        kl = kl or ql
+        q, k, v, _ = inputs(kind, e, sum(ql), sum(kl), heads, kv, heads)
+        out, lse = ops.attention_packed(q, k, v, cu(ql), cu(kl), scale=scale, causal=causal)
+        r = reference(q, k, v, ql, kl, causal, scale)
+        inside(out, r, "out"), inside(lse, r, "lse")
+
+
+@pytest.mark.parametrize("kind,e,scale", KINDS, ids=IDS)
+def test_large_scores_over_a_cache(kind, e, scale):
+    """Single tokens and short chunks over slabs, whose keys are walked in shares of unlike numbers of keys."""
+    ops = _ops()
+    slab = 6200
+    for ql, lens in (([1, 1, 1], [300, 6011, 700]), ([1], [300]), ([3, 1, 0, 9], [2000, 1, 40, 5003])):
+        q, k, v, _ = inputs(kind, e, sum(ql), slab * len(ql), 8, 2, len(ql))
+        out, lse = ops.attention_packed(q, k, v, cu(ql), cu([slab] * len(ql)), k_lens=torch.tensor(lens, dtype=torch.int32).cuda(),
+                                        scale=scale, causal=True)
+        r = reference(q, k, v, ql, lens, True, scale, starts=[b * slab for b in range(len(ql))])
+        inside(out, r, "out"), inside(lse, r, "lse")
+
+
+@pytest.mark.parametrize("kind,e,scale", KINDS, ids=IDS)
+def test_large_scores_before_a_masked_nan(kind, e, scale):
+    """The rows that a NaN behind the mask has done again."""
+    ops = _ops()
+    q, k, v, _ = inputs(kind, e, 180, 180, 2, 1, 5)
+    r = reference(q, k, v, [180], [180], True, scale)
+    k[179], v[179] = float("nan"), float("nan")
+    out, lse = ops.attention_packed(q, k, v, cu([180]), scale=scale, causal=True)
+    inside(out, r, "out", slice(0, 179)), inside(lse, r, "lse", slice(0, 179))
+
+
+def test_scores_beyond_the_largest_float():
+    """Scaled scores of about 2^131: the softmax is of their differences, lse is the nearest fp32 has."""
+    ops = _ops()
+    q, k, v, _ = inputs("low", 32, 70, 70, 1, 1, 3)
+    for sign in (1, -1):
+        r = reference(q, sign * k, v, [70], [70], False, 2.0 ** 64)
+        out, lse = ops.attention_packed(q, sign * k, v, cu([70]), scale=2.0 ** 64)
+        inside(out, r, "out")
+        # above the largest float infinity; -inf is a query that sees no key
+        over = r["lse"].abs() > 2.0 ** 128
+        assert over.any() and ((lse.cpu() == INF) if sign < 0 else (lse.cpu() == -torch.finfo(torch.float32).max))[over].all()

@@ -52,7 +52,8 @@ struct Args {
   bf16_t *dq, *dk, *dv;
   int64_t dq_t, dq_h, dk_t, dk_h, dv_t, dv_h;
   float scale;
-  float *nlse, *ndelta;          // [H][Tq]: -lse / scale and -D
+  float *nlse, *ndelta;          // [H][Tq]: -lse / scale (NaN: the next two instead) and -D
+  float *far_m, *far_l;          // [H][Tq]: a row's largest raw score, log2 of its sum relative to it
 };
 
 // The kernel's arguments, read again where they are used: for code that is hardly ever reached, so that its
@@ -789,11 +790,17 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_attnp_join(const Args
 }
 
 // ------------------------------------------------------------------ backward
+constexpr float kFarLse = 16384.f;
+
 // dQ: the forward's rows and tiles; per 32 keys S^T = K Q^T and dP^T = V dO^T (which starts at -D), then
 // dQ^T += K^T dS^T.  KW 2 as in the forward pass.  D = rowsum(dO O) is taken on the way from the rows that the kernel holds
 // anyway, and left for the dK / dV kernel: ndelta = -D, nlse = -lse / scale (-inf for a row that saw nothing, so that its
 // probabilities are 0), both [H][Tq].  The rounding of O to bf16 is off in D by |dO| |O| 2^-9, which counts where a row has
 // few keys (the share falls with the root of their number): there D = sum P dP is taken from the tile itself.
+// lse is rounded to fp32, and a probability is off by as much: 2^-20 |lse| with the roundings on the way of lse / scale.  Rows of
+// |lse| above 2^14, where that would pass bf16's own rounding, are done again at the end from their largest score and their sum,
+// which are left for the dK / dV kernel too; their nlse is NaN, so that a key which such a row sees becomes NaN there and is done
+// again.  (So is one that a NaN itself has spoilt.)
 // Bound as the forward pass: 8 x 4096 tokens of 16 heads 762 us, 1082 TF over the three products.  Three waves a SIMD; two
 // with the blocks interleaved as in the dK / dV kernel were slower (six images' step 91 against 84 us).
 template <bool CAUSAL, int KW>
@@ -842,13 +849,15 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
     df[t] = *reinterpret_cast<const bf16x8*>(dr + 16 * t + 8 * hh);
   }
   const float c = a.c;
-  const float lse = a.lse[(int64_t)(s.q0 + qi) * a.H + h], neg = lse == -INFINITY ? -INFINITY : -lse / a.scale, nl = neg * c;
+  const float lse = a.lse[(int64_t)(s.q0 + qi) * a.H + h];
+  const float neg = lse == -INFINITY ? -INFINITY : fabsf(lse) > kFarLse ? NAN : -lse / a.scale, nl = neg * c;
   float d = dot_row(a.out + (s.q0 + qi) * a.o_t + h * a.o_h, df, hh);
   __builtin_amdgcn_s_waitcnt(0xF70);
   __syncthreads();
 
   const Lanes ad(lds_addr(smem) + kw * 4096, lane);
   if (wave_on && nk_last <= kKV) {                   // D of rows with one tile of keys: sum P dP
+    const float rounded = d;
     d = 0.f;
 #pragma clang loop unroll(disable)
     for (int k2 = 0; 32 * k2 < nk_last; ++k2) {
@@ -864,6 +873,7 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
       for (int i = 0; i < 16; ++i) d += (i & 3) + 8 * (i >> 2) < lim ? __builtin_amdgcn_exp2f(fmaf(st[i], c, nl)) * dp[i] : 0.f;
     }
     d += __shfl_xor(d, 32);
+    if (nl != nl) d = rounded;
   }
   f32x16 nd, dq[2];
   for (int i = 0; i < 16; ++i) {
@@ -916,12 +926,35 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
     step(key0, std::integral_constant<int, 0>{});
     if (key0 + kKV < ke) step(key0 + kKV, std::integral_constant<int, 1>{});
   }
-  if (CAUSAL && __ballot(bad) != 0) {
+  const bool far = nl != nl;
+  if (wave_on && __ballot(bad != 0 || far) != 0) {
     for (int i = 0; i < 16; ++i) dq[0][i] = dq[1][i] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    ConstArgs* w = again();
+    const bf16_t* K = w->k + (s.k0 * w->k_t + hk * w->k_h);
+    const bf16_t* V = w->v + (s.k0 * w->v_t + hk * w->v_h);
+    if (__ballot(far) != 0) {
+#pragma clang loop unroll(disable)
+      for (int j = 0; j < nk_last; ++j) {
+        const float x = dot_row(K + j * w->k_t, qf, hh);
+        if (j < nk) {
+          const float m_new = fmaxf(m, x), alpha = m == m_new ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
+          l = fmaf(l, alpha, x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x - m_new) * c));
+          m = m_new;
+        }
+      }
+      l = log2f(l);
+      if (far && r < R && kw == 0 && hh == 0) {
+        const int64_t at = (int64_t)h * w->Tq + s.q0 + qi;
+        w->far_m[at] = m;
+        w->far_l[at] = l;
+      }
+    }
 #pragma clang loop unroll(disable)
     for (int j = 32 * kw; j < nk_last; j += KW == 2 && (j & 31) == 31 ? 33 : 1) {
-      const float x = dot_row(Kg + j * a.k_t, qf, hh), y = dot_row(Vg + j * a.v_t, df, hh);
-      if (j < nk) add_row(dq, __builtin_amdgcn_exp2f(fmaf(x, c, nl)) * (y + nd[0]), Kg + j * a.k_t, hh);
+      const float x = dot_row(K + j * w->k_t, qf, hh), y = dot_row(V + j * w->v_t, df, hh);
+      const float p = __builtin_amdgcn_exp2f(far ? fmaf(x - m, c, -l) : fmaf(x, c, nl));
+      if (j < nk) add_row(dq, p * (y + nd[0]), K + j * w->k_t, hh);
     }
   }
   if constexpr (KW == 2) {
@@ -1192,7 +1225,7 @@ __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
       for (; i1 < i_edge; i1 += RT) tile_step(i1, std::true_type{});
     for (; i1 < s.lq; i1 += RT) tile_step(i1, std::false_type{});
   }
-  if (CAUSAL && __ballot(bad) != 0) {
+  if (__ballot(bad != 0 || dv[0][0] != dv[0][0]) != 0) {
     for (int i = 0; i < 16; ++i) dk[0][i] = dk[1][i] = dv[0][i] = dv[1][i] = 0.f;
     ConstArgs* w = again();
     for (int g = g0; g < g1; ++g) {
@@ -1203,9 +1236,10 @@ __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
         const bf16_t* qr = w->q + (s.q0 + i) * w->q_t + h * w->q_h;
         const bf16_t* dr = w->dout + (s.q0 + i) * w->d_t + h * w->d_h;
         const float x = dot_row(qr, kf, hh), y = dot_row(dr, vf, hh);
-        if (i >= key - off) {
+        if (!CAUSAL || i >= key - off) {
           const int64_t st = (int64_t)h * w->Tq + s.q0 + i;
-          const float p = __builtin_amdgcn_exp2f((x + w->nlse[st]) * c);
+          const float nl = w->nlse[st];
+          const float p = __builtin_amdgcn_exp2f(nl != nl ? fmaf(x - w->far_m[st], c, -w->far_l[st]) : (x + nl) * c);
           add_row(dv, p, dr, hh);
           add_row(dk, p * (y + w->ndelta[st]), qr, hh);
         }
@@ -1434,9 +1468,9 @@ static int check_grad(const i2pc_attn_packed_grad_desc* g) {
 
 extern "C" size_t i2pc_attention_packed_backward_workspace_bytes(const i2pc_attn_packed_grad_desc* g) {
   if (check_grad(g) != I2PC_OK) return 0;
-  // -lse / scale and -D of every row, and the query heads' partial sums where they are split
+  // four statistics of every row, and the query heads' partial sums where they are split
   const attnp::KeySplit k = attnp::key_split(g->f);
-  return ((size_t)2 * g->f.total_q * g->f.heads + 3) / 4 * 4 * sizeof(float) +
+  return (size_t)4 * g->f.total_q * g->f.heads * sizeof(float) +
          (k.heads == 1 ? 0 : (size_t)k.heads * g->f.total_k * g->f.kv_heads * 128 * sizeof(float));
 }
 
@@ -1461,6 +1495,8 @@ extern "C" int i2pc_attention_packed_backward(const i2pc_attn_packed_grad_desc* 
   a.dv_t = attnp::pitch(g->dv_t, d.total_k), a.dv_h = g->dv_h;
   a.nlse = static_cast<float*>(workspace);
   a.ndelta = a.nlse + (size_t)a.Tq * a.H;
+  a.far_m = a.ndelta + (size_t)a.Tq * a.H;
+  a.far_l = a.far_m + (size_t)a.Tq * a.H;
   hipStream_t s = as_stream(stream);
   const dim3 block(256);
   if (a.Tq > 0) {
@@ -1474,7 +1510,7 @@ extern "C" int i2pc_attention_packed_backward(const i2pc_attn_packed_grad_desc* 
   if (a.Tk > 0) {
     const attnp::KeySplit k = attnp::key_split(d);
     a.nsplit = k.heads;
-    a.part_o = a.nlse + ((size_t)2 * a.Tq * a.H + 3) / 4 * 4;
+    a.part_o = a.nlse + (size_t)4 * a.Tq * a.H;
     const dim3 grid((uint32_t)(attnp::key_tiles(d, 32 * k.kw) * a.Hk * a.nsplit));
     if (k.kw == 4 && d.causal) hipLaunchKernelGGL((attnp::k_attnp_dkdv<true, 4>), grid, block, 0, s, a);
     else if (k.kw == 4) hipLaunchKernelGGL((attnp::k_attnp_dkdv<false, 4>), grid, block, 0, s, a);

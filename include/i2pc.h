@@ -617,7 +617,10 @@ size_t i2pc_attention_packed_workspace_bytes(const i2pc_attn_packed_desc* desc);
 int i2pc_attention_packed(const i2pc_attn_packed_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
 /* Gradients from dout and the forward's out and lse (desc as in the forward call, k_lens NULL): dq, dk, dv with the
  * shapes of q, k, v and their own strides.  Sums over the queries, and over the query heads that share a key head,
- * are fp32 in a fixed order.  Rows behind the last sequence are left as they were, or zero with zero_tail. */
+ * are fp32 in a fixed order.  Rows behind the last sequence are left as they were, or zero with zero_tail.
+ * The probabilities are taken again as exp(S - lse): lse's rounding leaves them up to 2^-20 |lse| off.  Rows whose |lse| is
+ * above 2^14 are done again from their largest score, and with them the keys that they see; so are keys whose gradients
+ * are NaN.  That is right for scores of any size, and slow. */
 typedef struct i2pc_attn_packed_grad_desc {
   i2pc_attn_packed_desc f;
   const void* dout;

@@ -162,3 +162,84 @@ def test_scores_beyond_the_largest_float():
         # above the largest float infinity; -inf is a query that sees no key
         over = r["lse"].abs() > 2.0 ** 128
         assert over.any() and ((lse.cpu() == INF) if sign < 0 else (lse.cpu() == -torch.finfo(torch.float32).max))[over].all()
+
+
+# ------------------------------------------------------------------ gradients
+# besides: lse of 2^13, below the size from which rows are done again, and 2^15, above it
+GRAD_KINDS = KINDS + [("offset", 8, 0.125), ("offset", 9, 0.125), ("-offset", 9, 0.125)]
+GRAD_IDS = [f"{n}-{e}-{math.log2(s):g}" for n, e, s in GRAD_KINDS]
+# Where a probability of the backward pass is exp(S - lse): lse's rounding, those of lse / scale, of its products with the scale and
+# log2(e), and the sums of the score's products that start at it
+ROUNDED = 2.0 ** -20
+
+
+def gradients(q, k, v, dout, ql, kl, causal, scale, **kw):
+    ops = _ops()
+    out, lse = ops.attention_packed(q, k, v, cu(ql), cu(kl), scale=scale, causal=causal)
+    got = ops.attention_packed_backward(dout, q, k, v, out, lse, cu(ql), cu(kl), scale=scale, causal=causal)
+    r = reference(q, k, v, ql, kl, causal, scale, dout, **kw)
+    return dict(zip(("dq", "dk", "dv"), got)), r
+
+
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("kind,e,scale", GRAD_KINDS, ids=GRAD_IDS)
+def test_gradients_of_large_scores(kind, e, scale, causal):
+    """Few tiles and many, heads of a group apart and together, rows of few keys."""
+    for ql, kl, heads, kv in (([200, 31], [200, 31], 2, 2), ([100, 3], [30, 400], 4, 2),
+                              ([577, 130, 577, 1, 577, 577, 577, 0, 577, 577], None, 26, 26), ([300] * 12, None, 24, 6)):
+        kl = kl or ql
+        q, k, v, dout = inputs(kind, e, sum(ql), sum(kl), heads, kv, heads + 1)
+        got, r = gradients(q, k, v, dout, ql, kl, causal, scale, rounded=ROUNDED if e == 8 else 0.0)
+        for n, t in got.items():
+            inside(t, r, n)
+
+
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+def test_gradients_of_large_and_small_scores_together(causal):
+    """Rows of either kind in a tile: what the one needs leaves the other's gradients right."""
+    q, k, v, dout = inputs("offset", 11, 180, 180, 4, 2, 9)
+    q[::3] = 0
+    got, r = gradients(q, k, v, dout, [180], [180], causal, 0.125)
+    for n, t in got.items():
+        inside(t, r, n)
+
+
+def test_gradients_of_large_scores_before_a_masked_nan():
+    ops = _ops()
+    q, k, v, dout = inputs("ties", 16, 180, 180, 2, 1, 5)
+    c = cu([180])
+    out, lse = ops.attention_packed(q, k, v, c, scale=0.125, causal=True)
+    r = reference(q, k, v, [180], [180], True, 0.125, dout)
+    q2, d2, k2, v2 = (t.clone() for t in (q, dout, k, v))
+    q2[20], d2[20], k2[150], v2[150] = (float("nan"),) * 4
+    _, dk, dv = ops.attention_packed_backward(d2, q2, k, v, out, lse, c, scale=0.125, causal=True)
+    inside(dk, r, "dk", slice(21, 180)), inside(dv, r, "dv", slice(21, 180))
+    dq, _, _ = ops.attention_packed_backward(dout, q, k2, v2, out, lse, c, scale=0.125, causal=True)
+    inside(dq, r, "dq", slice(0, 150))
+
+
+@pytest.mark.parametrize("size", [4.0, 8.0, 16.0])
+def test_gradients_of_peaked_scores(size):
+    """Ordinary values of some size: scores of some hundreds whose sums round, and an lse that rounds as much."""
+    gen = torch.Generator().manual_seed(4)
+    q, k, v, dout = ((s * torch.randn(195, 2, 64, generator=gen)).to(torch.bfloat16).cuda() for s in (size, size, 1.0, 1.0))
+    for causal in (False, True):
+        got, r = gradients(q, k, v, dout, [130, 65], [130, 65], causal, 0.125, rounded=ROUNDED,
+                           es=lambda mag: ES * (1 + mag))
+        for n, t in got.items():
+            inside(t, r, n)
+
+
+@pytest.mark.parametrize("rows", [5, 64, 150])
+def test_keys_of_scores_of_minus_infinity_have_no_gradient(rows):
+    """Nothing of theirs is in the output: dk and dv are 0, also where a tile ends behind the last query."""
+    ops = _ops()
+    gen = torch.Generator().manual_seed(4)
+    q, k, v, dout = (torch.randn(n, 2, 64, generator=gen).to(torch.bfloat16).cuda() for n in (rows, 100, 100, rows))
+    q = q.abs() + 0.5
+    k[:70, :, 0] = -INF
+    out, lse = ops.attention_packed(q, k, v, cu([rows]), cu([100]))
+    _, dk, dv = ops.attention_packed_backward(dout, q, k, v, out, lse, cu([rows]), cu([100]))
+    assert not dk[:70].any() and not dv[:70].any()
+    r = reference(q, k[70:], v[70:], [rows], [30], False, 0.125, dout, es=lambda mag: ES * (1 + mag))
+    inside(dk[70:], r, "dk"), inside(dv[70:], r, "dv")

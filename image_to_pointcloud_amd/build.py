@@ -56,8 +56,9 @@ def hipcc() -> str:
 def _flags(src: str) -> list[str]:
     f = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-result",
          "-fhip-fp32-correctly-rounded-divide-sqrt", "-I", os.path.join(ROOT, "include")]
-    # no packed FP32 instructions (v_pk_fma_f32 and the like): some of their forms have given wrong results
-    # on MI355X now and then; the host pass does not know the feature and says so
+    # no packed FP32 instructions (v_pk_fma_f32 and the like), which the compiler makes from ordinary float code: a precaution, no
+    # result here has shown a fault of theirs, and the default workload runs as fast without them.  The host pass does not know
+    # the feature and says so
     f += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     if src.endswith(".cpp"):
         f = ["-x", "hip"] + f

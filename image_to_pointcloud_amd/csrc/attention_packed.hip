@@ -30,7 +30,6 @@ using attn::kKV;
 using attn::kTileBytes;
 using attn::lds_addr;
 using attn::pack_bf16;
-using attn::tr_read;
 using attn::v4s;
 
 constexpr int kRows = 128;       // packed rows of a workgroup: 4 waves x 32
@@ -1323,7 +1322,11 @@ inline bool few_rows(const i2pc_attn_packed_desc& d) {
 }
 
 // Shares of the keys: one where the row tiles fill the chip, else so many that they do, of 256 keys at least on average
-// (few rows: 2048, since each share there is a partial row to join; an upper bound, a share may be empty).
+// (few rows: 2048; an upper bound, a share may be empty).  Each share of few rows is a partial row to join, and the join reads
+// them eight at a time.  Measured with shares of 2048 / 1024 / 512 keys at least, one new token, us (12.5 is the host's part):
+// one sequence of 131071 keys, 16 heads over 2: 17.8 / 19.6 / 21.7; four of 8192, 16 over 8: 19.9 / 20.2 / 23.0; but one of
+// 32768, 16 over 2: 17.1 / 12.4 / 12.6, and one of 8192, 16 over 8: 14.2 / 12.7 / 12.8.  Where the tiles fill the chip (64
+// sequences) the bound is not reached.
 inline int splits(const i2pc_attn_packed_desc& d) {
   if (d.total_k == 0) return 1;
   const bool few = few_rows(d);
@@ -1334,9 +1337,12 @@ inline int splits(const i2pc_attn_packed_desc& d) {
 }
 
 // The dK / dV call: keys of a workgroup / 32, and whether each query head of a group has workgroups of its own: where
-// 128-key tiles alone do not fill the chip's 512 places.  Measured backward, split / not (16 heads over 4, causal): 2 x 4096
-// tokens (268 tiles) 280 / 334 us, 4 x 4096 (532) 527 / 540, 16 x 1024 (580) 212 / 195, 64 x 512 (1284) 308 / 230 -- the
-// partial sums are 1 KiB a key and query head, written and read.
+// 128-key tiles alone do not fill the chip's 512 places.  The partial sums are 1 KiB a key and query head, written and read, so
+// short sequences lose by them at any number of tiles and long ones gain a little beyond 512 too; between them 512 costs least.
+// Measured backward, split / not, us (16 heads over 4, causal): tokens 4097, 2050, 1023, 130, 1 (248 tiles) 201 / 250, 2 x 4096
+// (264) 277 / 330, 3 x 4096 (396) 411 / 423, 12 x 1024 (432) 161 / 151, 7 x 2048 (476) 279 / 280; above 512, where it is not
+// split: 26 x 512 (520) 130 / 110, 4 x 4096 (528) 518 / 530, 8 x 2048 (544) 316 / 325, 16 x 1024 (576) 211 / 195, 8 x 4096
+// (1056) 1015 / 1034, 64 x 512 (1280) 307 / 226.
 struct KeySplit {
   int kw, heads;
 };

@@ -44,10 +44,7 @@ __device__ __forceinline__ float gelu_slope(float x, float tail, float ex) {
 }
 
 // x / 2^e within e4m3's range, which only infinities of a block of scale 2^127 leave
-template <bool ENDS>
-__device__ __forceinline__ float within(float v) {
-  return !ENDS || v != v ? v : fminf(fmaxf(v, -448.f), 448.f);
-}
+__device__ __forceinline__ float within(float v) { return v != v ? v : fminf(fmaxf(v, -448.f), 448.f); }
 
 __device__ __forceinline__ float lo16(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi16(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
@@ -77,7 +74,7 @@ __global__ __launch_bounds__(256) void k_gelu_keep(const uint16_t* x, int64_t ld
   for (int j = 0; j < 8; ++j) {
     float ex;
     const float tail = normal_tail(v[j], ex);
-    q[j] = within<false>(v[j] * mul);
+    q[j] = v[j] * mul;
     g[j] = gelu<false>(v[j], tail);
   }
   if (__builtin_expect(am == INFINITY, 0)) {
@@ -86,7 +83,7 @@ __global__ __launch_bounds__(256) void k_gelu_keep(const uint16_t* x, int64_t ld
     for (int j = 0; j < 8; ++j) {
       float ex;
       const float tail = normal_tail(v[j], ex);
-      q[j] = within<true>(v[j] * mul);
+      q[j] = within(v[j] * mul);
       g[j] = gelu<true>(v[j], tail);
     }
   }

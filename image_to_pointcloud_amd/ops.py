@@ -850,6 +850,8 @@ def maxpool3s2(x, out=None):
 
 
 # ------------------------------------------------------------------ training steps of the encoder's operators
+# Forward and backward are calls of their own, here and for packed attention below: results carry no gradient function, whether
+# an operand requires a gradient or not.
 _lib.register("i2pc_layernorm_train", ctypes.c_int, [c_void_p, ctypes.c_int, c_int64, c_void_p, c_void_p, ctypes.c_float,
                                                      ctypes.c_int, ctypes.c_int, c_void_p, c_int64, c_void_p, c_void_p])
 _lib.register("i2pc_layernorm_backward_workspace_bytes", ctypes.c_size_t, [ctypes.c_int, ctypes.c_int])
@@ -927,7 +929,8 @@ def _launch(label, nbytes, name, at, *args):
 def layernorm_train(x, gamma, beta, eps, out=None, stats=None):
     """LayerNorm of the rows of x [rows, dim] (fp32 or bf16, any row pitch and alignment; dim <= 8192) for a
     training step: (y, stats) with y bf16 [rows, dim] and stats fp32 [rows, 2] = each row's (mean, 1 / std),
-    which layernorm_backward reads.  gamma, beta: fp32 [dim].  Rows and statistics are held in fp32; out may not be x."""
+    which layernorm_backward reads.  gamma, beta: fp32 [dim].  Rows and statistics are held in fp32; out may not be x.
+    The results carry no gradient function: autograd does not see the call."""
     torch = _torch()
     f32, bf = torch.float32, torch.bfloat16
     rows, dim, pitch = _rows_dim(x, "x", (f32, bf))
@@ -994,7 +997,8 @@ def layernorm_backward(dy, x, stats, gamma, add=None, dx=None, dgamma=None, dbet
 
 def gelu_fp8(x, out=None, kept=None):
     """GELU (the erf form) of bf16 rows x [rows, dim], dim % 32 == 0: (y, kept) with y bf16 and kept the Fp8 rows
-    of x (quant_fp8's block rule) that gelu_fp8_backward works from: 1.03 bytes a value instead of two.  out may be x."""
+    of x (quant_fp8's block rule) that gelu_fp8_backward works from: 1.03 bytes a value instead of two.  out may be x.
+    The results carry no gradient function: autograd does not see the call."""
     torch = _torch()
     bf = torch.bfloat16
     rows, dim, pitch = _rows_dim(x, "x", (bf,))
@@ -1125,7 +1129,8 @@ def attention_packed(q, k, v, cu_q, cu_k=None, k_lens=None, scale=None, causal=F
     runs.  causal: query i of lq sees the keys j <= i + lk - lq of lk.  scale defaults to 1 / 8.
     out bf16 [total_q, heads, 64]; lse fp32 [total_q, heads] = log(sum(exp(scores))).  A query that sees no key has
     out 0, lse -inf.  Rows behind the last sequence keep what a given `out` / `lse` holds (give both, or neither), and
-    are 0 / -inf in new ones.  No output may overlap an input or itself.
+    are 0 / -inf in new ones.  No output may overlap an input or itself.  The results carry no gradient function:
+    attention_packed_backward is a call of its own, autograd does not see either.
     """
     torch = _torch()
     if (out is None) != (lse is None):
@@ -1152,7 +1157,8 @@ def attention_packed_backward(dout, q, k, v, out, lse, cu_q, cu_k=None, scale=No
     """Gradients of attention_packed (i2pc_attention_packed_backward): (dq, dk, dv), bf16, from dout bf16 [total_q,
     heads, 64], the forward call's operands and its (out, lse).  dk, dv are summed over the query heads that share a key
     head; all sums are fp32 in a fixed order.  Rows behind the last sequence keep what a given dq / dk / dv holds (give all
-    three, or none), and are 0 in new ones."""
+    three, or none), and are 0 in new ones.  Scores may have any size; rows whose |lse| is above 2^14, and keys whose gradients
+    are NaN, are done again one key or query at a time, which is slow."""
     torch = _torch()
     bf = torch.bfloat16
     fresh = dq is None

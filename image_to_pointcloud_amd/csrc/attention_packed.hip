@@ -346,13 +346,13 @@ struct Rows {
 
 // 32 keys (at bytes atK, atV behind the addresses' tile) for 32 rows: p = 2^(c s - c m), one FMA and one exponential a
 // score.  m moves only when a probability could pass 2^8 (harmless for the bf16 operand and the fp32 sums), so the usual
-// block has no maximum and no rescale.  `first`: the rows' first block, which sets m.  left: how many of the block's keys
+// block has no maximum and no rescale.  first: the rows' first block, which sets m (a bool, or its constant).  left: how many of the block's keys
 // the lane's row sees; partial (uniform): not all of them for some row of the wave.
 // c m is rounded and c s within the FMA is not: the exponent of s = m is off by up to 2^-25 |c m|, the same for a row's every
 // score, which the sum takes out again -- until it leaves the exponential's range.  Rows whose |c m| is above 2^12 (`far`) take
 // 2^(c (s - m)) instead, with their maximum anew in each block.
-template <bool CAUSAL>
-__device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const Lanes& ad, uint32_t atK, uint32_t atV, bool first,
+template <bool CAUSAL, class First>
+__device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const Lanes& ad, uint32_t atK, uint32_t atV, First first,
                                        bool partial, int left, float c, int hh) {
   constexpr float kThresh = 256.f, kFar = 4096.f;
   bf16x8 kf[4];
@@ -527,24 +527,25 @@ __global__ __launch_bounds__(256, 4) void k_attnp_fwd(const Args a) {
   Rows w;
   w.clear();
   const Lanes ad(lds_addr(smem) + kw * 4096, lane);
-  auto step = [&](int key0, auto buffer) {
+  auto step = [&](int key0, auto buffer, auto first) {
     constexpr int cur = decltype(buffer)::value;
     if (key0 + kKV < ke) stage(cur ^ 1, key0 + kKV);
     if (wave_on) {
-#pragma unroll
-      for (int k2 = 0; k2 < 2 / KW; ++k2) {
-        const int key = key0 + 32 * (k2 + kw);
-        if (key >= nk_last) break;                   // no row of the wave sees these keys
-        attend<CAUSAL>(w, qf, ad, cur * 2 * kTileBytes + k2 * 4096, (cur * 2 + 1) * kTileBytes + k2 * 4096, key == ks + 32 * kw,
-                       key + 32 > nk_first, nk - key, c, hh);
+      const int key = key0 + 32 * kw;
+      constexpr uint32_t atK = cur * 2 * kTileBytes, atV = atK + kTileBytes;
+      if (key < nk_last) {                           // some row of the wave sees these keys
+        attend<CAUSAL>(w, qf, ad, atK, atV, first, key + 32 > nk_first, nk - key, c, hh);
+        if (KW == 1 && key + 32 < nk_last)
+          attend<CAUSAL>(w, qf, ad, atK + 4096, atV + 4096, std::false_type{}, key + 64 > nk_first, nk - key - 32, c, hh);
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the next tile landed (this wave's part)
     __syncthreads();                                     // ... and every wave's
   };
-  for (int key0 = ks; key0 < ke; key0 += 2 * kKV) {
-    step(key0, std::integral_constant<int, 0>{});
-    if (key0 + kKV < ke) step(key0 + kKV, std::integral_constant<int, 1>{});
+  if (ks < ke) step(ks, std::integral_constant<int, 0>{}, std::true_type{});
+  for (int key0 = ks + kKV; key0 < ke; key0 += 2 * kKV) {
+    step(key0, std::integral_constant<int, 1>{}, std::false_type{});
+    if (key0 + kKV < ke) step(key0 + kKV, std::integral_constant<int, 0>{}, std::false_type{});
   }
   if (CAUSAL && __ballot(w.bad) != 0)
     attend_again(w, qf, Kg, a.k_t, Vg, a.v_t, ks + 32 * kw, min(ke, nk_last), KW == 2 ? 33 : 1, nk, c, hh);

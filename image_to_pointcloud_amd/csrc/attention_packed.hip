@@ -461,9 +461,11 @@ __device__ __forceinline__ void attend_again(Rows& w, const bf16x8 (&qf)[4], con
 // registers, which then are the B operand of O^T += V^T P^T.  K and V tiles of 64 keys go through LDS by
 // LDS-DMA, double-buffered.  KW 2: waves 2, 3 hold the rows of waves 0, 1 again and take the second 32 keys of each tile,
 // and the two states are joined at the end: twice the workgroups, of half the length.
-// Bound by the exponentials and the products together: 8 x 4096 tokens of 16 heads take 546 us (1006 TF), the vector unit 76 %
-// busy and the matrix unit 55 %, at the 1.6 GHz that the power limit leaves.  Four waves a SIMD: eight-wave workgroups of
-// 256 rows were slower (causal prompts 118 against 107 us), as were raised wave priorities.
+// Bound by the exponentials and the products together: 8 x 4096 tokens of 16 heads take 585 us in the kernel trace (940 TF; calls
+// one after the other 561, 980 TF), the vector unit 77 % busy and the matrix unit 58 %, at the 1.6 to 1.7 GHz that the power limit
+// leaves.  Four waves a SIMD: eight-wave workgroups of 256 rows were slower (causal prompts 118 against 107 us), as were raised
+// wave priorities.  The first tile is outside the loop: with its test for a row's first block inside, the loop had no registers
+// for the addresses of both buffers (588 us where it is 575 now).
 template <bool CAUSAL, bool SPLIT, int KW>
 __global__ __launch_bounds__(256, 4) void k_attnp_fwd(const Args a) {
   constexpr int kWgRows = kRows / KW;
@@ -601,8 +603,8 @@ __global__ __launch_bounds__(256, 4) void k_attnp_fwd(const Args a) {
 // Few rows (new tokens over a cache): 32 packed rows of one key head a workgroup, whose four waves take every fourth
 // block of 32 keys of a share, each with its own two LDS buffers and no barrier until the end -- what counts is how many
 // bytes of K and V are on their way, 8 KiB a wave.  A share is lk / nsplit keys, 256 at least.
-// Bound by HBM: one token of 64 sequences over 97 to 8096 keys, 16 heads over 4: 56 us and 5 us for the join (4.5 TB/s; a copy
-// reaches 4.9); one token over 131071 keys, 16 heads over 2: 14 and 4 us.
+// Bound by HBM: one token of 64 sequences over 97 to 8096 keys, 16 heads over 4: 58 us and 5 us for the join (4.4 TB/s; a copy
+// reaches 4.9); one token over 131071 keys, 16 heads over 2: 15 and 4 us.
 constexpr int kFew = 32;
 constexpr int kFewBlock = 32 * 128;                  // bytes of 32 keys' K (or V)
 template <bool CAUSAL>
@@ -801,7 +803,7 @@ constexpr float kFarLse = 16384.f;
 // |lse| above 2^14, where that would pass bf16's own rounding, are done again at the end from their largest score and their sum,
 // which are left for the dK / dV kernel too; their nlse is NaN, so that a key which such a row sees becomes NaN there and is done
 // again.  (So is one that a NaN itself has spoilt.)
-// Bound as the forward pass: 8 x 4096 tokens of 16 heads 762 us, 1082 TF over the three products.  Three waves a SIMD; two
+// Bound as the forward pass: 8 x 4096 tokens of 16 heads 795 us, 1038 TF over the three products.  Three waves a SIMD; two
 // with the blocks interleaved as in the dK / dV kernel were slower (six images' step 91 against 84 us).
 template <bool CAUSAL, int KW>
 __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
@@ -983,9 +985,9 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
 // dK^T += Q^T dS.  Tiles are of RT = 256 / KW rows: with KW 4 every wave has 32 keys and takes both 32-row blocks of a tile;
 // with KW 2 waves 2, 3 hold the keys of waves 0, 1 again, a wave takes two of the four blocks and the sums are added at the
 // end.  A wave's two blocks are independent: while one's exponentials are on the vector unit the other's products are on
-// the matrix unit.  8 x 4096 tokens of 16 heads: 1035 us, 1062 TF over the four products (851 cycles a block, 512 of them
+// the matrix unit.  8 x 4096 tokens of 16 heads: 1090 us, 1009 TF over the four products (847 cycles a block, 512 of them
 // on the matrix unit; the blocks interleaved and the addresses out of the loops took the whole backward pass from 1777 to
-// 1693 us).
+// 1693 us on one box; 1709 to 1755 on others).
 template <bool CAUSAL, int KW>
 __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
   constexpr int RT = 256 / KW, kRowBytes = RT * 128;

@@ -11,8 +11,8 @@
 // same read: a wave keeps the partial sums of its columns in registers over all the rows it takes, a
 // workgroup adds its waves' through LDS and writes one partial row, and k_lnt_cols adds the partial rows
 // -- fixed assignment and order, so the result does not change from run to run (no atomics).
-// Measured: 18464 x 1024 fp32 forward 24.5 us (4.6 TB/s), backward with add 54 us (4.9 TB/s; a copy of 2 GiB
-// reaches 4.9), the partial rows' sum 3 us of it; 4099 x 1111 bf16 8.1 and 16.7 us (its rows start at odd
+// Measured, calls one after the other: 18464 x 1024 fp32 forward 24.6 us (4.6 TB/s), backward with add 54 us (4.9 TB/s; a copy
+// of 2 GiB reaches 4.9), the partial rows' sum 5 us of it; 4099 x 1111 bf16 7.2 and 17.1 us (its rows start at odd
 // addresses); 5 x 384: the launches.
 #include "common.h"
 

@@ -793,6 +793,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_attnp_join(const Args
 
 // ------------------------------------------------------------------ backward
 constexpr float kFarLse = 16384.f;
+constexpr uint32_t kFarMark = 0x7fc0fa11u;           // a NaN of its own, for the nlse of such rows
+__device__ __forceinline__ bool is_far(float lse) { return fabsf(lse) > kFarLse && lse != -INFINITY; }
 
 // dQ: the forward's rows and tiles; per 32 keys S^T = K Q^T and dP^T = V dO^T (which starts at -D), then
 // dQ^T += K^T dS^T.  KW 2 as in the forward pass.  D = rowsum(dO O) is taken on the way from the rows that the kernel holds
@@ -801,8 +803,8 @@ constexpr float kFarLse = 16384.f;
 // few keys (the share falls with the root of their number): there D = sum P dP is taken from the tile itself.
 // lse is rounded to fp32, and a probability is off by as much: 2^-20 |lse| with the roundings on the way of lse / scale.  Rows of
 // |lse| above 2^14, where that would pass bf16's own rounding, are done again at the end from their largest score and their sum,
-// which are left for the dK / dV kernel too; their nlse is NaN, so that a key which such a row sees becomes NaN there and is done
-// again.  (So is one that a NaN itself has spoilt.)
+// which are left for the dK / dV kernel too; their nlse is a NaN of its own, so that a key which such a row sees becomes NaN there
+// and is done again.
 // Bound as the forward pass: 8 x 4096 tokens of 16 heads 795 us, 1038 TF over the three products.  Three waves a SIMD; two
 // with the blocks interleaved as in the dK / dV kernel were slower (six images' step 91 against 84 us).
 template <bool CAUSAL, int KW>
@@ -852,7 +854,8 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
   }
   const float c = a.c;
   const float lse = a.lse[(int64_t)(s.q0 + qi) * a.H + h];
-  const float neg = lse == -INFINITY ? -INFINITY : fabsf(lse) > kFarLse ? NAN : -lse / a.scale, nl = neg * c;
+  const float neg = lse == -INFINITY ? -INFINITY : is_far(lse) ? __uint_as_float(kFarMark) : lse != lse ? NAN : -lse / a.scale;
+  const float nl = neg * c;
   float d = dot_row(a.out + (s.q0 + qi) * a.o_t + h * a.o_h, df, hh);
   __builtin_amdgcn_s_waitcnt(0xF70);
   __syncthreads();
@@ -928,11 +931,11 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
     step(key0, std::integral_constant<int, 0>{});
     if (key0 + kKV < ke) step(key0 + kKV, std::integral_constant<int, 1>{});
   }
-  const bool far = nl != nl;
+  ConstArgs* w = again();
+  const bool far = wave_on && __ballot(nl != nl) != 0 && is_far(w->lse[(int64_t)(s.q0 + qi) * w->H + h]);
   if (wave_on && __ballot(bad != 0 || far) != 0) {
     for (int i = 0; i < 16; ++i) dq[0][i] = dq[1][i] = 0.f;
     float m = -INFINITY, l = 0.f;
-    ConstArgs* w = again();
     const bf16_t* K = w->k + (s.k0 * w->k_t + hk * w->k_h);
     const bf16_t* V = w->v + (s.k0 * w->v_t + hk * w->v_h);
     if (__ballot(far) != 0) {
@@ -1227,7 +1230,29 @@ __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
       for (; i1 < i_edge; i1 += RT) tile_step(i1, std::true_type{});
     for (; i1 < s.lq; i1 += RT) tile_step(i1, std::false_type{});
   }
-  if (__ballot(bad != 0 || dv[0][0] != dv[0][0]) != 0) {
+  const bool nan = dv[0][0] != dv[0][0];
+  if (__ballot(nan) != 0) {
+    // Done again: keys that a far row has made NaN, and those of an infinity, which the rows of zeros behind the last query have
+    // (not those that a NaN has spoilt: it would again)
+    bool inf = false, real = true;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = (float)kf[t][j];
+        inf |= fabsf(x) == INFINITY;
+        real &= x == x;
+      }
+    inf |= __shfl_xor((int)inf, 32) != 0;
+    real &= __shfl_xor((int)real, 32) != 0;
+    bad |= nan && inf && real;
+    ConstArgs* w = again();
+    for (int g = g0; g < g1; ++g) {
+      const uint32_t* nl = reinterpret_cast<const uint32_t*>(w->nlse + (int64_t)(hk * w->G + g) * w->Tq + s.q0);
+      for (int i = i_first + lane; i < s.lq; i += 64) bad |= nl[i] == kFarMark;
+    }
+  }
+  if (__ballot(bad != 0) != 0) {
     for (int i = 0; i < 16; ++i) dk[0][i] = dk[1][i] = dv[0][i] = dv[1][i] = 0.f;
     ConstArgs* w = again();
     for (int g = g0; g < g1; ++g) {
@@ -1241,7 +1266,7 @@ __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
         if (!CAUSAL || i >= key - off) {
           const int64_t st = (int64_t)h * w->Tq + s.q0 + i;
           const float nl = w->nlse[st];
-          const float p = __builtin_amdgcn_exp2f(nl != nl ? fmaf(x - w->far_m[st], c, -w->far_l[st]) : (x + nl) * c);
+          const float p = __builtin_amdgcn_exp2f(__float_as_uint(nl) == kFarMark ? fmaf(x - w->far_m[st], c, -w->far_l[st]) : (x + nl) * c);
           add_row(dv, p, dr, hh);
           add_row(dk, p * (y + w->ndelta[st]), qr, hh);
         }

@@ -1157,8 +1157,8 @@ def attention_packed_backward(dout, q, k, v, out, lse, cu_q, cu_k=None, scale=No
     """Gradients of attention_packed (i2pc_attention_packed_backward): (dq, dk, dv), bf16, from dout bf16 [total_q,
     heads, 64], the forward call's operands and its (out, lse).  dk, dv are summed over the query heads that share a key
     head; all sums are fp32 in a fixed order.  Rows behind the last sequence keep what a given dq / dk / dv holds (give all
-    three, or none), and are 0 in new ones.  Scores may have any size; rows whose |lse| is above 2^14, and keys whose gradients
-    are NaN, are done again one key or query at a time, which is slow."""
+    three, or none), and are 0 in new ones.  Scores may have any size; rows whose |lse| is above 2^14, and the keys that
+    they see, are done again one key or query at a time, which is slow."""
     torch = _torch()
     bf = torch.bfloat16
     fresh = dq is None

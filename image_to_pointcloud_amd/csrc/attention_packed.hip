@@ -346,8 +346,8 @@ struct Rows {
 
 // 32 keys (at bytes atK, atV behind the addresses' tile) for 32 rows: p = 2^(c s - c m), one FMA and one exponential a
 // score.  m moves only when a probability could pass 2^8 (harmless for the bf16 operand and the fp32 sums), so the usual
-// block has no maximum and no rescale.  first: the rows' first block, which sets m (a bool, or its constant).  left: how many of the block's keys
-// the lane's row sees; partial (uniform): not all of them for some row of the wave.
+// block has no maximum and no rescale.  first: the rows' first block, which sets m (a bool, or its constant).  left: how many of
+// the block's keys the lane's row sees; partial (uniform): not all of them for some row of the wave.
 // c m is rounded and c s within the FMA is not: the exponent of s = m is off by up to 2^-25 |c m|, the same for a row's every
 // score, which the sum takes out again -- until it leaves the exponential's range.  Rows whose |c m| is above 2^12 (`far`) take
 // 2^(c (s - m)) instead, with their maximum anew in each block.
@@ -394,10 +394,8 @@ __device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const Lan
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[i]);
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
     mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-    // a row that sees nothing here keeps its reference; one whose first 32 scores are all -inf gets one below the others that is
-    // finite, and times c too
-    const float low = -0x1p126f * __builtin_amdgcn_rcpf(fmaxf(c, 1.f));
-    const float m_new = first ? (mx == -INFINITY ? low : mx) : fmaxf(mx, w.m);
+    // a row that sees nothing here keeps its reference; one that has met no score but -inf has the lowest finite one (and is far)
+    const float m_new = fmaxf(mx, first ? -FLT_MAX : w.m);
     if (!first) {
       const float alpha = __builtin_amdgcn_exp2f((w.m - m_new) * c);
       w.l *= alpha;
@@ -409,7 +407,7 @@ __device__ __forceinline__ void attend(Rows& w, const bf16x8 (&qf)[4], const Lan
     }
     w.m = m_new;
     float mc = m_new * c;
-    w.far = __ballot(fabsf(mc) > kFar && m_new != low) != 0;
+    w.far = __ballot(fabsf(mc) > kFar) != 0;
     if (__builtin_expect(w.far, 0)) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) st[i] -= m_new;
@@ -990,7 +988,7 @@ __global__ __launch_bounds__(256, 3) void k_attnp_dq(const Args a) {
 // end.  A wave's two blocks are independent: while one's exponentials are on the vector unit the other's products are on
 // the matrix unit.  8 x 4096 tokens of 16 heads: 1090 us, 1009 TF over the four products (847 cycles a block, 512 of them
 // on the matrix unit; the blocks interleaved and the addresses out of the loops took the whole backward pass from 1777 to
-// 1693 us on one box; 1709 to 1755 on others).
+// 1693 us on one card; 1709 to 1755 on others).
 template <bool CAUSAL, int KW>
 __global__ __launch_bounds__(256, 2) void k_attnp_dkdv(const Args a) {
   constexpr int RT = 256 / KW, kRowBytes = RT * 128;

@@ -164,6 +164,22 @@ def test_scores_beyond_the_largest_float():
         assert over.any() and ((lse.cpu() == INF) if sign < 0 else (lse.cpu() == -torch.finfo(torch.float32).max))[over].all()
 
 
+@pytest.mark.parametrize("rows,heads", [(1, 8), (70, 2), (577, 40)])
+def test_scores_beyond_the_largest_float_behind_minus_infinity(rows, heads):
+    """A row whose first scores are all -inf takes the others as they are, however low."""
+    ops = _ops()
+    q, k, v, _ = inputs("low", 32, rows, 100, heads, heads, 3)
+    k[:40, :, 0] = -INF
+    for causal in (False, True):
+        if causal and rows > 100:
+            continue
+        r = reference(q, k[40:], v[40:], [rows], [60], causal, 2.0 ** 64)
+        out, lse = ops.attention_packed(q, k, v, cu([rows]), cu([100]), scale=2.0 ** 64, causal=causal)
+        seen = slice(max(0, rows - 60) if causal else 0, rows)
+        inside(out, r, "out", seen)
+        assert (lse.cpu()[seen] < -(2.0 ** 126)).all() and torch.isfinite(lse.cpu()[seen]).all()
+
+
 # ------------------------------------------------------------------ gradients
 # besides: lse of 2^13, below the size from which rows are done again, and 2^15, above it
 GRAD_KINDS = KINDS + [("offset", 8, 0.125), ("offset", 9, 0.125), ("-offset", 9, 0.125)]

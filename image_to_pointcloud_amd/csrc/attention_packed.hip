@@ -463,7 +463,7 @@ __device__ __forceinline__ void attend_again(Rows& w, const bf16x8 (&qf)[4], con
 // one after the other 561, 980 TF), the vector unit 77 % busy and the matrix unit 58 %, at the 1.6 to 1.7 GHz that the power limit
 // leaves.  Four waves a SIMD: eight-wave workgroups of 256 rows were slower (causal prompts 118 against 107 us), as were raised
 // wave priorities.  The first tile is outside the loop: with its test for a row's first block inside, the loop had no registers
-// for the addresses of both buffers (588 us where it is 575 now).
+// for the addresses of both buffers (2 % slower).
 template <bool CAUSAL, bool SPLIT, int KW>
 __global__ __launch_bounds__(256, 4) void k_attnp_fwd(const Args a) {
   constexpr int kWgRows = kRows / KW;

@@ -707,3 +707,19 @@ def test_a_half_without_a_probability_beside_a_masked_nan():
     inside(out[16:74], ref["out"][:58], ref["out_b"][:58], "out")
     inside(lse[16:], ref["lse"], ref["lse_b"], "lse")
     assert out[74:].isnan().all()
+
+
+@pytest.mark.parametrize("prompt", [700, 1500])
+def test_prompts_and_single_tokens_in_one_pack(prompt):
+    """Single tokens over slabs beside a prompt: a short one leaves their keys in shares, a long one fills the chip and does not."""
+    ops = _ops()
+    B, slab = 40, 3000
+    ql, lens = [1] * B + [prompt], [1 + i * 2654435761 % 2999 for i in range(B)] + [prompt + 100]
+    q, k, v, _ = make(ql, [slab] * (B + 1), 16, 4, seed=prompt)
+    for b, n in enumerate(lens):
+        k[b * slab + n:(b + 1) * slab] = float("nan")
+        v[b * slab + n:(b + 1) * slab] = float("inf")
+    out, lse = ops.attention_packed(q, k, v, cu(ql), cu([slab] * (B + 1)), k_lens=torch.tensor(lens, dtype=torch.int32).cuda(), causal=True)
+    ref = reference(q, k, v, ql, lens, True, 0.125, starts=[b * slab for b in range(B + 1)])
+    inside(out, ref["out"], ref["out_b"], "out")
+    inside(lse, ref["lse"], ref["lse_b"], "lse")
